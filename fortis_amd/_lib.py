@@ -70,6 +70,9 @@ PROTOTYPES = {
     "fortis_plan_concat_copy": (i, [vp, i, i, l, l, l, l]),
     "fortis_plan_conv3d": (i, [vp, i, i, i, vp, vp, l, l, l, l, l, l, l, i, f]),
     "fortis_plan_permute": (i, [vp, i, i, l, l, i]),
+    "fortis_plan_group_norm": (i, [vp, i, i, vp, vp, f, l, l, l, l, i, i, f]),
+    "fortis_plan_linear_adapters": (i, [vp, i, i, i, vp, vp, vp, vp, vp, l, l, l, l, l, i, f]),
+    "fortis_plan_recurrence": (i, [vp, i, i, i, i, i, l, l, l, i, i]),
     "fortis_plan_finalize": (i, [vp, i, i]), "fortis_plan_run": (None, [vp]),
     "fortis_plan_tensor_ptr": (vp, [vp, i]), "fortis_plan_num_kernels": (i, [vp]),
     # step + entries
@@ -78,7 +81,7 @@ PROTOTYPES = {
     "mlp_upload": (None, [vp]), "mlp_forward_dev": (None, []), "mlp_download": (None, [vp]),
     "mlp_forward": (None, [vp, vp]), "mlp_forward_batched": (None, [vp, vp]),
     "fortis_pack": (None, [vp, i]), "fortis_unpack": (None, [vp, i]),
-    "fortis_model_input": (vp, []), "fortis_model_output": (vp, []), "fortis_begin": (None, [i]),
+    "fortis_model_input": (vp, []), "fortis_model_output": (vp, []), "fortis_model_tensor": (vp, [i]), "fortis_begin": (None, [i]),
     # stencil
     "fortis_stencil_check": (i, [C.POINTER(Stencil)]),
     "fortis_stencil_route": (i, [C.POINTER(Stencil)]),

@@ -103,10 +103,54 @@ void fortis_launch_scatter_generic(const fortis_stencil_t& t, const int* dcells,
 void fortis_launch_scale(const float* src, float* dst, const float* vec, long rows, long n, int divide, hipStream_t s);
 void fortis_launch_mask_relu(const float* src, float* dst, long rows, long n, long tail, hipStream_t s);
 void fortis_launch_zero(float* dst, long n, hipStream_t s);
+void fortis_launch_fill_int(int* dst, int v, long n, hipStream_t s);
 void fortis_launch_boundary_pre(const void* A, float* X, long NI, long NK, const void* mean, const void* vmax,
                                 const void* vmin, int host_esz, hipStream_t s);
 void fortis_launch_boundary_post(const float* Y, void* B, long NI, long NK, const void* scale, int host_esz, hipStream_t s);
 void fortis_launch_permute(const float* src, float* dst, long C, long S, int to_channels_first, hipStream_t s);
+
+// ---- group normalisation (norm.hip) --------------------------------------------------------
+struct NormDesc {
+    long NB, S, C, G;
+    int first;                  // channels first
+    float eps;
+    int act;
+    float alpha;
+    const float *gamma, *beta;  // device, length C, or null
+};
+long fortis_norm_workspace(const NormDesc& d);          // bytes fortis_launch_group_norm needs at ws
+void fortis_launch_group_norm(const NormDesc& d, const float* x, float* y, void* ws, hipStream_t s);
+
+// ---- projection with an adapter per row (adapters.hip) -------------------------------------
+struct AdaptDesc {
+    long K, N, nadapt, rank;
+    int act;
+    float alpha;
+    const float *W, *bias;      // device; bias may be null
+    const float *A, *U, *scale; // device: [nadapt][rank][K], [nadapt][N][rank], [nadapt]
+};
+long fortis_adapters_workspace(const AdaptDesc& d, long B);
+void fortis_launch_linear_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s);
+
+// ---- gated linear recurrence (recurrence.hip) ----------------------------------------------
+struct RecurDesc {
+    long nseq, len, ch;
+    int time_major, reverse;
+};
+long fortis_recurrence_workspace(const RecurDesc& d);
+void fortis_launch_recurrence(const RecurDesc& d, const float* src, float* dst, const float* h_in, float* h_out, const int* lengths,
+                              void* ws, hipStream_t s);
+
+// SiLU as v * sigmoid(v) with the library's exp: v / (1 + exp(-v)) is -0 for v far below zero and v far above it.
+#ifdef __HIPCC__
+__device__ __forceinline__ float fortis_act_silu(float v, int act, float alpha)
+{
+    if (act == FORTIS_ACT_RELU) return v > 0.f ? v : 0.f;
+    if (act == FORTIS_ACT_LEAKY) return v > 0.f ? v : alpha * v;
+    if (act == FORTIS_ACT_SILU) return v / (1.f + expf(-v));
+    return v;
+}
+#endif
 
 // ---- convolution family (conv.hip) ---------------------------------------------------------
 // Workgroups are dealt to the chip's eight XCDs round-robin (workgroup b of a row of the grid runs on XCD

@@ -44,6 +44,17 @@ void fortis_launch_zero(float* dst, long n, hipStream_t s)
     hipLaunchKernelGGL(zero_kernel, dim3((unsigned)cdiv(n, EW_THREADS)), dim3(EW_THREADS), 0, s, dst, n);
     HIP_OK(hipGetLastError());
 }
+__global__ void fill_int_kernel(int* __restrict__ dst, int v, long n)
+{
+    const long idx = (long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (idx < n) dst[idx] = v;
+}
+void fortis_launch_fill_int(int* dst, int v, long n, hipStream_t s)
+{
+    if (n <= 0) return;
+    hipLaunchKernelGGL(fill_int_kernel, dim3((unsigned)cdiv(n, EW_THREADS)), dim3(EW_THREADS), 0, s, dst, v, n);
+    HIP_OK(hipGetLastError());
+}
 void fortis_launch_mask_relu(const float* src, float* dst, long rows, long n, long tail, hipStream_t s)
 {
     const long total = rows * n;

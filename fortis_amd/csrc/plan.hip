@@ -11,11 +11,12 @@
 #include "common.h"
 
 enum OpKind { OP_LINEAR, OP_SCALE, OP_MASK_RELU, OP_PRE, OP_POST, OP_CONV2D, OP_CONVT2D, OP_MAXPOOL, OP_UPSAMPLE,
-              OP_CONCAT, OP_CONV3D, OP_PERMUTE };
+              OP_CONCAT, OP_CONV3D, OP_PERMUTE, OP_NORM, OP_ADAPT, OP_RECUR };
 
 struct Op {
     OpKind kind;
     int src = -1, dst = -1, res = -1;
+    int side = -1, h_in = -1, h_out = -1;     // adapters: index; recurrence: lengths and the two states
     long B = 0, K = 0, N = 0;                 // linear; rows/n for scale & mask
     int act = 0; float alpha = 0.f;
     int flag = 0;                             // scale: divide; permute: to_channels_first; boundary: host_esz
@@ -29,7 +30,7 @@ struct Op {
 };
 
 enum ExecKind { EX_CHAIN, EX_GEMM, EX_SCALE, EX_MASK, EX_PRE, EX_POST, EX_CONV2D, EX_CONVT2D, EX_MAXPOOL, EX_UPSAMPLE,
-                EX_CONCAT, EX_CONV3D, EX_PERMUTE };
+                EX_CONCAT, EX_CONV3D, EX_PERMUTE, EX_NORM, EX_ADAPT, EX_RECUR };
 struct Exec {
     ExecKind kind;
     int src = -1, dst = -1, res = -1;
@@ -48,6 +49,10 @@ struct Exec {
     int head_dst = -1;              // conv2d: tensor that receives the thin 1 x 1 convolution folded into this conv (which then stores nothing itself)
     const float *head_w = nullptr, *head_b = nullptr;
     int head_n = 0;
+    int side = -1, h_in = -1, h_out = -1;
+    NormDesc norm = {};
+    AdaptDesc adapt = {};
+    void* ws = nullptr;             // scratch of this kernel alone (norm, adapters, recurrence)
 };
 
 struct fortis_plan {
@@ -58,6 +63,7 @@ struct fortis_plan {
     std::vector<Op> ops;
     std::vector<Exec> exec;
     std::vector<void*> owned;   // device allocations owned by the plan (weights, vectors)
+    std::vector<void*> work;    // device allocations behind the kernels' scratch (Exec::ws), sized for the rows of the buffers
     std::vector<void*> bufs;    // distinct pool buffers behind the tensors (several tensors may share one)
     bool finalized = false;
     bool upload_failed = false; // a weight / vector upload found no device memory
@@ -92,6 +98,21 @@ static bool tensor_ok(fortis_plan* p, int t, long need_bytes)
     return t >= 0 && t < (int)p->tbytes.size() && p->tbytes[t] >= need_bytes;
 }
 
+// a * b * c * d elements of 4 bytes, or -1 where that leaves 2^62 (every factor > 0)
+static long bytes_of(long a, long b, long c = 1, long d = 1)
+{
+    long n = 4;
+    for (long f : { a, b, c, d })
+        if (f <= 0 || __builtin_mul_overflow(n, f, &n) || n > (1L << 62)) return -1;
+    return n;
+}
+// Whether the windows of two tensors share memory (a window of a tensor against that tensor included).
+static bool overlap(const fortis_plan* p, int a, int b)
+{
+    const int ba = p->view_of[a] >= 0 ? p->view_of[a] : a, bb = p->view_of[b] >= 0 ? p->view_of[b] : b;
+    return ba == bb && p->view_off[a] < p->view_off[b] + p->tbytes[b] && p->view_off[b] < p->view_off[a] + p->tbytes[a];
+}
+
 extern "C" {
 
 fortis_plan* fortis_plan_create(void) { return new fortis_plan(); }
@@ -99,6 +120,7 @@ void fortis_plan_destroy(fortis_plan* p)
 {
     if (!p) return;
     for (void* d : p->owned) fortis_dev_free(d);
+    for (void* d : p->work) fortis_dev_free(d);
     for (void* b : p->bufs) fortis_free(b);
     delete p;
 }
@@ -274,13 +296,69 @@ int fortis_plan_permute(fortis_plan* p, int src, int dst, long C, long S, int to
     return 0;
 }
 
+int fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma, const float* beta, float eps, long NB,
+                           long S, long C, long G, int channels_first, int act, float alpha)
+{
+    if (!p || p->finalized) return bad("plan is null or already finalized");
+    const long need = bytes_of(NB, S, C);
+    if (need < 0 || G <= 0 || C % G || !(eps >= 0.f)) return bad("group_norm: bad shape, groups or eps");
+    if (act < 0 || act > FORTIS_ACT_SILU) return bad("group_norm: unknown activation");
+    if (!tensor_ok(p, src, need) || !tensor_ok(p, dst, need) || overlap(p, src, dst)) return bad("group_norm: tensors too small or overlapping");
+    Op o; o.kind = OP_NORM; o.src = src; o.dst = dst; o.B = NB; o.H = S; o.C = C; o.F = G; o.flag = channels_first ? 1 : 0;
+    o.act = act; o.alpha = alpha; o.eps = eps;
+    if (gamma) { o.v0.assign(gamma, gamma + C); o.has_v[0] = true; }
+    if (beta) { o.v1.assign(beta, beta + C); o.has_v[1] = true; }
+    p->ops.push_back(std::move(o));
+    return 0;
+}
+int fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, const float* W, const float* bias, const float* A,
+                                const float* U, const float* scale, long B, long K, long N, long nadapt, long rank, int act, float alpha)
+{
+    if (!p || p->finalized) return bad("plan is null or already finalized");
+    const long nx = bytes_of(B, K), ny = bytes_of(B, N), ni = bytes_of(B, 1);
+    if (nx < 0 || ny < 0 || bytes_of(N, K) < 0 || bytes_of(nadapt, rank, K) < 0 || bytes_of(nadapt, rank, N) < 0 || B >= (1L << 31) ||
+        K >= (1L << 22) || N >= (1L << 22) || !W || !A || !U)
+        return bad("linear_adapters: bad shape or arguments");
+    if (nadapt > FORTIS_MAX_ADAPTERS || rank > FORTIS_MAX_RANK) return bad("linear_adapters: too many adapters or too large a rank");
+    if (act < 0 || act > FORTIS_ACT_SILU) return bad("linear_adapters: unknown activation");
+    if (!tensor_ok(p, src, nx) || !tensor_ok(p, dst, ny) || !tensor_ok(p, index, ni) || overlap(p, src, dst) || overlap(p, index, dst) ||
+        overlap(p, index, src))
+        return bad("linear_adapters: tensors too small or overlapping");
+    Op o; o.kind = OP_ADAPT; o.src = src; o.dst = dst; o.side = index; o.B = B; o.K = K; o.N = N; o.F = nadapt; o.D = rank; o.act = act; o.alpha = alpha;
+    o.w.assign(W, W + N * K);
+    if (bias) { o.b.assign(bias, bias + N); o.has_bias = true; }
+    o.v0.assign(A, A + nadapt * rank * K);
+    o.v1.assign(U, U + nadapt * N * rank);
+    if (scale) o.v2.assign(scale, scale + nadapt); else o.v2.assign(nadapt, 1.f);
+    p->ops.push_back(std::move(o));
+    return 0;
+}
+int fortis_plan_recurrence(fortis_plan* p, int src, int dst, int h_in, int h_out, int lengths, long nseq, long len, long ch,
+                           int time_major, int reverse)
+{
+    if (!p || p->finalized) return bad("plan is null or already finalized");
+    const long nsrc = bytes_of(nseq, len, ch, 2), ndst = bytes_of(nseq, len, ch), nst = bytes_of(nseq, ch), nl = bytes_of(nseq, 1);
+    if (nsrc < 0 || len >= (1L << 31)) return bad("recurrence: bad shape");
+    if (!tensor_ok(p, src, nsrc) || !tensor_ok(p, dst, ndst) || (h_in >= 0 && !tensor_ok(p, h_in, nst)) || (h_out >= 0 && !tensor_ok(p, h_out, nst)) ||
+        (lengths >= 0 && !tensor_ok(p, lengths, nl)))
+        return bad("recurrence: tensors too small");
+    const int t[5] = { src, dst, h_in, h_out, lengths };
+    for (int a = 0; a < 5; a++)
+        for (int b = a + 1; b < 5; b++)
+            if (t[a] >= 0 && t[b] >= 0 && overlap(p, t[a], t[b]) && !(a == 2 && b == 3 && h_in == h_out)) return bad("recurrence: tensors overlap");
+    Op o; o.kind = OP_RECUR; o.src = src; o.dst = dst; o.side = lengths < 0 ? -1 : lengths; o.h_in = h_in < 0 ? -1 : h_in; o.h_out = h_out < 0 ? -1 : h_out;
+    o.B = nseq; o.H = len; o.C = ch; o.flag = (time_major ? 1 : 0) | (reverse ? 2 : 0);
+    p->ops.push_back(std::move(o));
+    return 0;
+}
+
 }  // extern "C"
 
 // ---- finalize: fusion + uploads -----------------------------------------------------------------
 static int uses_of(const fortis_plan* p, int t)
 {
     int n = (t == p->out_t) ? 1 : 0;
-    for (const Op& o : p->ops) n += (o.src == t) + (o.res == t);
+    for (const Op& o : p->ops) n += (o.src == t) + (o.res == t) + (o.side == t) + (o.h_in == t);
     return n;
 }
 
@@ -367,9 +445,26 @@ static int assign_buffers(fortis_plan* p)
     auto writes = [&](int t, int i) { if (t < 0) return; t = base(t); if (first[t] > i) first[t] = i; if (last[t] < i) last[t] = i; };
     for (int i = 0; i < ne; i++) {
         const Exec& e = p->exec[i];
-        reads(e.src, i); reads(e.res, i);
+        reads(e.src, i); reads(e.res, i); reads(e.side, i); reads(e.h_in, i);
         if (e.head_dst < 0) writes(e.dst, i);
-        writes(e.pool_dst, i); writes(e.head_dst, i);
+        writes(e.pool_dst, i); writes(e.head_dst, i); writes(e.h_out, i);
+    }
+    // A side tensor (adapter indices, lengths, a state that comes in) that no earlier kernel of the pass writes is the
+    // caller's or the last pass's: its buffer is never shared, whatever is written to other windows of it.  Nor is that
+    // of a state that goes out, which the caller reads behind the pass.
+    auto written_before = [&](int t, int i) {
+        for (int j = 0; j < i; j++) {
+            const Exec& e = p->exec[j];
+            for (int w : { e.head_dst < 0 ? e.dst : -1, e.pool_dst, e.head_dst, e.h_out }) if (w >= 0 && overlap(p, w, t)) return true;
+        }
+        return false;
+    };
+    std::vector<char> fill_side(ne, 0), fill_in(ne, 0), fill_out(ne, 0);
+    for (int i = 0; i < ne; i++) {
+        const Exec& e = p->exec[i];
+        if (e.side >= 0 && !written_before(e.side, i)) { fill_side[i] = 1; first[base(e.side)] = -1; last[base(e.side)] = ne; }
+        if (e.h_in >= 0 && !written_before(e.h_in, i)) { fill_in[i] = 1; first[base(e.h_in)] = -1; last[base(e.h_in)] = ne; }
+        if (e.h_out >= 0) { fill_out[i] = !written_before(e.h_out, i); first[base(e.h_out)] = -1; last[base(e.h_out)] = ne; }
     }
     for (int t = 0; t < nt; t++) if (first[t] == -1) last[t] = ne;          // filled by the caller: never handed back
     first[base(p->in_t)] = -1; last[base(p->in_t)] = ne;
@@ -412,6 +507,36 @@ static int assign_buffers(fortis_plan* p)
     if (rc != 0) { p->tptr.assign(nt, nullptr); return -1; }
     for (int t = 0; t < nt; t++)
         if (p->view_of[t] >= 0 && p->tptr[p->view_of[t]]) p->tptr[t] = (char*)p->tptr[p->view_of[t]] + p->view_off[t];
+    // what a side tensor that no kernel writes holds until the caller writes it (not for a test's host allocator: no device)
+    if (!fortis_pool_on_device()) return 0;
+    for (int i = 0; i < ne; i++) {
+        const Exec& e = p->exec[i];
+        if (fill_side[i])
+            fortis_launch_fill_int((int*)p->tptr[e.side], e.kind == EX_ADAPT ? -1 : (int)e.op->H, e.kind == EX_ADAPT ? e.rows_cap : e.op->B, fortis_stream_get());
+        if (fill_in[i]) fortis_launch_zero((float*)p->tptr[e.h_in], e.op->B * e.op->C, fortis_stream_get());
+        if (fill_out[i]) fortis_launch_zero((float*)p->tptr[e.h_out], e.op->B * e.op->C, fortis_stream_get());
+    }
+    return 0;
+}
+// Every kernel that needs scratch gets its own: nothing is shared between kernels, plans or captured graphs.
+static int assign_workspaces(fortis_plan* p)
+{
+    for (void* d : p->work) fortis_dev_free(d);
+    p->work.clear();
+    for (Exec& e : p->exec) {
+        long n = 0;
+        if (e.kind == EX_NORM) {
+            NormDesc d = e.norm;
+            if (d.S == 1) d.NB = e.rows_cap;
+            n = fortis_norm_workspace(d);
+        }
+        else if (e.kind == EX_ADAPT) n = fortis_adapters_workspace(e.adapt, e.rows_cap);
+        else if (e.kind == EX_RECUR) n = fortis_recurrence_workspace({ e.op->B, e.op->H, e.op->C, e.op->flag & 1, e.op->flag >> 1 });
+        e.ws = nullptr;
+        if (n <= 0) continue;
+        if (fortis_dev_malloc(&e.ws, (size_t)n, "kernel scratch") != 0) return -1;
+        p->work.push_back(e.ws);
+    }
     return 0;
 }
 
@@ -550,7 +675,7 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
                     ops[i + 1].src == o.dst && ops[i + 1].KD == 3 && ops[i + 1].pad == 1 && ops[i + 1].F >= 16 && out_t != o.dst) {
                     bool other = false;
                     for (size_t j = 0; j < ops.size(); j++)
-                        if (j != i + 1 && (ops[j].src == o.dst || ops[j].res == o.dst)) other = true;
+                        if (j != i + 1 && (ops[j].src == o.dst || ops[j].res == o.dst || ops[j].side == o.dst || ops[j].h_in == o.dst)) other = true;
                     if (ops[i + 1].res == o.dst) other = true;
                     if (!other) { fuse_ups_src = o.src; p->exec_skip++; i += 1; continue; }
                 }
@@ -558,6 +683,25 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
             }
             case OP_CONCAT: ex.kind = EX_CONCAT; break;
             case OP_PERMUTE: ex.kind = EX_PERMUTE; break;
+            case OP_NORM:
+                ex.kind = EX_NORM;
+                if (o.H == 1) ex.rows = ex.rows_cap = o.B;
+                ex.norm = { o.B, o.H, o.C, o.F, o.flag, o.eps, o.act, o.alpha, nullptr, nullptr };
+                if (o.has_v[0]) ex.norm.gamma = (const float*)upload(p, o.v0.data(), o.v0.size() * 4);
+                if (o.has_v[1]) ex.norm.beta = (const float*)upload(p, o.v1.data(), o.v1.size() * 4);
+                break;
+            case OP_ADAPT:
+                ex.kind = EX_ADAPT; ex.side = o.side; ex.rows = ex.rows_cap = o.B;
+                ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, nullptr, nullptr, nullptr, nullptr, nullptr };
+                ex.adapt.W = (const float*)upload(p, o.w.data(), o.w.size() * 4);
+                ex.adapt.bias = o.has_bias ? (const float*)upload(p, o.b.data(), o.b.size() * 4) : nullptr;
+                ex.adapt.A = (const float*)upload(p, o.v0.data(), o.v0.size() * 4);
+                ex.adapt.U = (const float*)upload(p, o.v1.data(), o.v1.size() * 4);
+                ex.adapt.scale = (const float*)upload(p, o.v2.data(), o.v2.size() * 4);
+                break;
+            case OP_RECUR:
+                ex.kind = EX_RECUR; ex.side = o.side; ex.h_in = o.h_in; ex.h_out = o.h_out;
+                break;
         }
         p->exec.push_back(ex);
         i += adv;
@@ -565,7 +709,8 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
     bool rowwise = true;
     long rows = -1;
     for (const Exec& e : p->exec) {
-        if (e.kind > EX_MASK) { rowwise = false; break; }
+        // (one-position group norms and adapted projections work row by row too)
+        if (e.kind > EX_MASK && e.kind != EX_ADAPT && !(e.kind == EX_NORM && e.norm.S == 1)) { rowwise = false; break; }
         if (rows < 0) rows = e.rows; else if (rows != e.rows) rowwise = false;
     }
     p->rows0 = rowwise ? rows : 0;
@@ -581,6 +726,7 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
     }
     if (p->upload_failed) return bad("finalize: out of device memory for the weights");
     if (assign_buffers(p) != 0) return bad("finalize: out of device memory for the activations");
+    if (assign_workspaces(p) != 0) return bad("finalize: out of device memory for the kernels' scratch");
     p->finalized = true;
     // (with a test's host allocator in place of the device's there is no device to wait for, and no launch may follow)
     if (fortis_pool_on_device()) { (void)fortis_stream_get(); HIP_OK(hipDeviceSynchronize()); }
@@ -646,6 +792,17 @@ void fortis_plan_run(fortis_plan* p)
             case EX_UPSAMPLE: fortis_launch_upsample(src, dst, o->C, o->D, o->H, o->W, o->sfac, o->nd, s); break;
             case EX_CONCAT: fortis_launch_concat_copy(src, dst + o->coff * o->H, o->C, o->H, o->coff, s); break;
             case EX_PERMUTE: fortis_launch_permute(src, dst, o->C, o->H, o->flag, s); break;
+            case EX_NORM: {
+                NormDesc d = e.norm;
+                if (d.S == 1) d.NB = e.rows;
+                fortis_launch_group_norm(d, src, dst, e.ws, s);
+                break;
+            }
+            case EX_ADAPT: fortis_launch_linear_adapters(e.adapt, src, (const int*)p->tptr[e.side], dst, e.rows, e.ws, s); break;
+            case EX_RECUR:
+                fortis_launch_recurrence({ o->B, o->H, o->C, o->flag & 1, o->flag >> 1 }, src, dst, e.h_in >= 0 ? (const float*)p->tptr[e.h_in] : nullptr,
+                                         e.h_out >= 0 ? (float*)p->tptr[e.h_out] : nullptr, e.side >= 0 ? (const int*)p->tptr[e.side] : nullptr, e.ws, s);
+                break;
         }
         if (rc != 0) fprintf(stderr, "fortis_plan_run: an op was rejected by its kernel launcher\n");
         mark();
@@ -680,7 +837,8 @@ static void plan_run_rows(fortis_plan* p, long i0, long n, hipStream_t s)
 }
 
 static const char* const kExecNames[] = { "mlp_chain", "gemm_bias_act", "scale", "mask_relu", "boundary_pre", "boundary_post",
-                                          "conv2d", "convt2d", "maxpool2d", "upsample", "concat_copy", "conv3d", "permute" };
+                                          "conv2d", "convt2d", "maxpool2d", "upsample", "concat_copy", "conv3d", "permute",
+                                          "group_norm", "linear_adapters", "recurrence" };
 const char* fortis_plan_kernel_name(fortis_plan* p, int idx)
 {
     if (!p || !p->finalized || idx < 0 || idx >= (int)p->exec.size()) return "";
@@ -735,16 +893,19 @@ static int plan_set_rows(fortis_plan* p, long rows)
     if (!p || !p->finalized || p->rows0 <= 0 || rows <= 0) return -1;
     if (rows > p->rows0) {
         for (int v : p->view_of) if (v >= 0) return -1;
+        for (const Exec& e : p->exec) if (e.kind == EX_ADAPT && rows >= (1L << 31)) return -1;
         std::vector<long> old(p->tbytes);
+        const long old_rows = p->rows0;
         for (long& b : p->tbytes) b = (long)(((__int128)b * rows + p->rows0 - 1) / p->rows0);
         HIP_OK(hipStreamSynchronize(fortis_stream_get()));      // nothing in flight may still use the old buffers
-        if (assign_buffers(p) != 0) {
+        for (Exec& e : p->exec) e.rows_cap = rows;
+        if (assign_buffers(p) != 0 || assign_workspaces(p) != 0) {
             p->tbytes = old;
-            if (assign_buffers(p) != 0) { fprintf(stderr, "fortis_plan: could not restore the plan's buffers\n"); p->finalized = false; }
+            for (Exec& e : p->exec) e.rows_cap = old_rows;
+            if (assign_buffers(p) != 0 || assign_workspaces(p) != 0) { fprintf(stderr, "fortis_plan: could not restore the plan's buffers\n"); p->finalized = false; }
             return -1;
         }
         p->rows0 = rows;
-        for (Exec& e : p->exec) e.rows_cap = rows;
     }
     for (Exec& e : p->exec) e.rows = rows;
     return 0;
@@ -824,6 +985,7 @@ static bool bound(const char* who)
 static long g_forward_gen = 0;   // bumped by every forward pass of the bound step
 void* fortis_model_input(void) { bind_if_pending(); return g_step.din; }
 void* fortis_model_output(void) { bind_if_pending(); return g_step.dout; }
+void* fortis_model_tensor(int t) { bind_if_pending(); return g_step.plan ? fortis_plan_tensor_ptr(g_step.plan, t) : nullptr; }
 long fortis_step_generation(void) { return g_forward_gen; }   // internal: lets the scatter entry notice a new forward pass
 
 void mlp_forward_dev(void)
@@ -1196,6 +1358,9 @@ void mlp_forward(void* in, void* out)
     bool direct = nin <= 32 * 1024 && nout <= 32 * 1024 && !getenv("FORTIS_NO_ZEROCOPY") && p->in_t != p->out_t;
     for (size_t t = 0; direct && t < p->view_of.size(); t++)
         if (p->view_of[t] == p->in_t || p->view_of[t] == p->out_t) direct = false;
+    // a side tensor or a carried state keeps its place on the device
+    for (const Exec& e : p->exec)
+        for (int t : { e.side, e.h_in, e.h_out }) if (t >= 0 && (t == p->in_t || t == p->out_t)) direct = false;
     if (direct) {
         if (!g_step.X) setup_xy();
         memcpy(g_step.X, in, nin);

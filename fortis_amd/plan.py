@@ -12,6 +12,7 @@ import numpy as np
 from ._lib import lib
 
 ACT = {None: 0, "none": 0, "relu": 1, "leaky": 2}
+ACT_SILU = dict(ACT, silu=3)     # group_norm and linear_adapters
 
 
 def _f32(a):
@@ -117,6 +118,26 @@ class Plan:
 
     def permute(self, src, dst, C_, S, to_channels_first):
         self._ok(self._L.fortis_plan_permute(self._p, src, dst, C_, S, 1 if to_channels_first else 0), "permute")
+
+    def group_norm(self, src, dst, NB, S, C_, G, gamma=None, beta=None, eps=1e-5, act=None, alpha=0.0, channels_first=False):
+        ga, be = [None if v is None else _f32(v) for v in (gamma, beta)]
+        assert all(v is None or v.shape == (C_,) for v in (ga, be))
+        self._ok(self._L.fortis_plan_group_norm(self._p, src, dst, _p(ga), _p(be), eps, NB, S, C_, G, 1 if channels_first else 0,
+                                                ACT_SILU[act], alpha), "group_norm")
+
+    def linear_adapters(self, src, dst, index, W, bias, A, U, B, scale=None, act=None, alpha=0.0):
+        W, A, U = _f32(W), _f32(A), _f32(U)
+        N, K = W.shape
+        nadapt, rank, Ka = A.shape
+        assert Ka == K and U.shape == (nadapt, N, rank)
+        b, sc = [None if v is None else _f32(v) for v in (bias, scale)]
+        assert (b is None or b.shape == (N,)) and (sc is None or sc.shape == (nadapt,))
+        self._ok(self._L.fortis_plan_linear_adapters(self._p, src, dst, index, _p(W), _p(b), _p(A), _p(U), _p(sc), B, K, N, nadapt, rank,
+                                                     ACT_SILU[act], alpha), "linear_adapters")
+
+    def recurrence(self, src, dst, nseq, length, ch, h_in=-1, h_out=-1, lengths=-1, time_major=True, reverse=False):
+        self._ok(self._L.fortis_plan_recurrence(self._p, src, dst, h_in, h_out, lengths, nseq, length, ch, 1 if time_major else 0,
+                                                1 if reverse else 0), "recurrence")
 
     def finalize(self, in_tensor, out_tensor):
         self._ok(self._L.fortis_plan_finalize(self._p, in_tensor, out_tensor), "finalize")

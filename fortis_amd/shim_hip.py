@@ -27,6 +27,7 @@ import sys
 import numpy as np
 
 ACT = {None: 0, "none": 0, "relu": 1, "leaky": 2}
+ACT_SILU = dict(ACT, silu=3)     # group_norm and linear_adapters
 VERDICT_C = {"batched": "FORTIS_VERDICT_BATCHED", "boundary": "FORTIS_VERDICT_BOUNDARY"}
 
 
@@ -221,6 +222,21 @@ class OpList:
     def permute(self, src, dst, C_, S, to_channels_first):
         self.ops.append(dict(op="permute", src=src, dst=dst, C=int(C_), S=int(S), to_channels_first=bool(to_channels_first)))
 
+    def group_norm(self, src, dst, NB, S, C_, G, gamma=None, beta=None, eps=1e-5, act=None, alpha=0.0, channels_first=False):
+        self.ops.append(dict(op="group_norm", src=src, dst=dst, gamma=self._w(gamma), beta=self._w(beta), eps=float(eps), NB=int(NB), S=int(S),
+                             C=int(C_), G=int(G), channels_first=bool(channels_first), act=act or "none", alpha=float(alpha)))
+
+    def linear_adapters(self, src, dst, index, W, bias, A, U, B, scale=None, act=None, alpha=0.0):
+        N, K = np.asarray(W).shape
+        nadapt, rank, _ = np.asarray(A).shape
+        self.ops.append(dict(op="linear_adapters", src=src, dst=dst, index=int(index), w=self._w(W), b=self._w(bias), A=self._w(A), U=self._w(U),
+                             scale=self._w(scale), B=int(B), K=int(K), N=int(N), nadapt=int(nadapt), rank=int(rank), act=act or "none",
+                             alpha=float(alpha)))
+
+    def recurrence(self, src, dst, nseq, length, ch, h_in=-1, h_out=-1, lengths=-1, time_major=True, reverse=False):
+        self.ops.append(dict(op="recurrence", src=src, dst=dst, h_in=int(h_in), h_out=int(h_out), lengths=int(lengths), nseq=int(nseq),
+                             len=int(length), ch=int(ch), time_major=bool(time_major), reverse=bool(reverse)))
+
     def finalize(self, in_tensor, out_tensor):
         self.in_tensor, self.out_tensor = in_tensor, out_tensor
         return self
@@ -301,14 +317,14 @@ def emit_step(attrs, outline, ops, env=None):
 
     def tid(o, key):
         v = o[key]
-        if not isinstance(v, int) or not -1 <= v < len(T) or (v < 0 and key != "res"):
+        if not isinstance(v, int) or not -1 <= v < len(T) or (v < 0 and key not in ("res", "h_in", "h_out", "lengths")):
             raise ValueError("ops.json: op %r names tensor %r" % (o["op"], v))
         return "t[%d]" % v if v >= 0 else "-1"
 
-    def act(o):
-        if o.get("act", "none") not in ACT:
+    def act(o, known=ACT):
+        if o.get("act", "none") not in known:
             raise ValueError("ops.json: unknown activation %r" % o["act"])
-        return "%d, %sf" % (ACT[o.get("act", "none")], repr(float(o.get("alpha", 0.0))))
+        return "%d, %sf" % (known[o.get("act", "none")], repr(float(o.get("alpha", 0.0))))
 
     for n, o in enumerate(ops["ops"]):
         k = o["op"]
@@ -348,6 +364,17 @@ def emit_step(attrs, outline, ops, env=None):
                 s, d, tid(o, "res") if "res" in o else "-1", W("w"), W("b"), o["C"], o["D"], o["H"], o["W"], o["F"], o["K"], o["pad"], act(o))
         elif k == "permute":
             c = "fortis_plan_permute(p, %s, %s, %d, %dL, %d)" % (s, d, o["C"], o["S"], 1 if o["to_channels_first"] else 0)
+        elif k == "group_norm":
+            c = "fortis_plan_group_norm(p, %s, %s, %s, %s, %sf, %dL, %dL, %d, %d, %d, %s)" % (
+                s, d, W("gamma"), W("beta"), repr(float(o.get("eps", 1e-5))), o["NB"], o["S"], o["C"], o["G"], 1 if o.get("channels_first") else 0,
+                act(o, ACT_SILU))
+        elif k == "linear_adapters":
+            c = "fortis_plan_linear_adapters(p, %s, %s, %s, %s, %s, %s, %s, %s, %dL, %d, %d, %d, %d, %s)" % (
+                s, d, tid(o, "index"), W("w"), W("b"), W("A"), W("U"), W("scale"), o["B"], o["K"], o["N"], o["nadapt"], o["rank"], act(o, ACT_SILU))
+        elif k == "recurrence":
+            side = [tid(o, key) if key in o else "-1" for key in ("h_in", "h_out", "lengths")]
+            c = "fortis_plan_recurrence(p, %s, %s, %s, %dL, %dL, %d, %d, %d)" % (
+                s, d, ", ".join(side), o["nseq"], o["len"], o["ch"], 1 if o.get("time_major", True) else 0, 1 if o.get("reverse") else 0)
         else:
             raise ValueError("ops.json: unknown op %r" % k)
         L.append("    OK(%s);" % c)

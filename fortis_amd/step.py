@@ -56,6 +56,10 @@ def fortis_unpack(row, col):
     lib().fortis_unpack(_vp(row), col)
 
 
+def fortis_model_tensor(t):
+    return lib().fortis_model_tensor(t)
+
+
 def fortis_begin(count):
     lib().fortis_begin(count)
 

@@ -29,7 +29,8 @@ extern "C" {
 /* ReLU is v > 0 ? v : 0 and LeakyReLU v > 0 ? v : alpha * v on finite values and infinities.  A NaN pre-activation is
  * outside the parity contract: ReLU turns it into 0 in most kernels, while the straight-line kernels of narrow
  * networks (all widths <= 64) take the maximum on the bit pattern and keep a NaN whose sign bit is clear. */
-enum { FORTIS_ACT_NONE = 0, FORTIS_ACT_RELU = 1, FORTIS_ACT_LEAKY = 2 };
+enum { FORTIS_ACT_NONE = 0, FORTIS_ACT_RELU = 1, FORTIS_ACT_LEAKY = 2,
+       FORTIS_ACT_SILU = 3 };  /* v / (1 + exp(-v)); fortis_plan_group_norm and fortis_plan_linear_adapters only */
 
 typedef struct fortis_plan fortis_plan;
 
@@ -95,6 +96,47 @@ int  fortis_plan_conv3d(fortis_plan* p, int src, int dst, int res, const float* 
  * otherwise [C][S] -> [S][C].  S = product of the spatial dims. */
 int  fortis_plan_permute(fortis_plan* p, int src, int dst, long C, long S, int to_channels_first);
 
+/* ---- operators without a counterpart in the reference: adapted, normalised and recurrent models ---------------
+ * All of them work on float32 tensors in the row layout of the other calls and refuse (-1 and a message) tensors
+ * that are too small or whose windows overlap.  Side tensors (index, lengths, states) are declared with
+ * fortis_plan_tensor like any other; the caller fills them through fortis_plan_tensor_ptr (a host behind the bind(c)
+ * entries: fortis_model_tensor) before a pass, and they keep their contents from pass to pass. */
+
+/* Group normalisation with an activation, NB samples of S positions and C channels, channels last ([NB][S][C]) or, with
+ * channels_first, [NB][C][S]: for every sample and every group of C / G neighbouring channels
+ *     dst = act(gamma[c] * (src - mean) / sqrt(var + eps) + beta[c])
+ * over the group's S * C / G values, var their biased variance.  gamma, beta: host pointers of length C, copied, or NULL
+ * (1 and 0).  G has to divide C; eps >= 0.  S = 1 normalises rows (one head of C / G features per group).  The mean is
+ * kept to twice float32's digits and sums are joined in float64, so a large common offset costs no accuracy.  A NaN or
+ * an infinity makes its own group NaN and no other. */
+int  fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma, const float* beta, float eps,
+                            long NB, long S, long C, long G, int channels_first, int act, float alpha);
+/* fortis_plan_linear with a low-rank adapter chosen per row:
+ *     dst[r] = act(src[r] . W^T + bias + scale[i] * ((src[r] . A[i]^T) . U[i]^T)),   i = index[r]
+ * A [nadapt][rank][K], U [nadapt][N][rank], scale [nadapt] (NULL: 1), W, bias as in fortis_plan_linear: host pointers,
+ * copied.  index: a tensor of B int32, read on the device at every pass, rows in any order; an index outside
+ * [0, nadapt) means no adapter for that row, and so all rows start (index is filled with -1 at finalize).  1 <= nadapt
+ * <= FORTIS_MAX_ADAPTERS, 1 <= rank <= FORTIS_MAX_RANK, B < 2^31.  A row's result depends on that row alone: not on the
+ * order of rows, nor on the adapters of the others. */
+#define FORTIS_MAX_ADAPTERS 4096
+#define FORTIS_MAX_RANK 256
+int  fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, const float* W, const float* bias,
+                                 const float* A, const float* U, const float* scale, long B, long K, long N,
+                                 long nadapt, long rank, int act, float alpha);
+/* Gated linear recurrence over `len` steps of `nseq` sequences of `ch` channels.  A row of src holds 2 * ch features,
+ * gates g first, candidates x behind them (one linear layer writes both):
+ *     f = 1 / (1 + exp(-g_t)),  h_t = f * h_(t-1) + (1 - f) * x_t,  dst row t = h_t  (ch features)
+ * Rows: time_major != 0: row t * nseq + s (the order in which the gather writes levels of columns), else s * len + t.
+ * reverse: steps are taken from the sequence's last to its first.
+ * h_in: tensor [nseq][ch] with the state in front of the first step taken, -1: zeros.  h_out: tensor [nseq][ch] that
+ * receives the state behind the last one, -1: none.  h_in == h_out carries the state from pass to pass (len = 1 is one
+ * step of a host that steps through time); a state that no operation of the plan writes first starts as zeros.
+ * lengths: tensor of nseq int32, -1: all `len`; sequence s takes steps 0 .. lengths[s] - 1 only (values are clamped to
+ * [0, len]; filled with len at finalize).  Rows of dst at and behind a sequence's length are left as they were, a
+ * sequence without steps hands its state on unchanged. */
+int  fortis_plan_recurrence(fortis_plan* p, int src, int dst, int h_in, int h_out, int lengths, long nseq, long len,
+                            long ch, int time_major, int reverse);
+
 /* Fixes the plan: allocates tensors, uploads weights, folds BatchNorm, fuses neighbouring ops
  * into single kernels.  in_tensor / out_tensor are what fortis_model_input/output return. */
 int   fortis_plan_finalize(fortis_plan* p, int in_tensor, int out_tensor);
@@ -141,6 +183,9 @@ void  fortis_pack(void* row, int col);            /* :105  col is 0-based */
 void  fortis_unpack(void* row, int col);          /* :106 */
 void* fortis_model_input(void);                   /* :109 */
 void* fortis_model_output(void);                  /* :110 */
+/* Device address of tensor `t` of the bound step's plan (its number in the op list), NULL if there is none: where a host
+ * writes adapter indices, lengths or a state (fortis_h2d) and reads a state back.  No reference counterpart. */
+void* fortis_model_tensor(int t);
 /* Run-time extents: re-specialises the bound step for `count` rows per call; no JIT, the
  * kernels take the row count at run time.                  driver/fortis_stub.c:12-31 */
 void  fortis_begin(int count);

@@ -1,0 +1,506 @@
+"""Group norm, projections with adapters per row and the gated recurrence on the GPU through the plan calls, against
+their formulas in float64 (tests/refops.py, where the error bounds are derived)."""
+import ctypes as C
+import os
+
+import numpy as np
+import pytest
+
+import refops as R
+from fortis_amd import plan as P, step
+from util import bits_equal
+
+pytestmark = pytest.mark.gpu
+
+
+def within(got, ref, bound):
+    got = np.asarray(got, np.float64).reshape(ref.shape)
+    bad = np.abs(got - ref) > bound + 1e-37          # NaN compares false: it is caught by the next line
+    assert not np.isnan(got).any()
+    assert not bad.any(), (int(bad.sum()), float((np.abs(got - ref) / (bound + 1e-37)).max()))
+
+
+# ---- group norm ----------------------------------------------------------------------------------------------
+def run_norm(x, G, gamma=None, beta=None, eps=1e-5, act=None, alpha=0.0, first=False, fill=None):
+    NB, S, Cc = (x.shape[0], x.shape[2], x.shape[1]) if first else x.shape
+    p = P.Plan()
+    t, o = p.tensor(x.size), p.tensor(x.size)
+    p.group_norm(t, o, NB, S, Cc, G, gamma, beta, eps, act, alpha, first)
+    p.finalize(t, o)
+    if fill is not None:
+        p.write(o, np.full(x.shape, fill, np.float32))
+    y = p.forward(x, x.shape)
+    p.close()
+    return y
+
+
+NORM_SHAPES = [(1, 1, 1, 1), (1, 1, 64, 4), (7, 1, 64, 4), (300, 1, 12, 3), (5000, 1, 64, 4), (2, 3, 5, 5), (3, 2, 30, 3), (1, 4095, 60, 5),
+               (2, 33 * 33, 24, 3), (1, 1024, 256, 8), (9, 130, 96, 32), (2, 7, 1000, 1), (1, 3, 4100, 2), (1, 2, 9000, 1), (1, 65536, 32, 8), (3, 20000, 7, 7),
+               (1, 35937, 64, 8), (64, 64, 128, 2), (1, 1, 70000, 1), (17, 257, 6, 2), (700, 15, 8, 2), (1, 5003, 3, 1), (4, 1, 2048, 16)]
+
+
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("NB,S,Cc,G", NORM_SHAPES)
+def test_group_norm(L, gpu, NB, S, Cc, G, first):
+    rng = np.random.default_rng(NB + S + Cc)
+    x = rng.standard_normal((NB, Cc, S) if first else (NB, S, Cc)).astype(np.float32)
+    off = (2 * rng.standard_normal(Cc)).astype(np.float32)
+    x += off[:, None] if first else off
+    gamma, beta = (1 + 0.2 * rng.standard_normal(Cc)).astype(np.float32), (0.1 * rng.standard_normal(Cc)).astype(np.float32)
+    act, alpha = [(None, 0.0), ("relu", 0.0), ("leaky", 0.2), ("silu", 0.0)][(NB + S + Cc + G) % 4]
+    within(run_norm(x, G, gamma, beta, 1e-5, act, alpha, first), *R.group_norm(x, G, gamma, beta, 1e-5, act, alpha, first))
+
+
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("act,alpha", [(None, 0.0), ("relu", 0.0), ("leaky", 0.2), ("leaky", -0.5), ("leaky", 1.5), ("silu", 0.0)])
+def test_group_norm_activations_without_vectors(L, gpu, act, alpha, first):
+    x = np.random.default_rng(1).standard_normal((4, 16, 50) if first else (4, 50, 16)).astype(np.float32)
+    within(run_norm(x, 4, None, None, 0.1, act, alpha, first), *R.group_norm(x, 4, None, None, 0.1, act, alpha, first))
+    beta = np.linspace(-1, 1, 16).astype(np.float32)
+    within(run_norm(x, 4, None, beta, 0.1, act, alpha, first), *R.group_norm(x, 4, None, beta, 0.1, act, alpha, first))
+
+
+@pytest.mark.parametrize("NB,S,Cc,G,first", [(3, 1, 64, 4, False), (2, 500, 32, 4, False), (1, 70000, 16, 2, False), (2, 500, 32, 4, True), (1, 70000, 16, 2, True)])
+def test_group_norm_of_a_large_common_offset(L, gpu, NB, S, Cc, G, first):
+    """The offset is 20000 times the spread: inputs are exact in float32 (steps of 2^-10 at 2^13..2^14), so the formula
+    in float64 on the same inputs is the answer, and the bound does not grow with the offset."""
+    rng = np.random.default_rng(5)
+    x = (np.round(rng.standard_normal((NB, Cc, S) if first else (NB, S, Cc)) * 512) / 1024 + 10000).astype(np.float32)
+    within(run_norm(x, G, first=first), *R.group_norm(x, G, None, None, 1e-5, None, 0, first))
+
+
+@pytest.mark.parametrize("NB,S,Cc,G,first", [(6, 1, 32, 4, False), (2, 300, 32, 4, False), (2, 70000, 16, 4, False), (2, 300, 32, 4, True), (2, 70000, 16, 4, True)])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+def test_a_nan_or_infinity_stays_in_its_group(L, gpu, NB, S, Cc, G, first, value):
+    rng = np.random.default_rng(6)
+    x = rng.standard_normal((NB, Cc, S) if first else (NB, S, Cc)).astype(np.float32)
+    clean = run_norm(x, G, first=first)
+    n, c, s = NB - 1, Cc // 2 + 1, S // 2
+    g = c // (Cc // G)
+    broken = x.copy()
+    broken[(n, c, s) if first else (n, s, c)] = value
+    y = run_norm(broken, G, first=first)
+    a = y if first else np.swapaxes(y, 1, 2)
+    b = clean if first else np.swapaxes(clean, 1, 2)
+    a, b = a.reshape(NB, G, -1), b.reshape(NB, G, -1)
+    assert np.isnan(a[n, g]).all()
+    keep = np.ones((NB, G), bool)
+    keep[n, g] = False
+    assert bits_equal(a[keep], b[keep])
+
+
+def test_group_norm_of_constant_groups_and_of_one_value(L, gpu):
+    x = np.full((2, 40, 8), 3.25, np.float32)
+    beta = np.arange(8, dtype=np.float32)
+    y = run_norm(x, 2, None, beta)
+    assert bits_equal(y, np.broadcast_to(beta, y.shape))                     # x - mean is exactly 0
+    y = run_norm(np.random.default_rng(0).standard_normal((5, 1, 8)).astype(np.float32), 8, None, beta)
+    assert bits_equal(y, np.broadcast_to(beta, y.shape))
+
+
+def test_group_norm_is_the_same_from_pass_to_pass(L, gpu):
+    x = np.random.default_rng(2).standard_normal((1, 50000, 32)).astype(np.float32)
+    assert bits_equal(run_norm(x, 8), run_norm(x, 8, fill=np.nan))
+
+
+# ---- adapters ------------------------------------------------------------------------------------------------
+class Adapted:
+    def __init__(self, B, K, N, nadapt, rank, act=None, alpha=0.15, bias=True, scale=True, seed=0):
+        rng = np.random.default_rng(seed)
+        f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+        self.W, self.A, self.U = f(N, K) / np.float32(np.sqrt(K)), f(nadapt, rank, K) / np.float32(np.sqrt(K)), f(nadapt, N, rank)
+        self.bias, self.scale = f(N) if bias else None, f(nadapt) if scale else None
+        self.X, self.act, self.alpha, self.shape = f(B, K), act, alpha, (B, K, N, nadapt, rank)
+        self.index = rng.integers(0, nadapt, B).astype(np.int32)
+        self.index[rng.uniform(size=B) < 0.1] = -1
+
+    def plan(self):
+        B, K, N, _, _ = self.shape
+        p = P.Plan()
+        self.t, self.i, self.o = p.tensor(B * K), p.tensor(B), p.tensor(B * N)
+        p.linear_adapters(self.t, self.o, self.i, self.W, self.bias, self.A, self.U, B, self.scale, self.act, self.alpha)
+        return p.finalize(self.t, self.o)
+
+    def run(self, X=None, index=None, p=None):
+        B, K, N, _, _ = self.shape
+        own = p is None
+        p = p or self.plan()
+        p.write(self.i, np.ascontiguousarray(self.index if index is None else index, np.int32))
+        y = p.forward(np.ascontiguousarray(self.X if X is None else X), (B, N))
+        if own:
+            p.close()
+        return y
+
+    def ref(self, X=None, index=None):
+        return R.linear_adapters(self.X if X is None else X, self.index if index is None else index, self.W, self.bias, self.A, self.U, self.scale,
+                                 self.act, self.alpha)
+
+
+ADAPT_SHAPES = [(1, 1, 1, 1, 1), (1, 768, 768, 64, 8), (1, 27, 64, 3, 4), (2, 64, 3, 2, 1), (3, 556, 368, 7, 12), (5, 9, 700, 40, 31), (16, 768, 100, 64, 16),
+                (17, 100, 100, 5, 3), (33, 768, 768, 64, 16), (48, 555, 129, 11, 5), (64, 64, 64, 1, 64), (127, 130, 66, 200, 2), (200, 256, 256, 9, 33),
+                (513, 96, 48, 4, 8), (1000, 27, 64, 15, 4), (1500, 556, 368, 7, 12), (3000, 61, 148, 1000, 6), (4099, 128, 132, 24, 16),
+                (700, 300, 33, 3, 256), (2500, 5, 2, 4, 3), (40, 1000, 1, 6, 7), (9000, 64, 256, 4096, 4), (300, 37, 501, 2, 100)]
+
+
+@pytest.mark.parametrize("B,K,N,nadapt,rank", ADAPT_SHAPES)
+def test_linear_adapters(L, gpu, B, K, N, nadapt, rank):
+    kind = ["relu", "leaky", None, "silu"][(B + K + N) % 4]
+    a = Adapted(B, K, N, nadapt, rank, kind, bias=B % 3 != 0, scale=B % 2 != 0, seed=B + K)
+    p = a.plan()
+    within(a.run(p=p), *a.ref())
+    for index in (np.sort(a.index), np.full(B, nadapt - 1, np.int32), np.full(B, -1, np.int32)):     # the same plan, other indices
+        within(a.run(index=index, p=p), *a.ref(index=index))
+    p.close()
+
+
+@pytest.mark.parametrize("B,K,N,nadapt,rank", [(7, 64, 40, 3, 4), (60, 64, 40, 3, 4), (900, 64, 200, 5, 16)])
+def test_indices_outside_the_adapters_mean_none(L, gpu, B, K, N, nadapt, rank):
+    a = Adapted(B, K, N, nadapt, rank)
+    wild = a.index.copy()
+    wild[wild < 0] = np.resize([-1, -2 ** 31, nadapt, 2 ** 31 - 1, nadapt + 5], (wild < 0).sum())
+    assert bits_equal(a.run(index=wild), a.run())
+
+
+def test_rows_start_without_an_adapter(L, gpu):
+    a = Adapted(40, 64, 48, 3, 4)
+    p = a.plan()
+    y = p.forward(a.X, (40, 48))
+    p.close()
+    assert bits_equal(y, a.run(index=np.full(40, -1)))
+
+
+@pytest.mark.parametrize("B,K,N,nadapt,rank", [(11, 100, 60, 4, 5), (80, 768, 96, 16, 8), (1000, 64, 130, 30, 16), (1000, 27, 64, 15, 4)])
+def test_a_rows_result_does_not_depend_on_the_order_of_rows(L, gpu, B, K, N, nadapt, rank):
+    a = Adapted(B, K, N, nadapt, rank, "silu")
+    order = np.random.default_rng(3).permutation(B)
+    y = a.run()
+    assert bits_equal(a.run(a.X[order], a.index[order]), y[order])
+    assert bits_equal(a.run(), y)
+
+
+@pytest.mark.parametrize("B,K,N,nadapt,rank", [(11, 100, 60, 4, 5), (80, 768, 96, 16, 8), (1000, 64, 130, 30, 16), (1000, 27, 64, 15, 4)])
+def test_nan_and_infinity_stay_with_their_rows_and_adapters(L, gpu, B, K, N, nadapt, rank):
+    a = Adapted(B, K, N, nadapt, rank)
+    a.index[:4] = [0, 1, -1, 2]
+    y = a.run()
+    X = a.X.copy()
+    X[0, K - 1], X[3, 0] = np.nan, np.inf
+    z = a.run(X)
+    keep = np.ones(B, bool)
+    keep[[0, 3]] = False
+    assert np.isnan(z[0]).all() and not np.isfinite(z[3]).any() and bits_equal(z[keep], y[keep])
+    a.U[1, N // 2, rank - 1] = np.nan
+    a.A[2, 0, K // 2] = np.inf
+    z = a.run()
+    keep = (a.index != 1) & (a.index != 2)
+    assert bits_equal(z[keep], y[keep]) and np.isnan(z[1, N // 2]) and not np.isfinite(z[3]).any()
+    other = np.arange(N) != N // 2
+    assert bits_equal(z[a.index == 1][:, other], y[a.index == 1][:, other])
+
+
+# ---- recurrence ----------------------------------------------------------------------------------------------
+class Recur:
+    def __init__(self, q, n, c, time_major, reverse, state=True, lengths=None, carried=False, seed=0):
+        rng = np.random.default_rng(seed)
+        self.src = rng.standard_normal((q * n, 2 * c)).astype(np.float32)
+        self.src[:, :c] = 2 * self.src[:, :c] + 1
+        self.h0 = rng.standard_normal((q, c)).astype(np.float32) if state else None
+        self.args, self.lengths, self.carried = (q, n, c, time_major, reverse), lengths, carried
+        p = self.p = P.Plan()
+        self.t, self.o = p.tensor(self.src.size), p.tensor(q * n * c)
+        self.hi = p.tensor(q * c) if state else -1
+        self.ho = self.hi if carried else p.tensor(q * c)
+        self.le = p.tensor(q) if lengths is not None else -1
+        p.recurrence(self.t, self.o, q, n, c, self.hi, self.ho, self.le, time_major, reverse)
+        p.finalize(self.t, self.o)
+        self.y0 = np.full((q * n, c), -77.0, np.float32)
+        if state:
+            p.write(self.hi, self.h0)
+        if lengths is not None:
+            p.write(self.le, np.asarray(lengths, np.int32))
+
+    def run(self, src=None):
+        q, n, c, _, _ = self.args
+        self.p.write(self.o, self.y0)
+        y = self.p.forward(self.src if src is None else src, self.y0.shape)
+        return y, self.p.read(self.ho, (q, c))
+
+    def ref(self, h0=None, src=None):
+        q, n, c, tm, rev = self.args
+        return R.recurrence(self.src if src is None else src, self.h0 if h0 is None else h0, self.lengths, q, n, c, tm, rev, self.y0)
+
+
+RECUR_SHAPES = [(1, 1, 1), (4736, 1, 64), (3, 2, 5), (1, 100, 3), (2, 1000, 7), (500, 15, 64), (4736, 15, 20), (1, 16384, 4), (7, 777, 33), (3, 4097, 128),
+                (40, 300, 12), (1, 3, 1000), (1000, 40, 1), (2, 6000, 192), (33, 64, 96), (1, 20011, 1)]
+
+
+@pytest.mark.parametrize("time_major,reverse", [(True, False), (True, True), (False, False), (False, True)])
+@pytest.mark.parametrize("q,n,c", RECUR_SHAPES)
+def test_recurrence(L, gpu, q, n, c, time_major, reverse):
+    r = Recur(q, n, c, time_major, reverse, state=(q + n + c) % 4 != 0, seed=q)
+    y, h = r.run()
+    ry, rh, ey, eh = r.ref()
+    within(y, ry, ey)
+    within(h, rh, eh)
+    r.p.close()
+
+
+@pytest.mark.parametrize("time_major,reverse", [(True, False), (True, True), (False, False), (False, True)])
+@pytest.mark.parametrize("q,n,c", [(6, 5, 4), (300, 15, 64), (5, 3000, 24), (40, 700, 3), (17, 129, 30)])
+def test_recurrence_lengths(L, gpu, q, n, c, time_major, reverse):
+    rng = np.random.default_rng(n)
+    lengths = rng.integers(0, n + 1, q)
+    lengths[:5] = [0, n, 1, -7, n + 100]
+    r = Recur(q, n, c, time_major, reverse, lengths=lengths)
+    y, h = r.run()
+    ry, rh, ey, eh = r.ref()
+    within(h, rh, eh)
+    within(y, ry, ey)
+    rows = y.reshape((n, q, c) if time_major else (q, n, c))
+    rows = rows if time_major else np.swapaxes(rows, 0, 1)
+    for s in range(q):
+        m = min(max(int(lengths[s]), 0), n)
+        assert (rows[m:, s] == -77.0).all()                                  # left as they were
+        if m == 0:
+            assert bits_equal(h[s], r.h0[s])
+    r.p.close()
+
+
+def test_lengths_start_as_all_steps_and_states_as_zeros(L, gpu):
+    rng = np.random.default_rng(0)
+    src = rng.standard_normal((12, 16)).astype(np.float32)
+    p = P.Plan()
+    t, o, h, le = p.tensor(192), p.tensor(96), p.tensor(32), p.tensor(4)
+    p.recurrence(t, o, 4, 3, 8, h, h, le)
+    p.finalize(t, o)
+    y = p.forward(src, (12, 8))
+    ry, rh, ey, eh = R.recurrence(src, None, None, 4, 3, 8, True, False, np.zeros((12, 8)))
+    within(y, ry, ey)
+    within(p.read(h, (4, 8)), rh, eh)
+    p.close()
+
+
+@pytest.mark.parametrize("time_major", [True, False])
+def test_a_carried_state_steps_through_time(L, gpu, time_major):
+    """One step per pass with h_in == h_out, 30 passes, is the 30-step recurrence; every pass takes the state the one before left."""
+    q, c, steps = 50, 24, 30
+    r = Recur(q, 1, c, time_major, False, carried=True)
+    rng = np.random.default_rng(9)
+    src = rng.standard_normal((steps, q, 2 * c)).astype(np.float32)
+    ry, rh, ey, eh = R.recurrence(src, r.h0, None, q, steps, c, True, False, np.zeros((steps * q, c)))
+    for t in range(steps):
+        y, h = r.run(src[t])
+        assert bits_equal(y, h)
+        within(y, ry[t * q:(t + 1) * q], ey[t * q:(t + 1) * q])
+    within(h, rh, eh)
+    r.p.close()
+
+
+def test_gates_at_their_limits(L, gpu):
+    """A gate of +inf (or 200) keeps the state to the bit, one of -inf (or -200) replaces it by the candidate; long runs of kept
+    states neither grow nor shrink."""
+    q, n, c = 2, 5000, 8
+    r = Recur(q, n, c, True, False)
+    src = r.src.copy().reshape(n, q, 2 * c)
+    src[:, :, :c] = 200.0
+    src[:, :, :2] = np.inf
+    y, h = r.run(src)
+    assert bits_equal(h, r.h0) and bits_equal(y.reshape(n, q, c)[n // 2], r.h0)
+    src[:, :, :c] = -200.0
+    src[:, :, :2] = -np.inf
+    y, h = r.run(src)
+    assert bits_equal(y.reshape(n, q, c), src[:, :, c:]) and bits_equal(h, src[-1, :, c:])
+    r.p.close()
+
+
+def test_a_nan_spoils_its_own_channel_from_its_step_on(L, gpu):
+    q, n, c = 3, 2500, 20
+    r = Recur(q, n, c, True, False)
+    y, _ = r.run()
+    src = r.src.copy().reshape(n, q, 2 * c)
+    src[1234, 1, c + 7] = np.nan
+    z, h = r.run(src)
+    y, z = y.reshape(n, q, c), z.reshape(n, q, c)
+    assert np.isnan(z[1234:, 1, 7]).all() and np.isnan(h[1, 7]) and np.isnan(h).sum() == 1
+    assert bits_equal(z[:1234], y[:1234])
+    keep = np.ones((q, c), bool)
+    keep[1, 7] = False
+    assert bits_equal(z[1234:, keep], y[1234:, keep])
+
+
+# ---- together ------------------------------------------------------------------------------------------------
+class Block:
+    """27 features -> adapted projection to gates and candidates -> recurrence over the levels of every column, state
+    carried -> group norm + SiLU per head -> adapted projection to 3 outputs."""
+
+    def __init__(self, q, n, c=32, K=27, N=3, nadapt=5, rank=4):
+        rng = np.random.default_rng(11)
+        f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+        rows = q * n
+        self.dims, self.rows = (q, n, c), rows
+        self.w1 = dict(W=f(2 * c, K) / np.float32(np.sqrt(K)), bias=f(2 * c), A=f(nadapt, rank, K) / np.float32(np.sqrt(K)), U=f(nadapt, 2 * c, rank), scale=f(nadapt))
+        self.w2 = dict(W=f(N, c) / np.float32(np.sqrt(c)), bias=None, A=f(nadapt, rank, c) / np.float32(np.sqrt(c)), U=f(nadapt, N, rank), scale=None)
+        self.gamma, self.beta = 1 + f(c) / 5, f(c) / 10
+        self.X, self.h0 = f(rows, K), f(q, c)
+        self.index = rng.integers(-1, nadapt, rows).astype(np.int32)
+        self.lengths = rng.integers(0, n + 1, q).astype(np.int32)
+        self.shapes = (rows, K), (rows, N)
+
+    def fill(self, p):
+        (rows, K), (_, N) = self.shapes
+        q, n, c = self.dims
+        self.x, self.i, self.g, self.h = p.tensor(rows * K), p.tensor(rows), p.tensor(rows * 2 * c), p.tensor(rows * c)
+        self.st, self.le, self.z, self.y = p.tensor(q * c), p.tensor(q), p.tensor(rows * c), p.tensor(rows * N)
+        w = self.w1
+        p.linear_adapters(self.x, self.g, self.i, w["W"], w["bias"], w["A"], w["U"], rows, w["scale"])
+        p.recurrence(self.g, self.h, q, n, c, self.st, self.st, self.le)
+        p.group_norm(self.h, self.z, rows, 1, c, 4, self.gamma, self.beta, act="silu")
+        w = self.w2
+        p.linear_adapters(self.z, self.y, self.i, w["W"], w["bias"], w["A"], w["U"], rows, w["scale"], act="leaky", alpha=0.1)
+        return p.finalize(self.x, self.y)
+
+    def ref(self, h0):
+        q, n, c = self.dims
+        w = self.w1
+        g, _ = R.linear_adapters(self.X, self.index, w["W"], w["bias"], w["A"], w["U"], w["scale"], None, 0)
+        h, state, _, _ = R.recurrence(g, h0, self.lengths, q, n, c, True, False, np.zeros((self.rows, c)))
+        z, _ = R.group_norm(h[:, None], 4, self.gamma, self.beta, 1e-5, "silu", 0, False)
+        w = self.w2
+        y, _ = R.linear_adapters(z[:, 0], self.index, w["W"], None, w["A"], w["U"], None, "leaky", 0.1)
+        valid = (np.arange(n)[:, None] < self.lengths[None]).reshape(-1)
+        return y, state, valid
+
+
+# The block's error: gates are off by 2e-6 of their size and move f by at most a quarter of that, the recurrence sums such
+# errors over 1 / (1 - f) steps, about ten here, and the group norm divides by the spread of eight values, which can be a
+# tenth of their size: 2e-6 * 2.5 * 10, under 1e-4 of the largest output.
+BLOCK_TOL = 1e-4
+
+
+def test_recurrent_block(L, gpu):
+    b = Block(200, 15)
+    p = b.fill(P.Plan())
+    assert p.kernel_names() == ["linear_adapters", "recurrence", "group_norm", "linear_adapters"]
+    p.write(b.i, b.index)
+    p.write(b.le, b.lengths)
+    p.write(b.st, b.h0)
+    h = b.h0
+    for _ in range(3):                                                       # three time steps of the host
+        y = p.forward(b.X, b.shapes[1])
+        ry, h, valid = b.ref(h)
+        assert np.abs(y[valid] - ry[valid]).max() < BLOCK_TOL * np.abs(ry[valid]).max()
+        assert np.abs(p.read(b.st, h.shape) - h).max() < BLOCK_TOL * np.abs(h).max()
+    p.close()
+
+
+def _vp(a):
+    return a.ctypes.data_as(C.c_void_p)
+
+
+@pytest.mark.parametrize("q", [4, 200])
+def test_recurrent_block_through_the_entries_and_a_graph(L, gpu, q, monkeypatch):
+    """mlp_forward on host arrays (the small sizes go through page-locked memory), then mlp_forward_dev captured on its second
+    call and replayed with other work between: every pass advances the carried state once and equals an eager plan's."""
+    monkeypatch.setenv("FORTIS_GRAPH_KEEP", "1")
+    b, e = Block(q, 15), Block(q, 15)
+    p, eager = b.fill(P.Plan()), e.fill(P.Plan())
+    for blk, pl in ((b, p), (e, eager)):
+        pl.write(blk.i, blk.index)
+        pl.write(blk.le, np.full_like(blk.lengths, 15))
+        pl.write(blk.st, blk.h0)
+    step.reset()
+    step.bind(p, b.X.size, b.rows * 3, graph=True)
+    assert step.fortis_model_tensor(b.i) == p.ptr(b.i) and step.fortis_model_tensor(999) is None
+    rng = np.random.default_rng(4)
+    for k in range(9):
+        X = rng.standard_normal(b.X.shape).astype(np.float32)
+        y = np.zeros(b.shapes[1], np.float32)
+        if k == 6:                                                           # another region for every row, between two replays
+            idx = np.roll(b.index, 3)
+            L.fortis_h2d(step.fortis_model_tensor(b.i), _vp(idx), idx.nbytes)
+            eager.write(e.i, idx)
+        if k < 3:
+            step.mlp_forward(X, y)
+        else:
+            step.mlp_upload(X)
+            step.mlp_forward_dev()
+            step.mlp_download(y)
+        assert bits_equal(y, eager.forward(X, b.shapes[1])), k
+    assert step.graph_active()
+    assert bits_equal(p.read(b.st, b.h0.shape), eager.read(e.st, b.h0.shape))
+    step.reset()
+    p.close()
+    eager.close()
+
+
+def test_run_time_extents_of_an_adapted_row_network(L, gpu):
+    """fortis_begin re-sizes a batched step of adapted projections and one-position norms, down and up."""
+    K, c, N, rows = 27, 32, 3, 500
+    rng = np.random.default_rng(3)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    w1, w2 = (f(c, K), f(c), f(4, 3, K), f(4, c, 3)), (f(N, c), f(N), f(4, 3, c), f(4, N, 3))
+    p = P.Plan()
+    x, i, h, z, y = p.tensor(rows * K), p.tensor(rows), p.tensor(rows * c), p.tensor(rows * c), p.tensor(rows * N)
+    p.linear_adapters(x, h, i, w1[0], w1[1], w1[2], w1[3], rows)
+    p.group_norm(h, z, rows, 1, c, 4, act="silu")
+    p.linear_adapters(z, y, i, w2[0], w2[1], w2[2], w2[3], rows)
+    p.finalize(x, y)
+    step.reset()
+    step.bind(p, rows * K, rows * N, verdict="batched", count=rows)
+    for n in (500, 77, 2000, 1):
+        step.fortis_begin(n)
+        X, Y, index = f(n, K), np.zeros((n, N), np.float32), rng.integers(-1, 4, n).astype(np.int32)
+        L.fortis_h2d(step.fortis_model_tensor(i), _vp(index), index.nbytes)
+        step.mlp_forward_batched(X, Y)
+        a, _ = R.linear_adapters(X, index, *w1[:2], w1[2], w1[3], None, None, 0)
+        a, _ = R.group_norm(a[:, None], 4, None, None, 1e-5, "silu", 0, False)
+        a, _ = R.linear_adapters(a[:, 0], index, *w2[:2], w2[2], w2[3], None, None, 0)
+        assert np.abs(Y - a).max() < 1e-4 * np.abs(a).max()
+    step.reset()
+    p.close()
+
+
+def test_image_block_channels_first_behind_a_convolution(L, gpu):
+    """conv 3 x 3 -> group norm + SiLU on the convolution's own order -> channels last -> adapted 1 x 1 projection."""
+    from oracle import oracle as O
+    rng = np.random.default_rng(8)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    Ci, Cc, H, N = 4, 32, 24, 10
+    x, w, b, gamma, beta = f(Ci, H, H), f(Cc, Ci, 3, 3) / np.float32(6), f(Cc), f(Cc), f(Cc)
+    W, A, U = f(N, Cc), f(2, 4, Cc), f(2, N, 4)
+    index = rng.integers(-1, 2, H * H).astype(np.int32)
+    p = P.Plan()
+    t, c1, c2, c3, i, o = p.tensor(x.size), p.tensor(Cc * H * H), p.tensor(Cc * H * H), p.tensor(Cc * H * H), p.tensor(H * H), p.tensor(N * H * H)
+    p.conv2d(t, c1, w, b, Ci, H, H, 1, 1)
+    p.group_norm(c1, c2, 1, H * H, Cc, 8, gamma, beta, act="silu", channels_first=True)
+    p.permute(c2, c3, Cc, H * H, False)
+    p.linear_adapters(c3, o, i, W, None, A, U, H * H)
+    p.finalize(t, o)
+    p.write(i, index)
+    y = p.forward(x, (H * H, N))
+    p.close()
+    r = O.conv2d(x[None], w, pad=(1, 1))[0] + b[:, None, None]
+    r, _ = R.group_norm(r.reshape(1, Cc, -1), 8, gamma, beta, 1e-5, "silu", 0, True)
+    r, _ = R.linear_adapters(r[0].T, index, W, None, A, U, None, None, 0)
+    assert np.abs(y - r).max() < 1e-5 * np.abs(r).max() * 4
+
+
+def test_two_plans_interleaved_share_nothing(L, gpu):
+    """Two plans with the same operators, enqueued in turn without a wait between: each has scratch and states of its own."""
+    a, b = Block(150, 15), Block(150, 15)
+    b.X, b.h0 = -b.X, 2 * b.h0
+    pa, pb = a.fill(P.Plan()), b.fill(P.Plan())
+    for blk, pl in ((a, pa), (b, pb)):
+        pl.write(blk.i, blk.index)
+        pl.write(blk.le, blk.lengths)
+        pl.write(blk.st, blk.h0)
+        pl.write(blk.x, blk.X)
+    for _ in range(2):
+        pa.run()
+        pb.run()
+    for blk, pl in ((a, pa), (b, pb)):
+        _, h, _ = blk.ref(blk.h0)
+        ry, h, valid = blk.ref(h)
+        y = pl.read(blk.y, blk.shapes[1])
+        assert np.abs(y[valid] - ry[valid]).max() < BLOCK_TOL * np.abs(ry[valid]).max()
+        pl.close()

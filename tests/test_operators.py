@@ -1,0 +1,167 @@
+"""Group norm, projections with adapters per row and the gated recurrence without a GPU: what the plan calls refuse, the
+buffers a plan gives their side tensors, and what the step generator writes for them."""
+import ctypes as C
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from fortis_amd import plan as P, shim_hip as SH
+from test_host_logic import pool, stats  # noqa: F401  (fixture)
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _f(*shape):
+    return np.ones(shape, np.float32)
+
+
+@pytest.fixture
+def plan(L):
+    p = P.Plan()
+    yield p
+    p.close()
+
+
+def test_group_norm_refusals(plan, capfd):
+    x, y, small = plan.tensor(2 * 5 * 12), plan.tensor(2 * 5 * 12), plan.tensor(2 * 5 * 12 - 1)
+    ok = dict(src=x, dst=y, NB=2, S=5, C_=12, G=3)
+    for change in (dict(G=5), dict(G=0), dict(G=-3), dict(NB=0), dict(S=0), dict(S=-5), dict(C_=0), dict(eps=-1e-5), dict(eps=float("nan")),
+                   dict(dst=x), dict(src=small), dict(dst=small), dict(src=99), dict(dst=-1), dict(NB=1 << 40, S=1 << 40)):
+        with pytest.raises(ValueError):
+            plan.group_norm(**dict(ok, **change))
+    assert "group_norm" in capfd.readouterr().err
+    assert plan._L.fortis_plan_group_norm(plan.handle, x, y, None, None, 1e-5, 2, 5, 12, 3, 0, 4, 0.0) == -1     # no such activation
+    with pytest.raises(KeyError):
+        plan.group_norm(act="gelu", **ok)
+    plan.group_norm(**ok)                                      # and the call they all vary is accepted
+
+
+def test_overlapping_windows_are_refused(plan):
+    base = plan.tensor(400)
+    a, b, c = plan.view(base, 0, 120), plan.view(base, 116, 120), plan.view(base, 240, 120)
+    for src, dst in ((a, b), (b, a), (a, base), (base, c)):
+        with pytest.raises(ValueError):
+            plan.group_norm(src, dst, 2, 5, 12, 3)
+    plan.group_norm(a, c, 2, 5, 12, 3)
+
+
+def test_linear_adapters_refusals(plan, capfd):
+    x, i, y, small = plan.tensor(6 * 9), plan.tensor(6), plan.tensor(6 * 7), plan.tensor(5)
+    L, h = plan._L, plan.handle
+    W, A, U = _f(7, 9), _f(3, 2, 9), _f(3, 7, 2)
+
+    def call(src=x, dst=y, index=i, w=P._p(W), a=P._p(A), u=P._p(U), B=6, K=9, N=7, nadapt=3, rank=2, act=0):
+        return L.fortis_plan_linear_adapters(h, src, dst, index, w, None, a, u, None, B, K, N, nadapt, rank, act, 0.0)
+
+    for change in (dict(src=y), dict(dst=x), dict(index=x), dict(index=y), dict(index=small), dict(index=-1), dict(index=50), dict(w=None), dict(a=None),
+                   dict(u=None), dict(B=0), dict(B=7), dict(K=0), dict(K=10), dict(N=0), dict(N=8), dict(nadapt=0), dict(nadapt=4097),
+                   dict(rank=0), dict(rank=257), dict(act=-1), dict(act=4), dict(B=1 << 31), dict(K=1 << 22, B=1)):
+        assert call(**change) == -1, change
+    assert "linear_adapters" in capfd.readouterr().err
+    assert call(act=3) == 0
+    for bad in (dict(A=_f(3, 2, 8)), dict(U=_f(3, 6, 2)), dict(U=_f(2, 7, 2)), dict(scale=_f(4)), dict(bias=_f(6))):
+        with pytest.raises(AssertionError):
+            plan.linear_adapters(**dict(dict(src=x, dst=y, index=i, W=W, bias=None, A=A, U=U, B=6), **bad))
+
+
+def test_silu_stays_with_the_operators_that_compute_it(plan):
+    x, y = plan.tensor(36), plan.tensor(36)
+    with pytest.raises(KeyError):
+        plan.linear(x, y, _f(6, 6), None, 6, "silu")
+    assert plan._L.fortis_plan_linear(plan.handle, x, y, P._p(_f(6, 6)), None, 6, 6, 6, 3, 0.0) == -1
+
+
+def test_recurrence_refusals(plan, capfd):
+    q, n, c = 4, 3, 5
+    x, y, h0, h1, le = plan.tensor(q * n * 2 * c), plan.tensor(q * n * c), plan.tensor(q * c), plan.tensor(q * c), plan.tensor(q)
+    small = plan.tensor(3)
+    w = plan.view(x, 40, 20)
+    ok = dict(src=x, dst=y, nseq=q, length=n, ch=c, h_in=h0, h_out=h1, lengths=le)
+    for change in (dict(nseq=0), dict(length=0), dict(ch=0), dict(nseq=5), dict(length=4), dict(ch=6), dict(dst=x), dict(h_in=y), dict(h_out=x),
+                   dict(h_out=y), dict(lengths=h1), dict(lengths=h0), dict(h_in=small), dict(h_out=small), dict(lengths=small), dict(h_in=70),
+                   dict(h_in=w), dict(h_out=w), dict(nseq=1 << 33, length=1 << 30)):
+        with pytest.raises(ValueError):
+            plan.recurrence(**dict(ok, **change))
+    assert "recurrence" in capfd.readouterr().err
+    plan.recurrence(**ok)
+    plan.recurrence(**dict(ok, h_in=h0, h_out=h0))
+    plan.recurrence(**dict(ok, h_in=-1, h_out=-1, lengths=-1))
+
+
+def test_half_overlapping_states_are_refused(plan):
+    x, y, s = plan.tensor(16), plan.tensor(8), plan.tensor(12)
+    a, b = plan.view(s, 0, 8), plan.view(s, 4, 8)
+    with pytest.raises(ValueError):
+        plan.recurrence(x, y, 1, 1, 8, h_in=a, h_out=b)
+    plan.recurrence(x, y, 1, 1, 8, h_in=a, h_out=a)
+
+
+def test_finalized_plans_take_no_operator(pool):  # noqa: F811
+    L, dev = pool
+    p = L.fortis_plan_create()
+    x, y, h = L.fortis_plan_tensor(p, 64), L.fortis_plan_tensor(p, 32), L.fortis_plan_tensor(p, 32)
+    assert L.fortis_plan_recurrence(p, x, y, h, h, -1, 1, 1, 8, 1, 0) == 0
+    assert L.fortis_plan_finalize(p, x, y) == 0
+    assert L.fortis_plan_recurrence(p, x, y, h, h, -1, 1, 1, 8, 1, 0) == -1
+    assert L.fortis_plan_group_norm(p, x, y, None, None, 1e-5, 1, 1, 8, 1, 0, 0, 0.0) == -1
+    assert L.fortis_plan_kernel_name(p, 0) == b"recurrence"
+    L.fortis_plan_destroy(p)
+
+
+def test_states_and_lengths_keep_buffers_of_their_own(pool):  # noqa: F811
+    """A carried state, the lengths and a state that goes out live as long as the plan: no temporary of the pass shares
+    their buffers, also where a state is a window beside one that a kernel writes."""
+    L, dev = pool
+    p = L.fortis_plan_create()
+    T = lambda n: L.fortis_plan_tensor(p, 4 * n)  # noqa: E731
+    x, a, b, c, d = T(16), T(8), T(16), T(8), T(8)
+    both = T(32)
+    written, state = L.fortis_plan_view(p, both, 0, 64), L.fortis_plan_view(p, both, 64, 32)
+    out, le = T(8), T(8)
+    ok = lambda r: r == 0 or pytest.fail("refused")  # noqa: E731
+    ok(L.fortis_plan_recurrence(p, x, a, -1, -1, -1, 1, 1, 8, 1, 0))
+    ok(L.fortis_plan_mask_relu(p, a, c, 1, 8, 8))
+    ok(L.fortis_plan_concat_copy(p, c, written, 1, 8, 0, 2))
+    ok(L.fortis_plan_concat_copy(p, c, written, 1, 8, 1, 2))
+    ok(L.fortis_plan_recurrence(p, written, d, state, out, le, 1, 1, 8, 1, 0))
+    ok(L.fortis_plan_mask_relu(p, d, b, 1, 8, 8))
+    assert L.fortis_plan_finalize(p, x, b) == 0
+    ptr = {t: L.fortis_plan_tensor_ptr(p, t) for t in (x, a, b, c, d, both, out, le)}
+    for t in (both, out, le):
+        assert all(ptr[t] != q for k, q in ptr.items() if k != t), t
+    L.fortis_plan_destroy(p)
+    assert stats(L)[1] == 0
+
+
+def test_model_tensor_without_a_step(L):
+    L.fortis_step_reset()
+    assert L.fortis_model_tensor(0) is None
+
+
+def _block(p, rows, q, n, c):
+    """Projection with adapters -> recurrence -> group norm + SiLU -> projection with adapters."""
+    rng = np.random.default_rng(0)
+    w = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    x, i, g, h, st, z, y = p.tensor(rows * 6), p.tensor(rows), p.tensor(rows * 2 * c), p.tensor(rows * c), p.tensor(q * c), p.tensor(rows * c), p.tensor(rows * 5)
+    p.linear_adapters(x, g, i, w(2 * c, 6), w(2 * c), w(3, 2, 6), w(3, 2 * c, 2), rows, w(3))
+    p.recurrence(g, h, q, n, c, h_in=st, h_out=st)
+    p.group_norm(h, z, rows, 1, c, 2, w(c), w(c), act="silu")
+    p.linear_adapters(z, y, i, w(5, c), None, w(3, 2, c), w(3, 5, 2), rows, act="leaky", alpha=0.1)
+    return p.finalize(x, y)
+
+
+def test_generator_writes_the_operators(tmp_path):
+    ops = _block(SH.OpList(), 12, 4, 3, 8)
+    data = ops.as_json()
+    outline = ops.outline("tensor<12x6xf32>", "tensor<12x5xf32>")
+    text, _ = SH.emit_step({}, outline, data)
+    assert text.count("fortis_plan_linear_adapters(p, ") == 2 and "t[4], t[4], -1, 4L, 3L, 8, 1, 0" in text and "2, 0, 3, 0.0f" in text
+    (tmp_path / "step_tables.c").write_text(text)
+    subprocess.check_call(["gcc", "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(ROOT, "include"), str(tmp_path / "step_tables.c")])
+    for op, key, value in ((0, "index", -1), (0, "act", "gelu"), (1, "h_in", -2), (1, "lengths", 40), (2, "act", "tanh"), (2, "gamma", "w99")):
+        broken = dict(data, ops=[dict(o) for o in data["ops"]])
+        broken["ops"][op][key] = value
+        with pytest.raises(ValueError):
+            SH.emit_step({}, outline, broken)
