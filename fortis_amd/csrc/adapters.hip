@@ -32,7 +32,7 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_simple_kernel(AdaptDesc d, c
         const float *h = H + r * d.rank, *u = d.U + ((long)i * d.N + n) * d.rank;
         for (long j = 0; j < d.rank; j++) acc = fmaf(h[j], u[j], acc);
     }
-    Y[e] = fortis_act_silu(acc + (d.bias ? d.bias[n] : 0.f), d.act, d.alpha);
+    Y[e] = fortis_act_any(acc + (d.bias ? d.bias[n] : 0.f), d.act, d.alpha);
 }
 
 long fortis_adapters_workspace(const AdaptDesc& d, long B) { return B * d.rank * 4; }

@@ -141,14 +141,49 @@ long fortis_recurrence_workspace(const RecurDesc& d);
 void fortis_launch_recurrence(const RecurDesc& d, const float* src, float* dst, const float* h_in, float* h_out, const int* lengths,
                               void* ws, hipStream_t s);
 
-// SiLU as v * sigmoid(v) with the library's exp: v / (1 + exp(-v)) is -0 for v far below zero and v far above it.
 #ifdef __HIPCC__
-__device__ __forceinline__ float fortis_act_silu(float v, int act, float alpha)
+// hi = 1 / (1 + exp(-|g|)) and lo = exp(-|g|) / (1 + exp(-|g|)): sigmoid of |g| and of -|g|, each to its own last digits.
+// The hardware's 2^t takes t = -|g| log2(e) rounded to a float, an error of |g| u in the result; what the rounding left
+// (r, formed with the constant's next digits) goes back in as 1 + r ln 2, and one Newton step follows the hardware's
+// reciprocal: hi is within 3.5 u, lo within 6 u (u = 2^-24), for about 15 instructions; expf and an IEEE division take
+// over 30, half the arithmetic a memory-bound kernel can hide.  From |g| = 150 on exp(-|g|) is 0 in float32; the
+// comparison lets a NaN through.
+__device__ __forceinline__ void fortis_sigmoids(float g, float& hi, float& lo)
+{
+    float a = fabsf(g);
+    a = a > 150.f ? 150.f : a;
+    const float t = a * -1.44269502162933349609375f;
+    float r = fmaf(a, -1.44269502162933349609375f, -t);
+    r = fmaf(a, -1.92596299e-8f, r);
+    float e = __builtin_amdgcn_exp2f(t);
+    e = fmaf(e, r * 0.693147180559945309f, e);
+    const float d = 1.f + e;
+    float q = __builtin_amdgcn_rcpf(d);
+    q = fmaf(fmaf(-d, q, 1.f), q, q);
+    hi = q;
+    lo = e * q;
+}
+// The activations of the plan calls that take FORTIS_ACT_SILU.
+__device__ __forceinline__ float fortis_act_any(float v, int act, float alpha)
 {
     if (act == FORTIS_ACT_RELU) return v > 0.f ? v : 0.f;
     if (act == FORTIS_ACT_LEAKY) return v > 0.f ? v : alpha * v;
-    if (act == FORTIS_ACT_SILU) return v / (1.f + expf(-v));
+    if (act == FORTIS_ACT_SILU) {
+        float hi, lo;
+        fortis_sigmoids(v, hi, lo);
+        return v * (v >= 0.f ? hi : lo);
+    }
     return v;
+}
+// n / d for n < 2^31 by one multiplication: with 2^l the power of two at or above d, m = ceil(2^(31 + l) / d) is at most
+// 2^32 - 1 and n m >> (31 + l) is the quotient.
+struct FastDiv { unsigned m, sh, d; };
+__device__ __forceinline__ unsigned fortis_div(unsigned n, const FastDiv& f) { return (unsigned)(((unsigned long long)n * f.m) >> f.sh); }
+static inline FastDiv fortis_fast_div(unsigned d)
+{
+    unsigned l = 0;
+    while ((1ull << l) < d) l++;
+    return { (unsigned)(((1ull << (31 + l)) + d - 1) / d), 31 + l, d };
 }
 #endif
 

@@ -1,45 +1,625 @@
 // Group normalisation with an activation (include/fortis_step.h, fortis_plan_group_norm):
 //     y = act(gamma_c (x - mean_{n,g}) / sqrt(var_{n,g} + eps) + beta_c)
-// over the S * C / G values of every (sample, group), channels last or first.
+// over the S * C / G values of every (sample, group) -- an "instance" below -- channels last or first.
+//
+// Memory-bound: 8 bytes and about ten operations a value.  Three forms by the size of an instance:
+//   lanes    up to 2048 values: 1 to 64 lanes hold the instance in registers, one read, one write, no barrier;
+//   block    up to 32768: one workgroup holds an instance (or the neighbouring instances whose channels share 128-byte
+//            lines) in registers, one read, one write;
+//   split    beyond: one launch sums over chunks of every sample, a second joins a sample's chunk sums and normalises.  The
+//            input is read twice, the second time from the caches as far as they hold it.
+// Sums.  Where the values stay in registers the mean comes first and the squares of what is left after it second, about
+// the instance's first value as a pivot (a pivot inside the data is at most sqrt(n) spreads from the mean), in float32.  The
+// split form has to take both sums in one read: every thread sums a few dozen values about the first one it meets, and from
+// there on everything is joined in float64 about the instance's first value, where cancellation costs digits that are there
+// to spare.  The mean is then subtracted as a float32 pair.
 #include "common.h"
 
-#define GN_THREADS 256
-
-// One workgroup per (sample, group), two reads of the input.  Sums are taken about the group's first value in float64.
-__global__ __launch_bounds__(GN_THREADS) void norm_simple_kernel(NormDesc d, const float* __restrict__ x, float* __restrict__ y)
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+template <int V> struct VecOf { typedef float T; };
+template <> struct VecOf<2> { typedef v2f T; };
+template <> struct VecOf<4> { typedef v4f T; };
+template <int V> struct Vals { float v[V]; };
+template <int V> __device__ __forceinline__ Vals<V> ld(const float* p)
 {
-    __shared__ double red[2][GN_THREADS];
-    const long n = blockIdx.x / d.G, g = blockIdx.x % d.G;
-    const long cg = d.C / d.G, count = d.S * cg;
-    auto at = [&](long e) {
-        return d.first ? ((n * d.C + g * cg) * d.S + e) : ((n * d.S + e / cg) * d.C + g * cg + e % cg);
-    };
-    const float pivot = x[at(0)];
-    double s1 = 0, s2 = 0;
-    for (long e = threadIdx.x; e < count; e += GN_THREADS) {
-        const double v = (double)x[at(e)] - (double)pivot;
-        s1 += v; s2 += v * v;
-    }
-    red[0][threadIdx.x] = s1; red[1][threadIdx.x] = s2;
-    __syncthreads();
-    for (int o = GN_THREADS / 2; o; o >>= 1) {
-        if ((int)threadIdx.x < o) { red[0][threadIdx.x] += red[0][threadIdx.x + o]; red[1][threadIdx.x] += red[1][threadIdx.x + o]; }
-        __syncthreads();
-    }
-    const double dm = red[0][0] / (double)count, raw = red[1][0] / (double)count - dm * dm;
-    const double var = raw < 0 ? 0 : raw;       // a NaN stays one
-    const float rstd = (float)(1.0 / sqrt(var + (double)d.eps));
-    for (long e = threadIdx.x; e < count; e += GN_THREADS) {
-        const long a = at(e), c = g * cg + (d.first ? e / d.S : e % cg);
-        const float v = (float)(((double)x[a] - (double)pivot) - dm) * rstd;
-        y[a] = fortis_act_silu(fmaf(v, d.gamma ? d.gamma[c] : 1.f, d.beta ? d.beta[c] : 0.f), d.act, d.alpha);
+    Vals<V> r;
+    const typename VecOf<V>::T t = *(const typename VecOf<V>::T*)p;
+    __builtin_memcpy(r.v, &t, sizeof t);
+    return r;
+}
+template <int V> __device__ __forceinline__ void st(float* p, const Vals<V>& r)
+{
+    typename VecOf<V>::T t;
+    __builtin_memcpy(&t, r.v, sizeof t);
+    *(typename VecOf<V>::T*)p = t;
+}
+
+#define GN_LANES_MAX 2048      // values of an instance in the lanes form
+#define GN_BLOCK_MAX 32768     // in the block form: 1024 threads x 32
+#define GN_BLOCK_EDGE 32       // channels whose floats fill a 128-byte line
+
+// Sum over the 2^k lanes around this one (L = 2^k).
+template <int L> __device__ __forceinline__ float sum_lanes(float v)
+{
+#pragma unroll
+    for (int o = L / 2; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+struct NormArgs {
+    NormDesc d;
+    const float* x;
+    float* y;
+    long cg, count;             // channels a group, values an instance
+    FastDiv row;                // vectors of an instance's row (channels last), or of a channel (channels first)
+};
+
+// ---- lanes form --------------------------------------------------------------------------------------------------
+// Element e (vectors of V) of an instance: position e / (cg / V), channel V * (e % (cg / V)); channels first: V values of
+// channel e / (S / V).  L lanes share an instance, E vectors a lane; a wave takes 64 / L neighbouring instances at a time.
+template <int V, int L, int E>
+__global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
+{
+    const NormDesc& d = a.d;
+    const int lane = threadIdx.x & 63, sub = lane & (L - 1);
+    const unsigned nv = (unsigned)(a.count / V);
+    const long step = (long)gridDim.x * (256 / L);
+    for (long first = (long)blockIdx.x * (256 / L); first < total; first += step) {
+        const long inst = first + threadIdx.x / L;
+        const bool on = inst < total;
+        const long n = on ? inst / d.G : 0;
+        const int g = on ? (int)(inst - n * d.G) : 0;
+        const long base = d.first ? (n * d.C + g * a.cg) * d.S : n * d.S * d.C + g * a.cg;
+        Vals<V> v[E];
+        unsigned ch[E];
+        long at[E];
+        bool have[E];
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            const unsigned e = sub + k * L;
+            have[k] = on && e < nv;
+            const unsigned q = fortis_div(e, a.row);
+            if (d.first) { at[k] = base + (long)e * V; ch[k] = (unsigned)(g * a.cg) + q; }
+            else { const unsigned c = (e - q * a.row.d) * V; at[k] = base + (long)q * d.C + c; ch[k] = (unsigned)(g * a.cg) + c; }
+            if (have[k]) v[k] = ld<V>(a.x + at[k]);
+        }
+        const float pivot = __shfl(v[0].v[0], lane & ~(L - 1), 64);
+        const float inv = 1.f / (float)a.count;
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; k++)
+#pragma unroll
+            for (int c = 0; c < V; c++) { v[k].v[c] -= pivot; s += have[k] ? v[k].v[c] : 0.f; }
+        const float mean = sum_lanes<L>(s) * inv;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; k++)
+#pragma unroll
+            for (int c = 0; c < V; c++) { v[k].v[c] -= mean; const float t = have[k] ? v[k].v[c] : 0.f; s = fmaf(t, t, s); }
+        const float rstd = 1.f / sqrtf(sum_lanes<L>(s) * inv + d.eps);
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            if (!have[k]) continue;
+            Vals<V> ga, be, o;
+            if (d.first) {
+                const float gs = d.gamma ? d.gamma[ch[k]] : 1.f, bs = d.beta ? d.beta[ch[k]] : 0.f;
+#pragma unroll
+                for (int c = 0; c < V; c++) { ga.v[c] = gs; be.v[c] = bs; }
+            } else {
+#pragma unroll
+                for (int c = 0; c < V; c++) { ga.v[c] = 1.f; be.v[c] = 0.f; }
+                if (d.gamma) ga = ld<V>(d.gamma + ch[k]);
+                if (d.beta) be = ld<V>(d.beta + ch[k]);
+            }
+#pragma unroll
+            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, ga.v[c], be.v[c]), d.act, d.alpha);
+            st<V>(a.y + at[k], o);
+        }
     }
 }
 
-long fortis_norm_workspace(const NormDesc&) { return 0; }
-
-void fortis_launch_group_norm(const NormDesc& d, const float* x, float* y, void*, hipStream_t s)
+// ---- block form --------------------------------------------------------------------------------------------------
+// Sum of one float per thread over the workgroup's T threads, the same order in every call; red: T / 64 floats.
+template <int T> __device__ __forceinline__ float sum_block(float v, float* red)
 {
-    hipLaunchKernelGGL(norm_simple_kernel, dim3((unsigned)(d.NB * d.G)), dim3(GN_THREADS), 0, s, d, x, y);
+    v = sum_lanes<64>(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < T / 64; w++) s += red[w];
+    __syncthreads();
+    return s;
+}
+// One instance per workgroup: vectors e = thread + k T of it.
+template <int V, int T, int E>
+__global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
+{
+    __shared__ float red[T / 64];
+    const NormDesc& d = a.d;
+    const unsigned nv = (unsigned)(a.count / V);
+    for (long inst = blockIdx.x; inst < total; inst += gridDim.x) {
+        const long n = inst / d.G;
+        const int g = (int)(inst - n * d.G);
+        const float* x = a.x + (d.first ? (n * d.C + g * a.cg) * d.S : n * d.S * d.C + g * a.cg);
+        float* y = a.y + (x - a.x);
+        Vals<V> v[E];
+        const unsigned gc = (unsigned)(g * a.cg);
+        // element e of the instance: where it lies and its (first) channel
+        auto place = [&](unsigned e, long& at, unsigned& ch) __attribute__((always_inline)) {
+            const unsigned q = fortis_div(e, a.row);
+            if (d.first) { at = (long)e * V; ch = gc + q; }
+            else { const unsigned c = (e - q * a.row.d) * V; at = (long)q * d.C + c; ch = gc + c; }
+        };
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            const unsigned e = threadIdx.x + k * T;
+            long at;
+            unsigned ch;
+            place(e, at, ch);
+            if (e < nv) v[k] = ld<V>(x + at);
+            if (k % 8 == 7) asm volatile("" ::: "memory");       // eight addresses at a time
+        }
+        const float pivot = x[0], inv = 1.f / (float)a.count;
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; k++)
+#pragma unroll
+            for (int c = 0; c < V; c++) { v[k].v[c] -= pivot; s += threadIdx.x + k * T < nv ? v[k].v[c] : 0.f; }
+        const float mean = sum_block<T>(s, red) * inv;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; k++)
+#pragma unroll
+            for (int c = 0; c < V; c++) { v[k].v[c] -= mean; const float t = threadIdx.x + k * T < nv ? v[k].v[c] : 0.f; s = fmaf(t, t, s); }
+        const float rstd = 1.f / sqrtf(sum_block<T>(s, red) * inv + d.eps);
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            unsigned e = threadIdx.x + k * T, ch;
+            if (e >= nv) continue;
+            asm volatile("" : "+v"(e));          // formed again: E addresses kept in registers would spill
+            long at;
+            place(e, at, ch);
+            Vals<V> o;
+#pragma unroll
+            for (int c = 0; c < V; c++) {
+                const unsigned i = ch + (d.first ? 0 : c);
+                o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, d.gamma ? d.gamma[i] : 1.f, d.beta ? d.beta[i] : 0.f), d.act, d.alpha);
+            }
+            st<V>(y + at, o);
+        }
+    }
+}
+// Channels last, `gs` neighbouring groups of one sample per workgroup (together up to a 128-byte line of channels or a little
+// more): a thread keeps its column of V channels, which lie in one group, and takes every rows-th position.
+template <int V, int T, int E>
+__global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs, int slices, long total)
+{
+    __shared__ float part[T], sums[T];
+    const NormDesc& d = a.d;
+    const int tid = threadIdx.x;
+    for (long item = blockIdx.x; item < total; item += gridDim.x) {
+        const long n = item / slices;
+        const int g0 = (int)(item - n * slices) * gs, ng = d.G - g0 < gs ? (int)(d.G - g0) : gs;
+        const int cgv = (int)(a.cg / V), wv = ng * cgv, rows = T / wv;
+        const int col = tid % wv, row = tid / wv, gl = col / cgv;
+        const bool on = row < rows;
+        const unsigned c0 = (unsigned)(g0 * a.cg) + col * V;
+        const long base = n * d.S * d.C + c0;
+        Vals<V> v[E];
+#pragma unroll
+        for (int k = 0; k < E; k++)
+            if (on && row + k * rows < d.S) v[k] = ld<V>(a.x + base + (long)(row + k * rows) * d.C);
+        const float pivot = a.x[n * d.S * d.C + (g0 + gl) * a.cg], inv = 1.f / (float)a.count;
+        // the group's sum: its threads are (row, columns gl cgv .. + cgv); one wave adds each group's partial sums
+        auto group_sum = [&](float s) __attribute__((always_inline)) {
+            part[tid] = on ? s : 0.f;
+            __syncthreads();
+            for (int g = tid >> 6; g < ng; g += T / 64) {
+                float t = 0.f;
+                for (int r = 0; r < rows; r++)
+                    for (int c = tid & 63; c < cgv; c += 64) t += part[r * wv + g * cgv + c];
+                t = sum_lanes<64>(t);
+                if ((tid & 63) == 0) sums[g] = t;
+            }
+            __syncthreads();
+            return sums[gl];
+        };
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; k++)
+#pragma unroll
+            for (int c = 0; c < V; c++) { v[k].v[c] -= pivot; s += on && row + k * rows < d.S ? v[k].v[c] : 0.f; }
+        const float mean = group_sum(s) * inv;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; k++)
+#pragma unroll
+            for (int c = 0; c < V; c++) { v[k].v[c] -= mean; const float t = on && row + k * rows < d.S ? v[k].v[c] : 0.f; s = fmaf(t, t, s); }
+        const float rstd = 1.f / sqrtf(group_sum(s) * inv + d.eps);
+        if (!on) continue;
+        Vals<V> ga, be;
+#pragma unroll
+        for (int c = 0; c < V; c++) { ga.v[c] = d.gamma ? d.gamma[c0 + c] : 1.f; be.v[c] = d.beta ? d.beta[c0 + c] : 0.f; }
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            if (row + k * rows >= d.S) continue;
+            Vals<V> o;
+#pragma unroll
+            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, ga.v[c], be.v[c]), d.act, d.alpha);
+            st<V>(a.y + base + (long)(row + k * rows) * d.C, o);
+        }
+    }
+}
+
+// ---- split form --------------------------------------------------------------------------------------------------
+#define GS_THREADS 1024
+#define GS_AHEAD 4             // loads a thread has in flight while it normalises
+struct SplitShape {
+    long chunks, per;        // chunks of a sample (an instance with channels first), positions (vectors) a chunk
+    int V;                   // floats a thread loads at a time
+    int gs, slices;          // channels last: groups and workgroups across the channels
+    int blocks;              // workgroups across one group's channels (1 unless a group is wider than 1024 vectors)
+    long parts;              // partial sums an instance has
+};
+
+// Partial sums of `n` values about P: a1 = sum(v - P), a2 = sum((v - P)^2), from sums about a pivot of the thread's own.
+__device__ __forceinline__ void about(float pivot, int n, float s1, float s2, double P, double& a1, double& a2)
+{
+    const double dn = (double)n;
+    a1 = a2 = 0.0;
+    if (n == 0) return;
+    const double t1 = dn * ((double)pivot - P) + (double)s1;
+    const double m2 = (double)s2 - (double)s1 * (double)s1 / dn;       // centred, of this thread's values
+    a1 = t1; a2 = m2 + t1 * t1 / dn;
+}
+__device__ __forceinline__ double sum_wave(double v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// Channels last.  The slice's columns (V channels each) by rows of the chunk; a thread keeps its column.
+template <int V>
+__global__ __launch_bounds__(GS_THREADS) void norm_sums_kernel(NormArgs a, SplitShape h, double2* __restrict__ out)
+{
+    __shared__ double2 part[GS_THREADS];
+    const NormDesc& d = a.d;
+    const int tid = threadIdx.x;
+    const long chunk = blockIdx.x % h.chunks, rest = blockIdx.x / h.chunks;
+    const int across = h.slices * h.blocks;
+    const long n = rest / across;
+    const int sl = (int)(rest - n * across) / h.blocks, bl = (int)(rest - n * across) % h.blocks;
+    const int g0 = sl * h.gs, ng = d.G - g0 < h.gs ? (int)(d.G - g0) : h.gs;
+    const long c_lo = (long)g0 * a.cg + (long)bl * GS_THREADS * V;                    // first channel of the workgroup
+    const long c_hi = h.blocks > 1 ? ((long)g0 + 1) * a.cg : (long)(g0 + ng) * a.cg;
+    const int wv = (int)((c_hi - c_lo) / V < GS_THREADS ? (c_hi - c_lo) / V : GS_THREADS), rows = GS_THREADS / wv;
+    const int col = tid % wv, row = tid / wv;
+    const long r0 = chunk * h.per, r1 = r0 + h.per < d.S ? r0 + h.per : d.S;
+    const float* x = a.x + (n * d.S) * d.C + c_lo + col * V;
+    float p[V], s1[V], s2[V];
+    int cnt = 0;
+#pragma unroll
+    for (int c = 0; c < V; c++) p[c] = s1[c] = s2[c] = 0.f;
+    if (row < rows && r0 + row < r1) {
+        const Vals<V> f = ld<V>(x + (r0 + row) * d.C);
+#pragma unroll
+        for (int c = 0; c < V; c++) p[c] = f.v[c];
+#pragma unroll 4
+        for (long r = r0 + row; r < r1; r += rows) {
+            const Vals<V> v = ld<V>(x + r * d.C);
+#pragma unroll
+            for (int c = 0; c < V; c++) { const float t = v.v[c] - p[c]; s1[c] += t; s2[c] = fmaf(t, t, s2[c]); }
+            cnt++;
+        }
+    }
+    // join: a column's V channels lie in one group unless the slice is all channels and V does not divide cg
+    const int gfirst = h.blocks > 1 ? g0 : (int)((c_lo + col * V) / a.cg);
+    const bool one = a.cg % V == 0;
+    for (int c = 0; c < (one ? 1 : V); c++) {
+        double a1 = 0, a2 = 0;
+        if (one) {
+            const double P = a.x[n * d.S * d.C + gfirst * a.cg];
+#pragma unroll
+            for (int k = 0; k < V; k++) { double b1, b2; about(p[k], cnt, s1[k], s2[k], P, b1, b2); a1 += b1; a2 += b2; }
+        } else {
+            // component c of every column; the groups then take the components one after the other
+            const int g = (int)((c_lo + col * V + c) / a.cg);
+            float pc = 0, s1c = 0, s2c = 0;
+#pragma unroll
+            for (int k = 0; k < V; k++) if (k == c) { pc = p[k]; s1c = s1[k]; s2c = s2[k]; }
+            about(pc, cnt, s1c, s2c, (double)a.x[n * d.S * d.C + g * a.cg], a1, a2);
+        }
+        __syncthreads();
+        part[tid] = make_double2(a1, a2);
+        __syncthreads();
+        for (int g = tid >> 6; g < ng; g += GS_THREADS / 64) {
+            // columns that hold a channel of group g0 + g in component c (any component when V divides cg)
+            const long lo = h.blocks > 1 ? 0 : (long)g * a.cg, hi = h.blocks > 1 ? (long)wv * V : lo + a.cg;
+            const int k0 = one ? (int)(lo / V) : (int)((lo - c + V - 1 + V) / V - 1), k1 = one ? (int)(hi / V) : (int)((hi - c + V - 1 + V) / V - 1);
+            double t1 = 0, t2 = 0;
+            const int w = k1 - k0;
+            for (int i = tid & 63; i < rows * w; i += 64) {
+                const double2 q = part[(i / w) * wv + k0 + i % w];
+                t1 += q.x; t2 += q.y;
+            }
+            t1 = sum_wave(t1); t2 = sum_wave(t2);
+            if ((tid & 63) == 0) {
+                double2* o = out + (n * d.G + g0 + g) * h.parts + chunk * h.blocks + bl;
+                if (c == 0) *o = make_double2(t1, t2);
+                else *o = make_double2(o->x + t1, o->y + t2);
+            }
+        }
+    }
+}
+// Channels first: chunks of `per` vectors of an instance, which is contiguous.
+template <int V>
+__global__ __launch_bounds__(GS_THREADS) void norm_sums_first_kernel(NormArgs a, SplitShape h, double2* __restrict__ out)
+{
+    __shared__ double2 part[GS_THREADS / 64];
+    const int tid = threadIdx.x;
+    const long chunk = blockIdx.x % h.chunks, inst = blockIdx.x / h.chunks;
+    const float* x = a.x + inst * a.count;
+    const long nv = a.count / V, e0 = chunk * h.per, e1 = e0 + h.per < nv ? e0 + h.per : nv;
+    float p = 0.f, s1 = 0.f, s2 = 0.f;
+    int cnt = 0;
+    if (e0 + tid < e1) {
+        p = x[(e0 + tid) * V];
+#pragma unroll 4
+        for (long e = e0 + tid; e < e1; e += GS_THREADS) {
+            const Vals<V> v = ld<V>(x + e * V);
+#pragma unroll
+            for (int c = 0; c < V; c++) { const float t = v.v[c] - p; s1 += t; s2 = fmaf(t, t, s2); }
+            cnt += V;
+        }
+    }
+    double a1, a2;
+    about(p, cnt, s1, s2, (double)x[0], a1, a2);
+    a1 = sum_wave(a1); a2 = sum_wave(a2);
+    if ((tid & 63) == 0) part[tid >> 6] = make_double2(a1, a2);
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < GS_THREADS / 64; w++) { a1 += part[w].x; a2 += part[w].y; }
+        out[inst * h.parts + chunk] = make_double2(a1, a2);
+    }
+}
+
+// mean (as a pair) and 1 / sqrt(var + eps) of an instance from its partial sums, by one wave.
+struct Stat { float hi, lo, rstd, pad; };
+__device__ __forceinline__ Stat join(const double2* part, long parts, double pivot, double count, float eps)
+{
+    double t1 = 0, t2 = 0;
+    for (long i = threadIdx.x & 63; i < parts; i += 64) { const double2 q = part[i]; t1 += q.x; t2 += q.y; }
+    t1 = sum_wave(t1) / count; t2 = sum_wave(t2) / count;
+    double var = t2 - t1 * t1;
+    if (var < 0) var = 0;                                  // a NaN stays one
+    const double mean = pivot + t1;
+    Stat s;
+    s.hi = (float)mean; s.lo = (float)(mean - (double)s.hi); s.rstd = (float)(1.0 / sqrt(var + (double)eps)); s.pad = 0.f;
+    return s;
+}
+// Channels last: the same chunks and columns as the sums, last position first (what the caches still hold).
+template <int V>
+__global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, SplitShape h, const double2* __restrict__ in)
+{
+    __shared__ Stat stat[GS_THREADS];
+    const NormDesc& d = a.d;
+    const int tid = threadIdx.x;
+    const long chunk = blockIdx.x % h.chunks, rest = blockIdx.x / h.chunks;
+    const int across = h.slices * h.blocks;
+    const long n = rest / across;
+    const int sl = (int)(rest - n * across) / h.blocks, bl = (int)(rest - n * across) % h.blocks;
+    const int g0 = sl * h.gs, ng = d.G - g0 < h.gs ? (int)(d.G - g0) : h.gs;
+    const long c_lo = (long)g0 * a.cg + (long)bl * GS_THREADS * V;
+    const long c_hi = h.blocks > 1 ? ((long)g0 + 1) * a.cg : (long)(g0 + ng) * a.cg;
+    const int wv = (int)((c_hi - c_lo) / V < GS_THREADS ? (c_hi - c_lo) / V : GS_THREADS), rows = GS_THREADS / wv;
+    for (int g = tid >> 6; g < ng; g += GS_THREADS / 64) {
+        const Stat s = join(in + (n * d.G + g0 + g) * h.parts, h.parts, (double)a.x[n * d.S * d.C + (g0 + g) * a.cg], (double)a.count, d.eps);
+        if ((tid & 63) == 0) stat[g] = s;
+    }
+    __syncthreads();
+    const int col = tid % wv, row = tid / wv;
+    if (row >= rows) return;
+    const long c0 = c_lo + col * V;
+    float hi[V], lo[V], sc[V], be[V];
+#pragma unroll
+    for (int c = 0; c < V; c++) {
+        const Stat s = stat[h.blocks > 1 ? 0 : (int)((c0 + c) / a.cg) - g0];
+        hi[c] = s.hi; lo[c] = s.lo;
+        sc[c] = s.rstd * (d.gamma ? d.gamma[c0 + c] : 1.f);
+        be[c] = d.beta ? d.beta[c0 + c] : 0.f;
+    }
+    const long r0 = chunk * h.per, r1 = r0 + h.per < d.S ? r0 + h.per : d.S;
+    const long off = n * d.S * d.C + c0;
+    if (r0 + row >= r1) return;
+    for (long r = r0 + row + (r1 - 1 - r0 - row) / rows * rows; r >= r0; r -= GS_AHEAD * rows) {
+        Vals<V> v[GS_AHEAD];
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++)
+            if (r - k * rows >= r0) v[k] = ld<V>(a.x + off + (r - k * rows) * d.C);
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++) {
+            if (r - k * rows < r0) break;
+#pragma unroll
+            for (int c = 0; c < V; c++) v[k].v[c] = fortis_act_any(fmaf((v[k].v[c] - hi[c]) - lo[c], sc[c], be[c]), d.act, d.alpha);
+            st<V>(a.y + off + (r - k * rows) * d.C, v[k]);
+        }
+    }
+}
+template <int V>
+__global__ __launch_bounds__(GS_THREADS) void norm_apply_first_kernel(NormArgs a, SplitShape h, const double2* __restrict__ in)
+{
+    __shared__ Stat stat;
+    const NormDesc& d = a.d;
+    const int tid = threadIdx.x;
+    const long chunk = blockIdx.x % h.chunks, inst = blockIdx.x / h.chunks;
+    const long g = inst % d.G;
+    const float* x = a.x + inst * a.count;
+    float* y = a.y + inst * a.count;
+    if (tid < 64) {
+        const Stat s = join(in + inst * h.parts, h.parts, (double)x[0], (double)a.count, d.eps);
+        if (tid == 0) stat = s;
+    }
+    __syncthreads();
+    const Stat s = stat;
+    const long nv = a.count / V, e0 = chunk * h.per, e1 = e0 + h.per < nv ? e0 + h.per : nv;
+    const bool small = nv < (1L << 31);
+    if (e0 + tid >= e1) return;
+    for (long e = e0 + tid + (e1 - 1 - e0 - tid) / GS_THREADS * GS_THREADS; e >= e0; e -= GS_AHEAD * GS_THREADS) {
+        Vals<V> v[GS_AHEAD];
+        float sc[GS_AHEAD], be[GS_AHEAD];
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++) {
+            const long i = e - k * GS_THREADS;
+            if (i < e0) break;
+            v[k] = ld<V>(x + i * V);
+            const long c = g * a.cg + (small ? (long)fortis_div((unsigned)i, a.row) : i / (d.S / V));
+            sc[k] = s.rstd * (d.gamma ? d.gamma[c] : 1.f);
+            be[k] = d.beta ? d.beta[c] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++) {
+            const long i = e - k * GS_THREADS;
+            if (i < e0) break;
+#pragma unroll
+            for (int c = 0; c < V; c++) v[k].v[c] = fortis_act_any(fmaf((v[k].v[c] - s.hi) - s.lo, sc[k], be[k]), d.act, d.alpha);
+            st<V>(y + i * V, v[k]);
+        }
+    }
+}
+
+// ---- choice ------------------------------------------------------------------------------------------------------
+static NormDesc norm_normal(const NormDesc& in)
+{
+    NormDesc d = in;
+    if (d.S == 1) d.first = 0;          // the two orders are the same
+    return d;
+}
+static SplitShape split_shape(const NormDesc& d)
+{
+    SplitShape h = {};
+    const long cg = d.C / d.G;
+    const long want = 256;              // workgroups of 1024 threads: one for every compute unit
+    if (d.first) {
+        h.V = d.S % 4 == 0 ? 4 : d.S % 2 == 0 ? 2 : 1;
+        const long nv = cg * d.S / h.V, insts = d.NB * d.G;
+        h.chunks = cdiv(want, insts);
+        if (h.chunks > cdiv(nv, GS_THREADS)) h.chunks = cdiv(nv, GS_THREADS);
+        h.per = cdiv(nv, h.chunks);
+        h.chunks = cdiv(nv, h.per);
+        h.gs = h.slices = h.blocks = 1;
+        h.parts = h.chunks;
+        return h;
+    }
+    h.V = d.C % 4 == 0 && d.C <= 4 * GS_THREADS ? 4 : cg % 4 == 0 ? 4 : cg % 2 == 0 ? 2 : 1;
+    const long fit = GS_THREADS * h.V;                  // channels a workgroup spans
+    h.gs = (int)(d.C <= fit ? d.G : cg <= fit ? fit / cg : 1);
+    h.slices = (int)cdiv(d.G, h.gs);
+    h.blocks = (int)cdiv(cg, fit);
+    const long across = (long)h.slices * h.blocks * d.NB;
+    const long width = d.C <= fit ? d.C : (long)h.gs * cg < fit ? (long)h.gs * cg : fit;
+    const long pass = GS_THREADS / cdiv(width, h.V) ? GS_THREADS / cdiv(width, h.V) : 1;      // rows a pass of the workgroup covers
+    h.chunks = cdiv(want, across);
+    if (h.chunks > cdiv(d.S, pass)) h.chunks = cdiv(d.S, pass);
+    h.per = cdiv(d.S, h.chunks);
+    h.chunks = cdiv(d.S, h.per);
+    h.parts = h.chunks * h.blocks;
+    return h;
+}
+
+long fortis_norm_workspace(const NormDesc& in)
+{
+    const NormDesc d = norm_normal(in);
+    if (d.S * (d.C / d.G) <= GN_BLOCK_MAX) return 0;
+    return d.NB * d.G * split_shape(d).parts * (long)sizeof(double2);
+}
+
+template <int V> static void launch_lanes(const NormArgs& a, long total, hipStream_t s)
+{
+    const long nv = a.count / V;
+    auto grid = [&](int L) { const long g = cdiv(total, 256 / L); return dim3((unsigned)(g < 8192 ? g : 8192)); };
+#define GN_LANES(L, E) hipLaunchKernelGGL((norm_lanes_kernel<V, L, E>), grid(L), dim3(256), 0, s, a, total)
+    if (nv <= 1) GN_LANES(1, 1);
+    else if (nv <= 2) GN_LANES(2, 1);
+    else if (nv <= 4) GN_LANES(4, 1);
+    else if (nv <= 8) GN_LANES(8, 1);
+    else if (nv <= 16) GN_LANES(16, 1);
+    else if (nv <= 32) GN_LANES(32, 1);
+    else if (nv <= 64) GN_LANES(64, 1);
+    else if (nv <= 128) GN_LANES(64, 2);
+    else if (nv <= 256) GN_LANES(64, 4);
+    else GN_LANES(64, 8);
+#undef GN_LANES
+}
+template <int V> static void launch_block(const NormArgs& a, int gs, hipStream_t s)
+{
+    const NormDesc& d = a.d;
+    if (gs == 1) {
+        const long total = d.NB * d.G, nv = a.count / V;
+        const dim3 grid((unsigned)(total < 65536 ? total : 65536));
+        if (nv <= 256 * 4) hipLaunchKernelGGL((norm_block_kernel<V, 256, 4>), grid, dim3(256), 0, s, a, total);
+        else if (nv <= 256 * 8) hipLaunchKernelGGL((norm_block_kernel<V, 256, 8>), grid, dim3(256), 0, s, a, total);
+        else if (nv <= 1024 * 4) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 4>), grid, dim3(1024), 0, s, a, total);
+        else if (nv <= 1024 * 8) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 8>), grid, dim3(1024), 0, s, a, total);
+        if constexpr (V <= 2) if (nv > 1024 * 8 && nv <= 1024 * 16) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 16>), grid, dim3(1024), 0, s, a, total);
+        if constexpr (V == 1) if (nv > 1024 * 16) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 32>), grid, dim3(1024), 0, s, a, total);
+        return;
+    }
+    const int slices = (int)cdiv(d.G, gs);
+    const long total = d.NB * slices;
+    const long wv = gs * a.cg / V;
+    const dim3 grid((unsigned)(total < 65536 ? total : 65536));
+    if (wv <= 256 && d.S <= 256 / wv * 4) hipLaunchKernelGGL((norm_block_groups_kernel<V, 256, 4>), grid, dim3(256), 0, s, a, gs, slices, total);
+    else if (d.S <= 1024 / wv * 4) hipLaunchKernelGGL((norm_block_groups_kernel<V, 1024, 4>), grid, dim3(1024), 0, s, a, gs, slices, total);
+    else hipLaunchKernelGGL((norm_block_groups_kernel<V, 1024, 8>), grid, dim3(1024), 0, s, a, gs, slices, total);
+}
+template <int V> static void launch_split(const NormArgs& a, const SplitShape& h, void* ws, hipStream_t s)
+{
+    const NormDesc& d = a.d;
+    double2* part = (double2*)ws;
+    if (d.first) {
+        const dim3 grid((unsigned)(d.NB * d.G * h.chunks));
+        hipLaunchKernelGGL((norm_sums_first_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, part);
+        hipLaunchKernelGGL((norm_apply_first_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+        return;
+    }
+    const dim3 grid((unsigned)(d.NB * h.slices * h.blocks * h.chunks));
+    hipLaunchKernelGGL((norm_sums_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, part);
+    hipLaunchKernelGGL((norm_apply_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+}
+
+void fortis_launch_group_norm(const NormDesc& in, const float* x, float* y, void* ws, hipStream_t s)
+{
+    NormArgs a = { norm_normal(in), x, y, in.C / in.G, in.S * (in.C / in.G), {} };
+    const NormDesc& d = a.d;
+    if (a.count > GN_BLOCK_MAX) {
+        const SplitShape h = split_shape(d);
+        if (d.first && d.S / h.V < (1L << 31)) a.row = fortis_fast_div((unsigned)(d.S / h.V));
+        if (h.V == 4) launch_split<4>(a, h, ws, s);
+        else if (h.V == 2) launch_split<2>(a, h, ws, s);
+        else launch_split<1>(a, h, ws, s);
+        HIP_OK(hipGetLastError());
+        return;
+    }
+    // a vector stays inside a group and a position (channels last) or inside a channel (channels first)
+    const long along = d.first ? d.S : a.cg;
+    const int V = along % 4 == 0 ? 4 : along % 2 == 0 ? 2 : 1;
+    a.row = fortis_fast_div((unsigned)(along / V));
+    // channels last and narrow groups over several positions: the groups whose channels share lines go to one workgroup
+    int gs = 1;
+    if (!d.first && d.S > 1 && a.cg < GN_BLOCK_EDGE && a.count > GN_LANES_MAX / 8) {
+        gs = (int)((GN_BLOCK_EDGE + a.cg - 1) / a.cg);
+        if (gs > d.G) gs = (int)d.G;
+        while (gs > 1 && d.S > 1024 / (gs * a.cg / V) * 8) gs--;       // what a workgroup's registers hold
+    }
+    if (gs == 1 && a.count <= (V == 4 ? GN_LANES_MAX : GN_LANES_MAX / 4 * V)) {
+        if (V == 4) launch_lanes<4>(a, d.NB * d.G, s);
+        else if (V == 2) launch_lanes<2>(a, d.NB * d.G, s);
+        else launch_lanes<1>(a, d.NB * d.G, s);
+    } else if (V == 4) launch_block<4>(a, gs, s);
+    else if (V == 2) launch_block<2>(a, gs, s);
+    else launch_block<1>(a, gs, s);
     HIP_OK(hipGetLastError());
 }

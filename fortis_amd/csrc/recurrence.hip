@@ -8,7 +8,8 @@
 // (f, (1 - f) x) of one step; 1 - f as sigmoid(-g), which keeps its digits where f is close to 1.
 __device__ __forceinline__ void rc_step(float g, float x, float& f, float& b)
 {
-    const float e = expf(-fabsf(g)), q = 1.f / (1.f + e), hi = q, lo = e * q;
+    float hi, lo;
+    fortis_sigmoids(g, hi, lo);
     f = g >= 0.f ? hi : lo;
     b = (g >= 0.f ? lo : hi) * x;
 }
