@@ -1,43 +1,184 @@
 // Gated linear recurrence (include/fortis_step.h, fortis_plan_recurrence):
 //     f = 1 / (1 + exp(-g_t)),  h_t = f h_(t-1) + (1 - f) x_t
 // per sequence and channel, rows of 2 * ch features (g first, x behind).
+//
+// Memory-bound: 12 bytes and about 25 instructions a value.  A lane owns V neighbouring channels of a sequence and walks
+// steps with the next loads in flight.  Where sequences and channels alone do not fill the chip, every sequence is cut into
+// K chunks: a step is the map h -> f h + b, maps compose to (F, B), so one launch composes every chunk's steps, one wave per
+// sequence and channel scans the K compositions and leaves the state in front of every chunk, and a third launch walks the
+// chunks from there.  All compositions happen in a fixed order: results repeat bit for bit.
 #include "common.h"
 
 #define RC_THREADS 256
+#define RC_AHEAD 8              // steps whose loads are in flight together
 
-// (f, (1 - f) x) of one step; 1 - f as sigmoid(-g), which keeps its digits where f is close to 1.
-__device__ __forceinline__ void rc_step(float g, float x, float& f, float& b)
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+template <int V> struct VecOf { typedef float T; };
+template <> struct VecOf<2> { typedef v2f T; };
+template <> struct VecOf<4> { typedef v4f T; };
+
+struct RecurArgs {
+    RecurDesc d;
+    const float* src;
+    float* dst;
+    const float* h_in;
+    float* h_out;
+    const int* lengths;
+    float2* maps;               // [nseq * ch][chunks]: (F, B) of a chunk, then (h in front of it, unused)
+    long chunks, per;           // chunks of a sequence, steps a chunk
+};
+
+template <int V> __device__ __forceinline__ void load(float (&o)[V], const float* p)
 {
-    float hi, lo;
-    fortis_sigmoids(g, hi, lo);
-    f = g >= 0.f ? hi : lo;
-    b = (g >= 0.f ? lo : hi) * x;
+    const typename VecOf<V>::T t = *(const typename VecOf<V>::T*)p;
+    __builtin_memcpy(o, &t, sizeof t);
+}
+template <int V> __device__ __forceinline__ void store(float* p, const float (&o)[V])
+{
+    typename VecOf<V>::T t;
+    __builtin_memcpy(&t, o, sizeof t);
+    *(typename VecOf<V>::T*)p = t;
+}
+__device__ __forceinline__ long steps_of(const RecurArgs& a, long s)
+{
+    if (!a.lengths) return a.d.len;
+    const long l = a.lengths[s];
+    return l < 0 ? 0 : l < a.d.len ? l : a.d.len;
 }
 
-// One lane per (sequence, channel) walks its steps.
-__global__ __launch_bounds__(RC_THREADS) void recurrence_simple_kernel(RecurDesc d, const float* __restrict__ src, float* __restrict__ dst,
-                                                                       const float* h_in, float* h_out, const int* __restrict__ lengths)
+// One lane, V channels, the steps of one chunk.  APPLY: from the state in front, writing every step; otherwise the map of the
+// chunk's steps.
+template <int V, bool APPLY>
+__global__ __launch_bounds__(RC_THREADS) void recurrence_walk_kernel(RecurArgs a)
 {
-    const long e = (long)blockIdx.x * RC_THREADS + threadIdx.x;
-    if (e >= d.nseq * d.ch) return;
-    const long s = e / d.ch, c = e % d.ch;
-    long len = d.len;
-    if (lengths) { const long l = lengths[s]; len = l < 0 ? 0 : l < len ? l : len; }
-    float h = h_in ? h_in[e] : 0.f;
-    for (long i = 0; i < len; i++) {
-        const long t = d.reverse ? len - 1 - i : i, row = d.time_major ? t * d.nseq + s : s * d.len + t;
-        float f, b;
-        rc_step(src[row * 2 * d.ch + c], src[row * 2 * d.ch + d.ch + c], f, b);
-        h = fmaf(f, h, b);
-        dst[row * d.ch + c] = h;
+    const RecurDesc& d = a.d;
+    const long lanes = d.nseq * d.ch / V;
+    const long id = (long)blockIdx.x * RC_THREADS + threadIdx.x;
+    if (id >= lanes * a.chunks) return;
+    const long k = id / lanes, e = (id - k * lanes) * V;      // chunk, first of the lane's values in [nseq][ch]
+    const long s = e / d.ch, c = e - s * d.ch;
+    const long len = steps_of(a, s);
+    const long i0 = k * a.per, i1 = i0 + a.per < len ? i0 + a.per : len;
+    float h[V], F[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) { h[v] = -0.f; F[v] = 1.f; }     // the identity to the bit: 1 h + -0 is h, also for h = -0
+    if (APPLY) {
+        if (a.chunks > 1) {
+#pragma unroll
+            for (int v = 0; v < V; v++) h[v] = a.maps[(e + v) * a.chunks + k].x;
+        } else if (a.h_in) load<V>(h, a.h_in + e);
+        else {
+#pragma unroll
+            for (int v = 0; v < V; v++) h[v] = 0.f;
+        }
     }
-    if (h_out) h_out[e] = h;
+    if (i0 < i1) {
+        const long row0 = d.time_major ? s : s * d.len, rstep = d.time_major ? d.nseq : 1;
+        const long t0 = d.reverse ? len - 1 - i0 : i0, dir = d.reverse ? -rstep : rstep;
+        const float* p = a.src + (row0 + t0 * rstep) * 2 * d.ch + c;
+        float* q = a.dst + (row0 + t0 * rstep) * d.ch + c;
+        const long ps = dir * 2 * d.ch, qs = dir * d.ch, n = i1 - i0;
+        float g[RC_AHEAD][V], x[RC_AHEAD][V];
+        for (long i = 0; i < n; i += RC_AHEAD, p += RC_AHEAD * ps, q += RC_AHEAD * qs) {
+            if (i + RC_AHEAD <= n) {
+#pragma unroll
+                for (int u = 0; u < RC_AHEAD; u++) { load<V>(g[u], p + u * ps); load<V>(x[u], p + u * ps + d.ch); }
+            } else {
+                const long last = (n - 1 - i) * ps;              // places behind the last step read it again
+#pragma unroll
+                for (int u = 0; u < RC_AHEAD; u++) {
+                    const long o = i + u < n ? u * ps : last;
+                    load<V>(g[u], p + o);
+                    load<V>(x[u], p + o + d.ch);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < RC_AHEAD; u++) {
+                if (i + u >= n) break;
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    float hi, lo;
+                    fortis_sigmoids(g[u][v], hi, lo);
+                    const float f = g[u][v] >= 0.f ? hi : lo, b = (g[u][v] >= 0.f ? lo : hi) * x[u][v];
+                    h[v] = fmaf(f, h[v], b);
+                    if (!APPLY) F[v] *= f;
+                }
+                if (APPLY) store<V>(q + u * qs, h);
+            }
+        }
+    }
+    if (APPLY) {
+        if (a.chunks == 1 && a.h_out) store<V>(a.h_out + e, h);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; v++) a.maps[(e + v) * a.chunks + k] = make_float2(F[v], h[v]);
+    }
 }
 
-long fortis_recurrence_workspace(const RecurDesc&) { return 0; }
-
-void fortis_launch_recurrence(const RecurDesc& d, const float* src, float* dst, const float* h_in, float* h_out, const int* lengths, void*, hipStream_t s)
+// One wave per (sequence, channel): the maps of its chunks become the states in front of them.
+__global__ __launch_bounds__(RC_THREADS) void recurrence_scan_kernel(RecurArgs a)
 {
-    hipLaunchKernelGGL(recurrence_simple_kernel, dim3((unsigned)cdiv(d.nseq * d.ch, RC_THREADS)), dim3(RC_THREADS), 0, s, d, src, dst, h_in, h_out, lengths);
+    const long e = (long)blockIdx.x * (RC_THREADS / 64) + (threadIdx.x >> 6);
+    if (e >= a.d.nseq * a.d.ch) return;
+    const int lane = threadIdx.x & 63;
+    const long q = (a.chunks + 63) / 64, k0 = lane * q, k1 = k0 + q < a.chunks ? k0 + q : a.chunks;
+    float2* m = a.maps + e * a.chunks;
+    float F = 1.f, B = -0.f;
+    for (long k = k0; k < k1; k++) { const float2 w = m[k]; B = fmaf(w.x, B, w.y); F *= w.x; }
+    // inclusive scan over the lanes: (F, B) after (Fp, Bp) is (F Fp, F Bp + B)
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const float Fp = __shfl_up(F, o, 64), Bp = __shfl_up(B, o, 64);
+        if (lane >= o) { B = fmaf(F, Bp, B); F *= Fp; }
+    }
+    const float h0 = a.h_in ? a.h_in[e] : 0.f;
+    if (a.h_out && lane == 63) a.h_out[e] = fmaf(F, h0, B);
+    float Fx = __shfl_up(F, 1, 64), Bx = __shfl_up(B, 1, 64);
+    if (lane == 0) { Fx = 1.f; Bx = -0.f; }
+    float h = fmaf(Fx, h0, Bx);
+    for (long k = k0; k < k1; k++) {
+        const float2 w = m[k];
+        m[k] = make_float2(h, 0.f);
+        h = fmaf(w.x, h, w.y);
+    }
+}
+
+struct RecurShape { int V; long chunks, per; };
+static RecurShape recur_shape(const RecurDesc& d)
+{
+    RecurShape r;
+    const long values = d.nseq * d.ch, full = 256 * 8 * 64;      // lanes that fill the chip: eight waves a compute unit
+    r.V = d.ch % 4 == 0 && values / 4 >= full / 2 ? 4 : d.ch % 2 == 0 && values / 2 >= full / 2 ? 2 : 1;
+    r.chunks = 1;
+    if (values / r.V < full / 2) r.chunks = cdiv(full, values / r.V);
+    if (r.chunks > cdiv(d.len, 32)) r.chunks = cdiv(d.len, 32);
+    r.per = cdiv(d.len, r.chunks);
+    r.chunks = cdiv(d.len, r.per);
+    return r;
+}
+
+long fortis_recurrence_workspace(const RecurDesc& d)
+{
+    const RecurShape r = recur_shape(d);
+    return r.chunks > 1 ? d.nseq * d.ch * r.chunks * (long)sizeof(float2) : 0;
+}
+
+template <int V> static void launch_walks(const RecurArgs& a, hipStream_t s)
+{
+    const dim3 grid((unsigned)cdiv(a.d.nseq * a.d.ch / V * a.chunks, RC_THREADS)), block(RC_THREADS);
+    if (a.chunks > 1) {
+        hipLaunchKernelGGL((recurrence_walk_kernel<V, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL(recurrence_scan_kernel, dim3((unsigned)cdiv(a.d.nseq * a.d.ch, RC_THREADS / 64)), block, 0, s, a);
+    }
+    hipLaunchKernelGGL((recurrence_walk_kernel<V, true>), grid, block, 0, s, a);
+}
+void fortis_launch_recurrence(const RecurDesc& d, const float* src, float* dst, const float* h_in, float* h_out, const int* lengths, void* ws, hipStream_t s)
+{
+    const RecurShape r = recur_shape(d);
+    const RecurArgs a = { d, src, dst, h_in, h_out, lengths, (float2*)ws, r.chunks, r.per };
+    if (r.V == 4) launch_walks<4>(a, s);
+    else if (r.V == 2) launch_walks<2>(a, s);
+    else launch_walks<1>(a, s);
     HIP_OK(hipGetLastError());
 }
