@@ -1,46 +1,406 @@
 // A projection with a low-rank adapter chosen per row (include/fortis_step.h, fortis_plan_linear_adapters):
 //     Y[r] = act(X[r] W^T + b + s_i (X[r] A_i^T) U_i^T),  i = index[r], no adapter where i is outside [0, nadapt)
-#include "common.h"
+// fp32 throughout, sums on the fp32 matrix instructions.
+//
+// Few rows (up to AD_FEW_ROWS): bound by latency and by reading W and the named adapters once.  One launch forms the
+// low-rank rows H[r] = s_i X[r] A_i^T with a wave per row and four ranks, a second the outputs: a workgroup owns 16 rows
+// by 16 columns and its eight waves divide K, so that all of a wave's loads are in flight at once.
+//
+// Many rows: bound by the matrix pipes.  Rows are sorted by adapter inside windows of AD_WINDOW rows (one launch), H is
+// formed for 32 sorted rows at a time, and the GEMM tile of gemm.hip runs over the sorted rows: a row of A is found through
+// the permutation, and behind the k loop each wave adds, per 32 rows and adapter among them, H U_i^T to the sums
+// of that adapter's rows.  Sorted rows leave one or two adapters to a block of 32; rows that were not sorted would leave up to
+// 32.  A window keeps a tile's rows and the rows it writes within a few megabytes of each other.  Sorting places equal
+// adapters in any order: a row's sums do not depend on its place.
+#include "gemm_dev.h"
 
 #define AD_THREADS 256
+#define AD_WINDOW 2048          // rows sorted together; a multiple of the tile's 128
+#define AD_FEW_ROWS 512
 
-// H[r][j] = s_i X[r] . A_i[j]; rows without an adapter are not written.
-__global__ __launch_bounds__(AD_THREADS) void adapt_low_simple_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
-                                                                      float* __restrict__ H, long B)
+static inline long up(long n, long m) { return (n + m - 1) / m * m; }
+
+// ---- weights, laid out once --------------------------------------------------------------------------------------
+// W [N][ldw], A [nadapt][R16][Ka], U [nadapt][N][Rp], padded with zeros.
+AdaptPitch fortis_adapters_pitch(long K, long rank) { return { up(K, 4), up(K, 16), up(rank, 16), up(rank, 8) }; }
+
+// Element k .. k + 3 of a row of K floats at p; what lies at or beyond K is 0.  SC: K is no multiple of 4.
+template <bool SC> __device__ __forceinline__ v4f load_row4(const float* p, long k, long K)
 {
-    const long e = (long)blockIdx.x * AD_THREADS + threadIdx.x;
-    if (e >= B * d.rank) return;
-    const long r = e / d.rank, j = e % d.rank;
+    v4f v;
+    if constexpr (SC) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) { const float t = p[k + c < K ? k + c : K - 1]; v[c] = k + c < K ? t : 0.f; }
+    } else {
+        v = *(const v4f*)(p + (k < K ? k : 0));
+        if (k >= K) v = (v4f)(0.f);
+    }
+    return v;
+}
+
+// ---- few rows ----------------------------------------------------------------------------------------------------
+// H[r][4 q .. 4 q + 3], one wave each: lanes stride over k.
+template <bool SC>
+__global__ __launch_bounds__(AD_THREADS) void adapt_low_rows_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
+                                                                    float* __restrict__ H, long B)
+{
+    const int lane = threadIdx.x & 63;
+    const long quads = d.p.Rp / 4, id = (long)blockIdx.x * (AD_THREADS / 64) + (threadIdx.x >> 6);
+    if (id >= B * quads) return;
+    const long r = id / quads, q = id - r * quads;
     const int i = index[r];
     if (i < 0 || i >= d.nadapt) return;
-    const float *x = X + r * d.K, *a = d.A + ((long)i * d.rank + j) * d.K;
-    float acc = 0.f;
-    for (long k = 0; k < d.K; k++) acc = fmaf(x[k], a[k], acc);
-    H[e] = acc * d.scale[i];
-}
-__global__ __launch_bounds__(AD_THREADS) void adapt_simple_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
-                                                                  const float* __restrict__ H, float* __restrict__ Y, long B)
-{
-    const long e = (long)blockIdx.x * AD_THREADS + threadIdx.x;
-    if (e >= B * d.N) return;
-    const long r = e / d.N, n = e % d.N;
-    const float *x = X + r * d.K, *w = d.W + n * d.K;
-    float acc = 0.f;
-    for (long k = 0; k < d.K; k++) acc = fmaf(x[k], w[k], acc);
-    const int i = index[r];
-    if (i >= 0 && i < d.nadapt) {
-        const float *h = H + r * d.rank, *u = d.U + ((long)i * d.N + n) * d.rank;
-        for (long j = 0; j < d.rank; j++) acc = fmaf(h[j], u[j], acc);
+    const float* x = X + r * d.K;
+    const float* a = d.A + ((long)i * d.p.R16 + 4 * q) * d.p.Ka;
+    float s[4] = { 0.f, 0.f, 0.f, 0.f };
+    for (long k = lane * 4; k < d.p.Ka; k += 256) {
+        const v4f xv = load_row4<SC>(x, k, d.K);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const v4f av = *(const v4f*)(a + j * d.p.Ka + k);
+            s[j] = fmaf(xv[3], av[3], fmaf(xv[2], av[2], fmaf(xv[1], av[1], fmaf(xv[0], av[0], s[j]))));
+        }
     }
-    Y[e] = fortis_act_any(acc + (d.bias ? d.bias[n] : 0.f), d.act, d.alpha);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) s[j] += __shfl_xor(s[j], o, 64);
+    if (lane < 4) {
+        const float v = lane == 0 ? s[0] : lane == 1 ? s[1] : lane == 2 ? s[2] : s[3];
+        H[r * d.p.Rp + 4 * q + lane] = 4 * q + lane < d.rank ? v * d.scale[i] : 0.f;
+    }
 }
 
-long fortis_adapters_workspace(const AdaptDesc& d, long B) { return B * d.rank * 4; }
+// 16 rows x 16 columns of Y; wave w takes the 16-wide k groups w, w + 8, ...  A lane reads four consecutive k of a row of X
+// and of W as one 16-byte load each and feeds four matrix instructions: instruction c multiplies k = 16 g + 4 q + c for lane
+// quarter q on both sides.
+#define FEW_WAVES 8
+template <bool SC>
+__global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
+                                                                   const float* __restrict__ H, float* __restrict__ Y, long B)
+{
+    __shared__ float part[FEW_WAVES][16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+    const long tn = (d.N + 15) / 16, m0 = blockIdx.x / tn * 16, n0 = blockIdx.x % tn * 16;
+    const float* x = X + (m0 + lr < B ? m0 + lr : B - 1) * d.K;
+    const float* w = d.W + (n0 + lr < d.N ? n0 + lr : d.N - 1) * d.p.ldw;
+    v4f acc = (v4f)(0.f);
+    const long groups = d.p.Ka / 16;
+    constexpr int AHEAD = 6;
+    for (long g = wave; g < groups; g += FEW_WAVES * AHEAD) {
+        v4f xv[AHEAD], wv[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const long k = (g + u * FEW_WAVES) * 16 + 4 * lq;
+            xv[u] = load_row4<SC>(x, k, d.K);
+            wv[u] = load_row4<false>(w, k, d.p.ldw);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[u][c], wv[u][c], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) part[wave][4 * lq + r][lr] = acc[r];
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (t >= 256) return;
+    const long m = m0 + t / 16, n = n0 + t % 16;
+    if (m >= B || n >= d.N) return;
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < FEW_WAVES; k++) v += part[k][t / 16][t % 16];
+    const int i = index[m];
+    if (i >= 0 && i < d.nadapt) {
+        const float *h = H + m * d.p.Rp, *u = d.U + ((long)i * d.N + n) * d.p.Rp;
+        for (long j = 0; j < d.p.Rp; j += 4) {
+            const v4f hv = *(const v4f*)(h + j), uv = *(const v4f*)(u + j);
+            v = fmaf(hv[3], uv[3], fmaf(hv[2], uv[2], fmaf(hv[1], uv[1], fmaf(hv[0], uv[0], v))));
+        }
+    }
+    Y[m * d.N + n] = fortis_act_any(v + (d.bias ? d.bias[n] : 0.f), d.act, d.alpha);
+}
 
+// ---- many rows ---------------------------------------------------------------------------------------------------
+// Rows of a window in order of their adapter, those without one behind: perm[p] = row inside the window, key[p] = its
+// adapter or -1.
+__global__ __launch_bounds__(1024) void adapt_sort_kernel(const int* __restrict__ index, int* __restrict__ perm, int* __restrict__ key, long B, int nadapt)
+{
+    extern __shared__ int bin[];        // [nadapt + 1], then 16 wave sums
+    const int tid = threadIdx.x, bins = nadapt + 1;
+    int* wsum = bin + bins;
+    const long r0 = (long)blockIdx.x * AD_WINDOW;
+    for (int b = tid; b < bins; b += 1024) bin[b] = 0;
+    __syncthreads();
+    int mine[AD_WINDOW / 1024];
+#pragma unroll
+    for (int k = 0; k < AD_WINDOW / 1024; k++) {
+        const long r = r0 + tid + k * 1024;
+        mine[k] = -1;
+        if (r < B) {
+            const int i = index[r];
+            mine[k] = i >= 0 && i < nadapt ? i : nadapt;
+            atomicAdd(&bin[mine[k]], 1);
+        }
+    }
+    __syncthreads();
+    // exclusive sums of the bins: `per` neighbouring bins a thread
+    const int per = (bins + 1023) / 1024, b0 = tid * per;
+    int sum = 0;
+    for (int b = b0; b < b0 + per && b < bins; b++) sum += bin[b];
+    int run = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(run, o, 64); if ((tid & 63) >= o) run += t; }
+    if ((tid & 63) == 63) wsum[tid >> 6] = run;
+    __syncthreads();
+    int before = run - sum;
+    for (int w = 0; w < (tid >> 6); w++) before += wsum[w];
+    for (int b = b0; b < b0 + per && b < bins; b++) { const int t = bin[b]; bin[b] = before; before += t; }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < AD_WINDOW / 1024; k++) {
+        if (mine[k] < 0) continue;
+        const int p = atomicAdd(&bin[mine[k]], 1);
+        perm[r0 + p] = tid + k * 1024;
+        key[r0 + p] = mine[k] < nadapt ? mine[k] : -1;
+    }
+}
+
+// H of 32 sorted rows: the four waves divide the 16-wide k groups, 16 ranks at a time; per adapter among the rows all 32 are
+// multiplied with its A and its own rows kept.
+template <bool SC>
+__global__ __launch_bounds__(AD_THREADS) void adapt_low_sorted_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ perm,
+                                                                      const int* __restrict__ key, float* __restrict__ H, long B)
+{
+    __shared__ float part[4][32][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
+    const long p0 = (long)blockIdx.x * 32, base = p0 / AD_WINDOW * AD_WINDOW;
+    const int kk = p0 + (lane & 31) < B ? key[p0 + (lane & 31)] : -1;
+    const float* x[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const long p = p0 + 16 * h + lr < B ? p0 + 16 * h + lr : B - 1;
+        x[h] = X + (base + perm[p]) * d.K;
+    }
+    const long groups = d.p.Ka / 16;
+    constexpr int AHEAD = 4;
+    unsigned live = (unsigned)__ballot(kk >= 0);
+    while (live) {
+        const int a = __builtin_amdgcn_readlane(kk, __builtin_ctz(live));
+        const unsigned rows = (unsigned)__ballot(kk == a);
+        live &= ~rows;
+        const float sc = d.scale[a];
+        for (long j0 = 0; j0 < d.rank; j0 += 16) {
+            const float* w = d.A + ((long)a * d.p.R16 + j0 + lr) * d.p.Ka;
+            v4f acc[2] = { (v4f)(0.f), (v4f)(0.f) };
+            for (long g = wave; g < groups; g += 4 * AHEAD) {
+                v4f xv[2][AHEAD], wv[AHEAD];
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++) {
+                    const long k = (g + u * 4) * 16 + 4 * lq;
+                    xv[0][u] = load_row4<SC>(x[0], k, d.K);
+                    xv[1][u] = load_row4<SC>(x[1], k, d.K);
+                    wv[u] = load_row4<false>(w, k, d.p.Ka);
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[0][u][c], wv[u][c], acc[0], 0, 0, 0);
+                        acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[1][u][c], wv[u][c], acc[1], 0, 0, 0);
+                    }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) part[wave][16 * h + 4 * lq + r][lr] = acc[h][r];
+            __syncthreads();
+#pragma unroll
+            for (int e = threadIdx.x; e < 512; e += AD_THREADS) {
+                const int m = e >> 4, j = e & 15;
+                if (!((rows >> m) & 1) || j0 + j >= d.p.Rp) continue;
+                const float v = ((part[0][m][j] + part[1][m][j]) + part[2][m][j]) + part[3][m][j];
+                H[(p0 + m) * d.p.Rp + j0 + j] = j0 + j < d.rank ? v * sc : 0.f;
+            }
+        }
+    }
+}
+
+// The GEMM tile over sorted rows.
+template <bool SC> struct AdaptRows {
+    static constexpr bool kPlain = false, kScalar = SC;
+    const int *perm, *key;
+    const float *H, *U;
+    long ldw, B, N, Rp;
+    __device__ __forceinline__ long base(long m0) const { return m0 / AD_WINDOW * AD_WINDOW; }
+    __device__ __forceinline__ unsigned rel(long m) const { return (unsigned)perm[m]; }
+    template <int TM, int TN> __device__ __forceinline__ void add(v16f (&acc)[TM][TN], long m, long n, int lr, int lh) const
+    {
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const long pb = m + i * 32;
+            if (pb >= B) continue;
+            const long p = pb + lr < B ? pb + lr : B - 1;
+            const int kk = pb + lr < B ? key[p] : -1;
+            const float* h = H + p * Rp + 4 * lh;
+            unsigned live = (unsigned)__ballot(kk >= 0);
+            while (live) {
+                const int a = __builtin_amdgcn_readlane(kk, __builtin_ctz(live));
+                const unsigned rows = (unsigned)__ballot(kk == a);
+                live &= ~rows;
+                v16f sum[TN];
+                const float* u[TN];
+#pragma unroll
+                for (int j = 0; j < TN; j++) {
+                    sum[j] = (v16f)(0.f);
+                    u[j] = U + ((long)a * N + (n + j * 32 + lr < N ? n + j * 32 + lr : N - 1)) * Rp + 4 * lh;
+                }
+                for (long k = 0; k < Rp; k += 8) {
+                    const v4f hv = *(const v4f*)(h + k);
+                    v4f uv[TN];
+#pragma unroll
+                    for (int j = 0; j < TN; j++) uv[j] = *(const v4f*)(u[j] + k);
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int j = 0; j < TN; j++) sum[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(hv[c], uv[j][c], sum[j], 0, 0, 0);
+                }
+                const unsigned sel = rows >> (4 * lh);
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        acc[i][j][r] += (sel >> (8 * (r >> 2) + (r & 3))) & 1 ? sum[j][r] : 0.f;
+            }
+        }
+    }
+    template <int ACT, int TM, int TN>
+    __device__ __forceinline__ void store_act(const v16f (&acc)[TM][TN], float* C, long m, long n, int lr, int lh, const GemmEpi& epi) const
+    {
+        float bv[TN];
+#pragma unroll
+        for (int j = 0; j < TN; j++) bv[j] = epi.bias && n + j * 32 + lr < N ? epi.bias[n + j * 32 + lr] : 0.f;
+        const long b = base(m);
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const long p = m + i * 32 + 8 * q + 4 * lh;
+                const int4 to = *(const int4*)(perm + p);             // the list is a whole number of windows long
+                const int row[4] = { to.x, to.y, to.z, to.w };
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (p + c >= B) continue;
+                    float* y = C + (b + row[c]) * N + n + lr;
+#pragma unroll
+                    for (int j = 0; j < TN; j++)
+                        if (n + j * 32 + lr < N) y[j * 32] = fortis_act_any(acc[i][j][4 * q + c] + bv[j], ACT, epi.alpha);
+                }
+            }
+    }
+    template <int TM, int TN>
+    __device__ __forceinline__ void store(const v16f (&acc)[TM][TN], float* C, long, long, long m, long n, int lr, int lh, const GemmEpi& epi) const
+    {
+        if (epi.act == FORTIS_ACT_RELU) store_act<FORTIS_ACT_RELU>(acc, C, m, n, lr, lh, epi);
+        else if (epi.act == FORTIS_ACT_LEAKY) store_act<FORTIS_ACT_LEAKY>(acc, C, m, n, lr, lh, epi);
+        else if (epi.act == FORTIS_ACT_SILU) store_act<FORTIS_ACT_SILU>(acc, C, m, n, lr, lh, epi);
+        else store_act<FORTIS_ACT_NONE>(acc, C, m, n, lr, lh, epi);
+    }
+};
+
+#define AD_BK 32
+// The phases of gemm.hip's persistent kernel.
+template <bool SC>
+__global__ __launch_bounds__(GM_THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) void adapt_gemm_kernel(const float* __restrict__ A, const float* __restrict__ W,
+                                                          float* __restrict__ C, long B, long N, long K, GemmSched sc, GemmEpi epi, AdaptRows<SC> ext)
+{
+    extern __shared__ float4 smem4[];
+    float* smem = (float*)smem4;
+    const long w = blockIdx.x;
+    for (int p = 0; p < sc.nphase; p++) {
+        const int level = sc.ph[p].level;
+        const long base = sc.ph[p].base, count = sc.ph[p].count;
+        if (level == 0) {
+            const long place = (w & 7) * (sc.slots / 8) + (w >> 3);
+            const long rounds = count / sc.slots;
+            v4f ra[2 * AD_BK / 16], rw[2 * AD_BK / 16];
+            for (long r = 0; r < rounds; r++) {
+                const long tile = base + r * sc.slots + place, next = tile + sc.slots;
+                const long tm = tile / sc.tiles_n, tn = tile - tm * sc.tiles_n;
+                const long tmn = next / sc.tiles_n, tnn = next - tmn * sc.tiles_n;
+                gemm_tile<2, 2, AD_BK>(A, W, C, B, N, K, tm * 128, tn * 128, epi, smem, ra, rw, r > 0, r + 1 < rounds, tmn * 128, tnn * 128, ext);
+            }
+            continue;
+        }
+        const long per_xcd = (count + 7) / 8;
+        if ((w >> 3) >= per_xcd) continue;
+        const long item = (w & 7) * per_xcd + (w >> 3);
+        if (item >= count) continue;
+        const long tile = base + (level == 1 ? (item >> 1) : (item >> 2));
+        const long tm = tile / sc.tiles_n, tn = tile - tm * sc.tiles_n;
+        if (level == 1) {
+            const long m0 = tm * 128, n0 = tn * 128 + (item & 1) * 64;
+            if (m0 >= B || n0 >= N) continue;
+            v4f ra[2 * AD_BK / 16], rw[AD_BK / 16];
+            gemm_tile<2, 1, AD_BK>(A, W, C, B, N, K, m0, n0, epi, smem, ra, rw, false, false, 0, 0, ext);
+        } else {
+            const long m0 = tm * 128 + ((item >> 1) & 1) * 64, n0 = tn * 128 + (item & 1) * 64;
+            if (m0 >= B || n0 >= N) continue;
+            v4f ra[AD_BK / 16], rw[AD_BK / 16];
+            gemm_tile<1, 1, AD_BK>(A, W, C, B, N, K, m0, n0, epi, smem, ra, rw, false, false, 0, 0, ext);
+        }
+    }
+}
+template <bool SC>
+static void launch_adapt_gemm(const AdaptDesc& d, const float* X, float* Y, long B, const AdaptRows<SC>& ext, hipStream_t s)
+{
+    const size_t shmem = (size_t)2 * (128 + 128) * (AD_BK + 4) * sizeof(float);
+    static long slots = 0;
+    if (!slots) {
+        HIP_OK(hipFuncSetAttribute((const void*)adapt_gemm_kernel<SC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem));
+        int occ = 0, dev = 0;
+        hipDeviceProp_t prop;
+        HIP_OK(hipGetDevice(&dev));
+        HIP_OK(hipGetDeviceProperties(&prop, dev));
+        HIP_OK(hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, (const void*)adapt_gemm_kernel<SC>, GM_THREADS, shmem));
+        if (occ < 1) occ = 1;
+        slots = (long)occ * prop.multiProcessorCount / 8 * 8;
+        if (slots < 8) slots = 8;
+    }
+    GemmSched sc;
+    gemm_make_sched(B, d.N, slots, &sc);
+    long items = 0;
+    for (int p = 0; p < sc.nphase; p++) items = sc.ph[p].count > items ? sc.ph[p].count : items;
+    const long grid = items < slots ? cdiv(items, 8) * 8 : slots;
+    const GemmEpi epi = { d.bias, nullptr, d.act, d.alpha, d.N };
+    hipLaunchKernelGGL((adapt_gemm_kernel<SC>), dim3((unsigned)grid), dim3(GM_THREADS), shmem, s, X, d.W, Y, B, d.N, d.K, sc, epi, ext);
+}
+
+// Both forms' scratch: a step that has been re-sized to fewer rows may take the other one.
+long fortis_adapters_workspace(const AdaptDesc& d, long B)
+{
+    return up(B, AD_WINDOW) * 8 + B * d.p.Rp * 4;
+}
+template <bool SC>
+static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
+{
+    if (B <= AD_FEW_ROWS) {
+        float* H = (float*)ws;
+        hipLaunchKernelGGL((adapt_low_rows_kernel<SC>), dim3((unsigned)cdiv(B * (d.p.Rp / 4), AD_THREADS / 64)), dim3(AD_THREADS), 0, s, d, X, index, H, B);
+        hipLaunchKernelGGL((adapt_few_kernel<SC>), dim3((unsigned)(cdiv(B, 16) * cdiv(d.N, 16))), dim3(64 * FEW_WAVES), 0, s, d, X, index, (const float*)H, Y, B);
+        return;
+    }
+    const long Bw = up(B, AD_WINDOW);
+    int *perm = (int*)ws, *key = perm + Bw;
+    float* H = (float*)(key + Bw);
+    hipLaunchKernelGGL(adapt_sort_kernel, dim3((unsigned)(Bw / AD_WINDOW)), dim3(1024), (size_t)(d.nadapt + 1 + 16) * 4, s, index, perm, key, B, (int)d.nadapt);
+    hipLaunchKernelGGL((adapt_low_sorted_kernel<SC>), dim3((unsigned)cdiv(B, 32)), dim3(AD_THREADS), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
+    launch_adapt_gemm<SC>(d, X, Y, B, { perm, key, H, d.U, d.p.ldw, B, d.N, d.p.Rp }, s);
+}
 void fortis_launch_linear_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {
-    float* H = (float*)ws;
-    hipLaunchKernelGGL(adapt_low_simple_kernel, dim3((unsigned)cdiv(B * d.rank, AD_THREADS)), dim3(AD_THREADS), 0, s, d, X, index, H, B);
-    hipLaunchKernelGGL(adapt_simple_kernel, dim3((unsigned)cdiv(B * d.N, AD_THREADS)), dim3(AD_THREADS), 0, s, d, X, index, H, Y, B);
+    if (d.K % 4 == 0) launch_adapters<false>(d, X, index, Y, B, ws, s);
+    else launch_adapters<true>(d, X, index, Y, B, ws, s);
     HIP_OK(hipGetLastError());
 }

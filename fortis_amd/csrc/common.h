@@ -122,12 +122,15 @@ long fortis_norm_workspace(const NormDesc& d);          // bytes fortis_launch_g
 void fortis_launch_group_norm(const NormDesc& d, const float* x, float* y, void* ws, hipStream_t s);
 
 // ---- projection with an adapter per row (adapters.hip) -------------------------------------
+struct AdaptPitch { long ldw, Ka, R16, Rp; };   // floats a row of W, of A; rows of A an adapter; floats a row of U and of the low-rank rows
+AdaptPitch fortis_adapters_pitch(long K, long rank);
 struct AdaptDesc {
     long K, N, nadapt, rank;
     int act;
     float alpha;
-    const float *W, *bias;      // device; bias may be null
-    const float *A, *U, *scale; // device: [nadapt][rank][K], [nadapt][N][rank], [nadapt]
+    AdaptPitch p;
+    const float *W, *bias;      // device, padded with zeros: W [N][ldw]; bias may be null
+    const float *A, *U, *scale; // [nadapt][R16][Ka], [nadapt][N][Rp], [nadapt]
 };
 long fortis_adapters_workspace(const AdaptDesc& d, long B);
 void fortis_launch_linear_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s);

@@ -92,6 +92,17 @@ static void* upload(fortis_plan* p, const void* h, size_t nbytes)
     return d;
 }
 
+// `count` matrices of rows x cols as matrices of prows x pcols with zeros around them.
+static const float* upload_padded(fortis_plan* p, const std::vector<float>& m, long count, long rows, long cols, long prows, long pcols)
+{
+    if (rows == prows && cols == pcols) return (const float*)upload(p, m.data(), m.size() * 4);
+    std::vector<float> out((size_t)(count * prows * pcols), 0.f);
+    for (long c = 0; c < count; c++)
+        for (long r = 0; r < rows; r++)
+            memcpy(&out[(size_t)((c * prows + r) * pcols)], &m[(size_t)((c * rows + r) * cols)], (size_t)cols * 4);
+    return (const float*)upload(p, out.data(), out.size() * 4);
+}
+
 static int bad(const char* what) { fprintf(stderr, "fortis_plan: %s\n", what); return -1; }
 static bool tensor_ok(fortis_plan* p, int t, long need_bytes)
 {
@@ -317,7 +328,7 @@ int fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, con
     if (!p || p->finalized) return bad("plan is null or already finalized");
     const long nx = bytes_of(B, K), ny = bytes_of(B, N), ni = bytes_of(B, 1);
     if (nx < 0 || ny < 0 || bytes_of(N, K) < 0 || bytes_of(nadapt, rank, K) < 0 || bytes_of(nadapt, rank, N) < 0 || B >= (1L << 31) ||
-        K >= (1L << 22) || N >= (1L << 22) || !W || !A || !U)
+        K >= (1L << 19) || N >= (1L << 19) || !W || !A || !U)
         return bad("linear_adapters: bad shape or arguments");
     if (nadapt > FORTIS_MAX_ADAPTERS || rank > FORTIS_MAX_RANK) return bad("linear_adapters: too many adapters or too large a rank");
     if (act < 0 || act > FORTIS_ACT_SILU) return bad("linear_adapters: unknown activation");
@@ -692,11 +703,11 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
                 break;
             case OP_ADAPT:
                 ex.kind = EX_ADAPT; ex.side = o.side; ex.rows = ex.rows_cap = o.B;
-                ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, nullptr, nullptr, nullptr, nullptr, nullptr };
-                ex.adapt.W = (const float*)upload(p, o.w.data(), o.w.size() * 4);
+                ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, fortis_adapters_pitch(o.K, o.D), nullptr, nullptr, nullptr, nullptr, nullptr };
+                ex.adapt.W = upload_padded(p, o.w, 1, o.N, o.K, o.N, ex.adapt.p.ldw);
                 ex.adapt.bias = o.has_bias ? (const float*)upload(p, o.b.data(), o.b.size() * 4) : nullptr;
-                ex.adapt.A = (const float*)upload(p, o.v0.data(), o.v0.size() * 4);
-                ex.adapt.U = (const float*)upload(p, o.v1.data(), o.v1.size() * 4);
+                ex.adapt.A = upload_padded(p, o.v0, o.F, o.D, o.K, ex.adapt.p.R16, ex.adapt.p.Ka);
+                ex.adapt.U = upload_padded(p, o.v1, o.F, o.N, o.D, o.N, ex.adapt.p.Rp);
                 ex.adapt.scale = (const float*)upload(p, o.v2.data(), o.v2.size() * 4);
                 break;
             case OP_RECUR:

@@ -116,7 +116,7 @@ int  fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma
  * A [nadapt][rank][K], U [nadapt][N][rank], scale [nadapt] (NULL: 1), W, bias as in fortis_plan_linear: host pointers,
  * copied.  index: a tensor of B int32, read on the device at every pass, rows in any order; an index outside
  * [0, nadapt) means no adapter for that row, and so all rows start (index is filled with -1 at finalize).  1 <= nadapt
- * <= FORTIS_MAX_ADAPTERS, 1 <= rank <= FORTIS_MAX_RANK, B < 2^31.  A row's result depends on that row alone: not on the
+ * <= FORTIS_MAX_ADAPTERS, 1 <= rank <= FORTIS_MAX_RANK, B < 2^31, K and N < 2^19.  A row's result depends on that row alone: not on the
  * order of rows, nor on the adapters of the others. */
 #define FORTIS_MAX_ADAPTERS 4096
 #define FORTIS_MAX_RANK 256
