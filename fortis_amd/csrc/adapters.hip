@@ -6,6 +6,9 @@
 // low-rank rows H[r] = s_i X[r] A_i^T with a wave per row and four ranks, a second the outputs: a workgroup owns 16 rows
 // by 16 columns and its eight waves divide K, so that all of a wave's loads are in flight at once.
 //
+// Narrow layers (K and N up to 128): bound by reading X and writing Y.  One launch does it all: W lies in LDS, a wave
+// takes 16 rows at a time from X to Y.
+//
 // Many rows: bound by the matrix pipes.  Rows are sorted by adapter inside windows of AD_WINDOW rows (one launch), H is
 // formed for 32 sorted rows at a time, and the GEMM tile of gemm.hip runs over the sorted rows: a row of A is found through
 // the permutation, and behind the k loop each wave adds, per 32 rows and adapter among them, H U_i^T to the sums
@@ -119,6 +122,131 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
         }
     }
     Y[m * d.N + n] = fortis_act_any(v + (d.bias ? d.bias[n] : 0.f), d.act, d.alpha);
+}
+
+// ---- narrow layers -----------------------------------------------------------------------------------------------
+#define NARROW_K 128
+#define NARROW_N 128
+#define NARROW_RANK 64
+// A wave owns 16 rows: their X as KG operands of four k (k = 16 g + 4 q + c, as above), the next rows' X on its way.  Per adapter
+// among the rows: all 16 are multiplied with its A, 16 ranks at a time, the products change places through the wave's own
+// piece of LDS into operands of the second product, and the sums are kept for the adapter's rows only (a NaN in the others'
+// products goes nowhere).
+template <int KG, int NT, bool SC>
+__global__ __launch_bounds__(AD_THREADS) void adapt_narrow_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
+                                                                  float* __restrict__ Y, long B)
+{
+    extern __shared__ float4 smem4[];
+    constexpr int LDW = 16 * KG + 4;
+    float* sW = (float*)smem4;                                              // [16 NT][LDW]
+    float* sH = sW + 16 * NT * LDW + (threadIdx.x >> 6) * 16 * 20;          // [16][20] for this wave
+    const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+    for (int e = threadIdx.x; e < 16 * NT * 4 * KG; e += AD_THREADS) {
+        const int n = e / (4 * KG), k = e % (4 * KG) * 4;
+        *(v4f*)(sW + n * LDW + k) = load_row4<false>(d.W + (n < d.N ? n : d.N - 1) * d.p.ldw, k, d.p.ldw);
+    }
+    __syncthreads();
+    float bv[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) bv[t] = d.bias && 16 * t + lr < d.N ? d.bias[16 * t + lr] : 0.f;
+    const long step = (long)gridDim.x * (AD_THREADS / 64) * 16;
+    long m0 = ((long)blockIdx.x * (AD_THREADS / 64) + (threadIdx.x >> 6)) * 16;
+    if (m0 >= B) return;
+    v4f xn[KG];
+    int in;
+    auto fetch = [&](long m) __attribute__((always_inline)) {
+        const long r = m + lr < B ? m + lr : B - 1;
+#pragma unroll
+        for (int g = 0; g < KG; g++) xn[g] = load_row4<SC>(X + r * d.K, 16 * g + 4 * lq, d.K);
+        in = m + lr < B ? index[r] : -1;
+    };
+    fetch(m0);
+    for (; m0 < B; m0 += step) {
+        v4f xv[KG], acc[NT];
+#pragma unroll
+        for (int g = 0; g < KG; g++) xv[g] = xn[g];
+        const int i = in >= 0 && in < d.nadapt ? in : -1;
+        if (m0 + step < B) fetch(m0 + step);
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[t] = (v4f)(0.f);
+#pragma unroll
+        for (int g = 0; g < KG; g++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const v4f w = *(const v4f*)(sW + (16 * t + lr) * LDW + 16 * g + 4 * lq);
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[g][c], w[c], acc[t], 0, 0, 0);
+            }
+        unsigned live = (unsigned)__ballot(i >= 0) & 0xffff;
+        while (live) {
+            const int a = __builtin_amdgcn_readlane(i, __builtin_ctz(live));
+            const unsigned rows = (unsigned)__ballot(i == a) & 0xffff;
+            live &= ~rows;
+            const float sc = d.scale[a];
+            v4f sum[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) sum[t] = (v4f)(0.f);
+            for (int j0 = 0; j0 < d.rank; j0 += 16) {
+                const float* A = d.A + ((long)a * d.p.R16 + j0 + lr) * d.p.Ka + 4 * lq;
+                v4f h = (v4f)(0.f), av[KG], uv[NT];
+#pragma unroll
+                for (int g = 0; g < KG; g++) av[g] = 16 * g < d.p.Ka ? *(const v4f*)(A + 16 * g) : (v4f)(0.f);
+                const int j = j0 + 4 * lq;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const long n = 16 * t + lr < d.N ? 16 * t + lr : d.N - 1;
+                    uv[t] = *(const v4f*)(d.U + ((long)a * d.N + n) * d.p.Rp + (j < d.p.Rp ? j : 0));
+                }
+#pragma unroll
+                for (int g = 0; g < KG; g++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) h = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[g][c], av[g][c], h, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) sH[(4 * lq + r) * 20 + lr] = h[r] * sc;
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                v4f hv = *(const v4f*)(sH + lr * 20 + 4 * lq);
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int c = 0; c < 4; c++) if (j + c >= d.rank) hv[c] = 0.f;      // what is read of U there belongs to other ranks
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) sum[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[c], j < d.p.Rp ? uv[t][c] : 0.f, sum[t], 0, 0, 0);
+            }
+            const unsigned sel = rows >> (4 * lq);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[t][r] += (sel >> r) & 1 ? sum[t][r] : 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const long m = m0 + 4 * lq + r;
+            if (m >= B) continue;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+                if (16 * t + lr < d.N) Y[m * d.N + 16 * t + lr] = fortis_act_any(acc[t][r] + bv[t], d.act, d.alpha);
+        }
+    }
+}
+template <int KG, int NT, bool SC>
+static void launch_narrow(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, hipStream_t s)
+{
+    const size_t shmem = (size_t)(16 * NT * (16 * KG + 4) + (AD_THREADS / 64) * 16 * 20) * 4;
+    static bool set = false;
+    if (!set) { HIP_OK(hipFuncSetAttribute((const void*)adapt_narrow_kernel<KG, NT, SC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem)); set = true; }
+    const long wgs = cdiv(B, 16 * (AD_THREADS / 64));
+    hipLaunchKernelGGL((adapt_narrow_kernel<KG, NT, SC>), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(AD_THREADS), shmem, s, d, X, index, Y, B);
+}
+template <int KG, bool SC>
+static void narrow_by_columns(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, hipStream_t s)
+{
+    if (d.N <= 16) launch_narrow<KG, 1, SC>(d, X, index, Y, B, s);
+    else if (d.N <= 32) launch_narrow<KG, 2, SC>(d, X, index, Y, B, s);
+    else if (d.N <= 64) launch_narrow<KG, 4, SC>(d, X, index, Y, B, s);
+    else launch_narrow<KG, 8, SC>(d, X, index, Y, B, s);
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------------------
@@ -385,6 +513,13 @@ long fortis_adapters_workspace(const AdaptDesc& d, long B)
 template <bool SC>
 static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {
+    if (d.K <= NARROW_K && d.N <= NARROW_N && d.rank <= NARROW_RANK) {
+        if (d.K <= 16) narrow_by_columns<1, SC>(d, X, index, Y, B, s);
+        else if (d.K <= 32) narrow_by_columns<2, SC>(d, X, index, Y, B, s);
+        else if (d.K <= 64) narrow_by_columns<4, SC>(d, X, index, Y, B, s);
+        else narrow_by_columns<8, SC>(d, X, index, Y, B, s);
+        return;
+    }
     if (B <= AD_FEW_ROWS) {
         float* H = (float*)ws;
         hipLaunchKernelGGL((adapt_low_rows_kernel<SC>), dim3((unsigned)cdiv(B * (d.p.Rp / 4), AD_THREADS / 64)), dim3(AD_THREADS), 0, s, d, X, index, H, B);
