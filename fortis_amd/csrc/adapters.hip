@@ -11,8 +11,8 @@
 //
 // Many rows: bound by the matrix pipes.  Rows are sorted by adapter inside windows of AD_WINDOW rows (one launch), H is
 // formed for 32 sorted rows at a time, and the GEMM tile of gemm.hip runs over the sorted rows: a row of A is found through
-// the permutation, and behind the k loop each wave adds, per 32 rows and adapter among them, H U_i^T to the sums
-// of that adapter's rows.  Sorted rows leave one or two adapters to a block of 32; rows that were not sorted would leave up to
+// the permutation, and behind the k loop each wave adds, per 32 rows and adapter among them, H U_i^T with the H of other
+// adapters' rows as zeros.  Sorted rows leave one or two adapters to a block of 32; rows that were not sorted would leave up to
 // 32.  A window keeps a tile's rows and the rows it writes within a few megabytes of each other.  Sorting places equal
 // adapters in any order: a row's sums do not depend on its place.
 #include "gemm_dev.h"
@@ -128,45 +128,75 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
 #define NARROW_K 128
 #define NARROW_N 128
 #define NARROW_RANK 64
-// A wave owns 16 rows: their X as KG operands of four k (k = 16 g + 4 q + c, as above), the next rows' X on its way.  Per adapter
-// among the rows: all 16 are multiplied with its A, 16 ranks at a time, the products change places through the wave's own
-// piece of LDS into operands of the second product, and the sums are kept for the adapter's rows only (a NaN in the others'
-// products goes nowhere).
+#define NARROW_WAVE_FLOATS(KG, SC) (16 * 20 + ((SC) ? 16 * (16 * (KG) + 4) : 0))
+// A wave owns 16 rows: their X as KG operands of four k (k = 16 g + 4 q + c, as above).  Per adapter among the rows: all 16 are
+// multiplied with its A, 16 ranks at a time, the products change places through the wave's own piece of LDS into operands of
+// the second product, where those of other adapters' rows are zeros.  (0 times U is 0 for a finite U; others take the
+// few-rows form.)  Loads of X start before W is brought to LDS.
 template <int KG, int NT, bool SC>
-__global__ __launch_bounds__(AD_THREADS) void adapt_narrow_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
-                                                                  float* __restrict__ Y, long B)
+__global__ __launch_bounds__(AD_THREADS, KG <= 2 && NT <= 4 ? 5 : 2) void adapt_narrow_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
+                                                                  float* __restrict__ Y, long B, FastDiv byK)
 {
     extern __shared__ float4 smem4[];
     constexpr int LDW = 16 * KG + 4;
-    float* sW = (float*)smem4;                                              // [16 NT][LDW]
-    float* sH = sW + 16 * NT * LDW + (threadIdx.x >> 6) * 16 * 20;          // [16][20] for this wave
+    float* sW = (float*)smem4;                                                     // [16 NT][LDW]
+    float* sH = sW + 16 * NT * LDW + (threadIdx.x >> 6) * NARROW_WAVE_FLOATS(KG, SC);      // [16][20] for this wave
+    float* sX = sH + 16 * 20;                                                      // SC: [16][LDW], zeros behind K
     const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
+    const int K = (int)d.K;
+    const long step = (long)gridDim.x * (AD_THREADS / 64) * 16;
+    long m0 = ((long)blockIdx.x * (AD_THREADS / 64) + (threadIdx.x >> 6)) * 16;
+    v4f xv[KG];
+    int i = -1;
+    auto fetch = [&](long m) __attribute__((always_inline)) {
+        i = m + lr < B ? index[m + lr] : -1;
+        if constexpr (SC) {
+            // 16 K floats in the order of memory, whatever K is
+            const float* p = X + m * K;
+            const int n = B - m < 16 ? (int)(B - m) * K : 16 * K;
+#pragma unroll
+            for (int u = 0; u < 4 * KG; u++) {
+                const int e = lane + 64 * u;
+                xv[u / 4][u % 4] = p[e < n ? e : n - 1];
+            }
+        } else {
+            const long r = m + lr < B ? m + lr : B - 1;
+#pragma unroll
+            for (int g = 0; g < KG; g++) xv[g] = load_row4<false>(X + r * K, 16 * g + 4 * lq, K);
+        }
+    };
+    if (m0 < B) fetch(m0);
+    if constexpr (SC) {
+        for (int e = lane; e < 16 * LDW; e += 64) sX[e] = 0.f;
+    }
+    float bv[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) bv[t] = d.bias && 16 * t + lr < d.N ? d.bias[16 * t + lr] : 0.f;
     for (int e = threadIdx.x; e < 16 * NT * 4 * KG; e += AD_THREADS) {
         const int n = e / (4 * KG), k = e % (4 * KG) * 4;
         *(v4f*)(sW + n * LDW + k) = load_row4<false>(d.W + (n < d.N ? n : d.N - 1) * d.p.ldw, k, d.p.ldw);
     }
     __syncthreads();
-    float bv[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++) bv[t] = d.bias && 16 * t + lr < d.N ? d.bias[16 * t + lr] : 0.f;
-    const long step = (long)gridDim.x * (AD_THREADS / 64) * 16;
-    long m0 = ((long)blockIdx.x * (AD_THREADS / 64) + (threadIdx.x >> 6)) * 16;
-    if (m0 >= B) return;
-    v4f xn[KG];
-    int in;
-    auto fetch = [&](long m) __attribute__((always_inline)) {
-        const long r = m + lr < B ? m + lr : B - 1;
-#pragma unroll
-        for (int g = 0; g < KG; g++) xn[g] = load_row4<SC>(X + r * d.K, 16 * g + 4 * lq, d.K);
-        in = m + lr < B ? index[r] : -1;
+    auto turn = [&]() __attribute__((always_inline)) {         // the wave's LDS writes before its reads
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
-    fetch(m0);
-    for (; m0 < B; m0 += step) {
-        v4f xv[KG], acc[NT];
+    for (; m0 < B; ) {
+        v4f acc[NT];
+        if (i >= d.nadapt) i = -1;
+        unsigned live = (unsigned)__ballot(i >= 0) & 0xffff;
+        if constexpr (SC) {
 #pragma unroll
-        for (int g = 0; g < KG; g++) xv[g] = xn[g];
-        const int i = in >= 0 && in < d.nadapt ? in : -1;
-        if (m0 + step < B) fetch(m0 + step);
+            for (int u = 0; u < 4 * KG; u++) {
+                const unsigned e = lane + 64 * u, r = fortis_div(e, byK);
+                if (e < 16u * K) sX[r * LDW + e - r * K] = xv[u / 4][u % 4];
+            }
+            turn();
+#pragma unroll
+            for (int g = 0; g < KG; g++) xv[g] = *(const v4f*)(sX + lr * LDW + 16 * g + 4 * lq);
+            __builtin_amdgcn_wave_barrier();
+        }
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[t] = (v4f)(0.f);
 #pragma unroll
@@ -177,15 +207,12 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_narrow_kernel(AdaptDesc d, c
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[g][c], w[c], acc[t], 0, 0, 0);
             }
-        unsigned live = (unsigned)__ballot(i >= 0) & 0xffff;
         while (live) {
             const int a = __builtin_amdgcn_readlane(i, __builtin_ctz(live));
             const unsigned rows = (unsigned)__ballot(i == a) & 0xffff;
             live &= ~rows;
+            const bool mine = (rows >> lr) & 1;
             const float sc = d.scale[a];
-            v4f sum[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) sum[t] = (v4f)(0.f);
             for (int j0 = 0; j0 < d.rank; j0 += 16) {
                 const float* A = d.A + ((long)a * d.p.R16 + j0 + lr) * d.p.Ka + 4 * lq;
                 v4f h = (v4f)(0.f), av[KG], uv[NT];
@@ -203,42 +230,36 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_narrow_kernel(AdaptDesc d, c
                     for (int c = 0; c < 4; c++) h = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[g][c], av[g][c], h, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < 4; r++) sH[(4 * lq + r) * 20 + lr] = h[r] * sc;
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                turn();
                 v4f hv = *(const v4f*)(sH + lr * 20 + 4 * lq);
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int c = 0; c < 4; c++) if (j + c >= d.rank) hv[c] = 0.f;      // what is read of U there belongs to other ranks
+                for (int c = 0; c < 4; c++) if (!mine || j + c >= d.rank) hv[c] = 0.f;
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) sum[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[c], j < d.p.Rp ? uv[t][c] : 0.f, sum[t], 0, 0, 0);
+                    for (int c = 0; c < 4; c++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[c], uv[t][c], acc[t], 0, 0, 0);
             }
-            const unsigned sel = rows >> (4 * lq);
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) acc[t][r] += (sel >> r) & 1 ? sum[t][r] : 0.f;
         }
+        const long m = m0;
+        m0 += step;
+        if (m0 < B) fetch(m0);
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const long m = m0 + 4 * lq + r;
-            if (m >= B) continue;
+        for (int t = 0; t < NT; t++) {
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-                if (16 * t + lr < d.N) Y[m * d.N + 16 * t + lr] = fortis_act_any(acc[t][r] + bv[t], d.act, d.alpha);
+            for (int r = 0; r < 4; r++)
+                if (m + 4 * lq + r < B && 16 * t + lr < d.N) Y[(m + 4 * lq + r) * d.N + 16 * t + lr] = fortis_act_any(acc[t][r] + bv[t], d.act, d.alpha);
         }
     }
 }
 template <int KG, int NT, bool SC>
 static void launch_narrow(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, hipStream_t s)
 {
-    const size_t shmem = (size_t)(16 * NT * (16 * KG + 4) + (AD_THREADS / 64) * 16 * 20) * 4;
+    const size_t shmem = (size_t)(16 * NT * (16 * KG + 4) + (AD_THREADS / 64) * NARROW_WAVE_FLOATS(KG, SC)) * 4;
     static bool set = false;
     if (!set) { HIP_OK(hipFuncSetAttribute((const void*)adapt_narrow_kernel<KG, NT, SC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem)); set = true; }
     const long wgs = cdiv(B, 16 * (AD_THREADS / 64));
-    hipLaunchKernelGGL((adapt_narrow_kernel<KG, NT, SC>), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(AD_THREADS), shmem, s, d, X, index, Y, B);
+    hipLaunchKernelGGL((adapt_narrow_kernel<KG, NT, SC>), dim3((unsigned)(wgs < 1536 ? wgs : 1536)), dim3(AD_THREADS), shmem, s, d, X, index, Y, B, fortis_fast_div((unsigned)d.K));
 }
 template <int KG, bool SC>
 static void narrow_by_columns(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, hipStream_t s)
@@ -377,29 +398,20 @@ template <bool SC> struct AdaptRows {
                 const int a = __builtin_amdgcn_readlane(kk, __builtin_ctz(live));
                 const unsigned rows = (unsigned)__ballot(kk == a);
                 live &= ~rows;
-                v16f sum[TN];
+                const bool mine = (rows >> lr) & 1;
                 const float* u[TN];
 #pragma unroll
-                for (int j = 0; j < TN; j++) {
-                    sum[j] = (v16f)(0.f);
-                    u[j] = U + ((long)a * N + (n + j * 32 + lr < N ? n + j * 32 + lr : N - 1)) * Rp + 4 * lh;
-                }
+                for (int j = 0; j < TN; j++) u[j] = U + ((long)a * N + (n + j * 32 + lr < N ? n + j * 32 + lr : N - 1)) * Rp + 4 * lh;
                 for (long k = 0; k < Rp; k += 8) {
-                    const v4f hv = *(const v4f*)(h + k);
-                    v4f uv[TN];
+                    v4f hv = *(const v4f*)(h + k), uv[TN];
+                    if (!mine) hv = (v4f)(0.f);
 #pragma unroll
                     for (int j = 0; j < TN; j++) uv[j] = *(const v4f*)(u[j] + k);
 #pragma unroll
                     for (int c = 0; c < 4; c++)
 #pragma unroll
-                        for (int j = 0; j < TN; j++) sum[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(hv[c], uv[j][c], sum[j], 0, 0, 0);
+                        for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(hv[c], uv[j][c], acc[i][j], 0, 0, 0);
                 }
-                const unsigned sel = rows >> (4 * lh);
-#pragma unroll
-                for (int j = 0; j < TN; j++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        acc[i][j][r] += (sel >> (8 * (r >> 2) + (r & 3))) & 1 ? sum[j][r] : 0.f;
             }
         }
     }
@@ -513,14 +525,15 @@ long fortis_adapters_workspace(const AdaptDesc& d, long B)
 template <bool SC>
 static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {
-    if (d.K <= NARROW_K && d.N <= NARROW_N && d.rank <= NARROW_RANK) {
+    // (an adapter with an infinity or a NaN in U would reach other rows through 0 times U)
+    if (d.finite && d.K <= NARROW_K && d.N <= NARROW_N && d.rank <= NARROW_RANK) {
         if (d.K <= 16) narrow_by_columns<1, SC>(d, X, index, Y, B, s);
         else if (d.K <= 32) narrow_by_columns<2, SC>(d, X, index, Y, B, s);
         else if (d.K <= 64) narrow_by_columns<4, SC>(d, X, index, Y, B, s);
         else narrow_by_columns<8, SC>(d, X, index, Y, B, s);
         return;
     }
-    if (B <= AD_FEW_ROWS) {
+    if (B <= AD_FEW_ROWS || !d.finite) {
         float* H = (float*)ws;
         hipLaunchKernelGGL((adapt_low_rows_kernel<SC>), dim3((unsigned)cdiv(B * (d.p.Rp / 4), AD_THREADS / 64)), dim3(AD_THREADS), 0, s, d, X, index, H, B);
         hipLaunchKernelGGL((adapt_few_kernel<SC>), dim3((unsigned)(cdiv(B, 16) * cdiv(d.N, 16))), dim3(64 * FEW_WAVES), 0, s, d, X, index, (const float*)H, Y, B);

@@ -129,6 +129,7 @@ struct AdaptDesc {
     int act;
     float alpha;
     AdaptPitch p;
+    int finite;                 // every value of U is
     const float *W, *bias;      // device, padded with zeros: W [N][ldw]; bias may be null
     const float *A, *U, *scale; // [nadapt][R16][Ka], [nadapt][N][Rp], [nadapt]
 };

@@ -3,6 +3,7 @@
 // buffer ownership, upload/download choreography, pack/unpack staging, graph capture on the
 // second call and replay afterwards, with an eager fallback.
 #include <atomic>
+#include <cmath>
 #include <condition_variable>
 #include <mutex>
 #include <functional>
@@ -703,7 +704,8 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
                 break;
             case OP_ADAPT:
                 ex.kind = EX_ADAPT; ex.side = o.side; ex.rows = ex.rows_cap = o.B;
-                ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, fortis_adapters_pitch(o.K, o.D), nullptr, nullptr, nullptr, nullptr, nullptr };
+                ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, fortis_adapters_pitch(o.K, o.D), 1, nullptr, nullptr, nullptr, nullptr, nullptr };
+                for (float u : o.v1) if (!std::isfinite(u)) ex.adapt.finite = 0;
                 ex.adapt.W = upload_padded(p, o.w, 1, o.N, o.K, o.N, ex.adapt.p.ldw);
                 ex.adapt.bias = o.has_bias ? (const float*)upload(p, o.b.data(), o.b.size() * 4) : nullptr;
                 ex.adapt.A = upload_padded(p, o.v0, o.F, o.D, o.K, ex.adapt.p.R16, ex.adapt.p.Ka);
