@@ -25,7 +25,18 @@ static inline long up(long n, long m) { return (n + m - 1) / m * m; }
 
 // ---- weights, laid out once --------------------------------------------------------------------------------------
 // W [N][ldw], A [nadapt][R16][Ka], U [nadapt][N][Rp], padded with zeros.
-AdaptPitch fortis_adapters_pitch(long K, long rank) { return { up(K, 4), up(K, 16), up(rank, 16), up(rank, 8) }; }
+#define NARROW_K 128
+#define NARROW_N 128
+#define NARROW_RANK 64
+AdaptPitch fortis_adapters_pitch(long K, long N, long rank, bool finite)
+{
+    // (an adapter with an infinity or a NaN in U would reach other rows through 0 times U in all forms but the few-rows one)
+    const int narrow = finite && K <= NARROW_K && N <= NARROW_N && rank <= NARROW_RANK;
+    return { up(K, 4), up(K, 16), up(rank, 16), up(rank, narrow ? 16 : 8), narrow, finite };
+}
+// Where rank j of a row of U lies: in order, but 4 x 4 transposed within sixteen for the narrow form, whose instruction c then
+// multiplies ranks 4 c .. 4 c + 3 and which leaves out the instructions behind the last rank.
+long fortis_adapters_place(const AdaptPitch& p, long j) { return p.narrow ? j / 16 * 16 + j % 4 * 4 + j % 16 / 4 : j; }
 
 // Element k .. k + 3 of a row of K floats at p; what lies at or beyond K is 0.  SC: K is no multiple of 4.
 template <bool SC> __device__ __forceinline__ v4f load_row4(const float* p, long k, long K)
@@ -125,56 +136,57 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
 }
 
 // ---- narrow layers -----------------------------------------------------------------------------------------------
-#define NARROW_K 128
-#define NARROW_N 128
-#define NARROW_RANK 64
-#define NARROW_WAVE_FLOATS(KG, SC) (16 * 20 + ((SC) ? 16 * (16 * (KG) + 4) : 0))
-// A wave owns 16 rows: their X as KG operands of four k (k = 16 g + 4 q + c, as above).  Per adapter among the rows: all 16 are
-// multiplied with its A, 16 ranks at a time, the products change places through the wave's own piece of LDS into operands of
-// the second product, where those of other adapters' rows are zeros.  (0 times U is 0 for a finite U; others take the
-// few-rows form.)  Loads of X start before W is brought to LDS.
-template <int KG, int NT, bool SC>
-__global__ __launch_bounds__(AD_THREADS, KG <= 2 && NT <= 4 ? 5 : 2) void adapt_narrow_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
+// A wave owns RT times 16 rows: their X as KG operands of four k (k = 16 g + 4 q + c, as above).  Per adapter among the rows: all
+// are multiplied with its A, 16 ranks at a time, the products change places through the wave's own piece of LDS into
+// operands of the second product, where those of other adapters' rows are zeros.  Loads of X start before W is brought to LDS.
+#define NARROW_WAVE_FLOATS(KG, RT, SC) (16 * (RT) * 20 + ((SC) ? 16 * (RT) * (16 * (KG) + 4) : 0))
+template <int KG, int NT, int RT, bool SC>
+__global__ __launch_bounds__(AD_THREADS, KG * RT <= 4 && NT <= 4 ? 3 : 2) void adapt_narrow_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
                                                                   float* __restrict__ Y, long B, FastDiv byK)
 {
     extern __shared__ float4 smem4[];
-    constexpr int LDW = 16 * KG + 4;
-    float* sW = (float*)smem4;                                                     // [16 NT][LDW]
-    float* sH = sW + 16 * NT * LDW + (threadIdx.x >> 6) * NARROW_WAVE_FLOATS(KG, SC);      // [16][20] for this wave
-    float* sX = sH + 16 * 20;                                                      // SC: [16][LDW], zeros behind K
+    constexpr int LDW = 16 * KG + 4, ROWS = 16 * RT;
+    float* sW = (float*)smem4;                                                                 // [16 NT][LDW]
+    float* sH = sW + 16 * NT * LDW + (threadIdx.x >> 6) * NARROW_WAVE_FLOATS(KG, RT, SC);      // [ROWS][20] for this wave
+    float* sX = sH + ROWS * 20;                                                                // SC: [ROWS][LDW], zeros behind K
     const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
-    const int K = (int)d.K;
-    const long step = (long)gridDim.x * (AD_THREADS / 64) * 16;
-    long m0 = ((long)blockIdx.x * (AD_THREADS / 64) + (threadIdx.x >> 6)) * 16;
-    v4f xv[KG];
-    int i = -1;
+    const int K = (int)d.K, N = (int)d.N;
+    const long step = (long)gridDim.x * (AD_THREADS / 64) * ROWS;
+    long m0 = ((long)blockIdx.x * (AD_THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * ROWS;
+    v4f xv[RT][KG];
+    int i = -1;                                                                                // adapter of row lane % ROWS
     auto fetch = [&](long m) __attribute__((always_inline)) {
-        i = m + lr < B ? index[m + lr] : -1;
+        const int n = B - m < ROWS ? (int)(B - m) : ROWS, row = lane & (ROWS - 1);
+        i = row < n ? index[m + row] : -1;
+        const float* p = X + m * K;
         if constexpr (SC) {
-            // 16 K floats in the order of memory, whatever K is
-            const float* p = X + m * K;
-            const int n = B - m < 16 ? (int)(B - m) * K : 16 * K;
+            // the rows' floats in the order of memory, whatever K is
 #pragma unroll
-            for (int u = 0; u < 4 * KG; u++) {
+            for (int u = 0; u < 4 * KG * RT; u++) {
                 const int e = lane + 64 * u;
-                xv[u / 4][u % 4] = p[e < n ? e : n - 1];
+                xv[u / (4 * KG)][u / 4 % KG][u % 4] = p[e < n * K ? e : n * K - 1];
             }
         } else {
-            const long r = m + lr < B ? m + lr : B - 1;
 #pragma unroll
-            for (int g = 0; g < KG; g++) xv[g] = load_row4<false>(X + r * K, 16 * g + 4 * lq, K);
+            for (int h = 0; h < RT; h++)
+#pragma unroll
+                for (int g = 0; g < KG; g++) xv[h][g] = load_row4<false>(p + (16 * h + lr < n ? 16 * h + lr : n - 1) * K, 16 * g + 4 * lq, K);
         }
     };
     if (m0 < B) fetch(m0);
     if constexpr (SC) {
-        for (int e = lane; e < 16 * LDW; e += 64) sX[e] = 0.f;
+        for (int e = lane; e < ROWS * LDW; e += 64) sX[e] = 0.f;
     }
     float bv[NT];
+    int ucol[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) bv[t] = d.bias && 16 * t + lr < d.N ? d.bias[16 * t + lr] : 0.f;
+    for (int t = 0; t < NT; t++) {
+        bv[t] = d.bias && 16 * t + lr < N ? d.bias[16 * t + lr] : 0.f;
+        ucol[t] = (16 * t + lr < N ? 16 * t + lr : N - 1) * (int)d.p.Rp + 4 * lq;
+    }
     for (int e = threadIdx.x; e < 16 * NT * 4 * KG; e += AD_THREADS) {
         const int n = e / (4 * KG), k = e % (4 * KG) * 4;
-        *(v4f*)(sW + n * LDW + k) = load_row4<false>(d.W + (n < d.N ? n : d.N - 1) * d.p.ldw, k, d.p.ldw);
+        *(v4f*)(sW + n * LDW + k) = load_row4<false>(d.W + (n < N ? n : N - 1) * d.p.ldw, k, d.p.ldw);
     }
     __syncthreads();
     auto turn = [&]() __attribute__((always_inline)) {         // the wave's LDS writes before its reads
@@ -182,92 +194,124 @@ __global__ __launch_bounds__(AD_THREADS, KG <= 2 && NT <= 4 ? 5 : 2) void adapt_
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
-    for (; m0 < B; ) {
-        v4f acc[NT];
+    while (m0 < B) {
+        v4f acc[RT][NT];
         if (i >= d.nadapt) i = -1;
-        unsigned live = (unsigned)__ballot(i >= 0) & 0xffff;
+        unsigned live = (unsigned)__ballot(i >= 0) & (unsigned)((1ull << ROWS) - 1);
         if constexpr (SC) {
 #pragma unroll
-            for (int u = 0; u < 4 * KG; u++) {
+            for (int u = 0; u < 4 * KG * RT; u++) {
                 const unsigned e = lane + 64 * u, r = fortis_div(e, byK);
-                if (e < 16u * K) sX[r * LDW + e - r * K] = xv[u / 4][u % 4];
+                if (e < (unsigned)(ROWS * K)) sX[r * LDW + e - r * K] = xv[u / (4 * KG)][u / 4 % KG][u % 4];
             }
             turn();
 #pragma unroll
-            for (int g = 0; g < KG; g++) xv[g] = *(const v4f*)(sX + lr * LDW + 16 * g + 4 * lq);
+            for (int h = 0; h < RT; h++)
+#pragma unroll
+                for (int g = 0; g < KG; g++) xv[h][g] = *(const v4f*)(sX + (16 * h + lr) * LDW + 16 * g + 4 * lq);
             __builtin_amdgcn_wave_barrier();
         }
 #pragma unroll
-        for (int t = 0; t < NT; t++) acc[t] = (v4f)(0.f);
+        for (int h = 0; h < RT; h++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) acc[h][t] = (v4f)(0.f);
 #pragma unroll
         for (int g = 0; g < KG; g++)
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const v4f w = *(const v4f*)(sW + (16 * t + lr) * LDW + 16 * g + 4 * lq);
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[g][c], w[c], acc[t], 0, 0, 0);
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int h = 0; h < RT; h++) acc[h][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[h][g][c], w[c], acc[h][t], 0, 0, 0);
             }
         while (live) {
             const int a = __builtin_amdgcn_readlane(i, __builtin_ctz(live));
-            const unsigned rows = (unsigned)__ballot(i == a) & 0xffff;
+            const unsigned rows = (unsigned)__ballot(i == a) & (unsigned)((1ull << ROWS) - 1);
             live &= ~rows;
-            const bool mine = (rows >> lr) & 1;
             const float sc = d.scale[a];
             for (int j0 = 0; j0 < d.rank; j0 += 16) {
-                const float* A = d.A + ((long)a * d.p.R16 + j0 + lr) * d.p.Ka + 4 * lq;
-                v4f h = (v4f)(0.f), av[KG], uv[NT];
+                const float* A = d.A + ((long)a * d.p.R16 + j0) * d.p.Ka;                       // uniform
+                const float* U = d.U + (long)a * N * d.p.Rp + j0;
+                v4f h[RT], av[KG], uv[NT];
 #pragma unroll
-                for (int g = 0; g < KG; g++) av[g] = 16 * g < d.p.Ka ? *(const v4f*)(A + 16 * g) : (v4f)(0.f);
-                const int j = j0 + 4 * lq;
+                for (int g = 0; g < KG; g++) av[g] = 16 * g < d.p.Ka ? *(const v4f*)(A + lr * (int)d.p.Ka + 4 * lq + 16 * g) : (v4f)(0.f);
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const long n = 16 * t + lr < d.N ? 16 * t + lr : d.N - 1;
-                    uv[t] = *(const v4f*)(d.U + ((long)a * d.N + n) * d.p.Rp + (j < d.p.Rp ? j : 0));
-                }
+                for (int t = 0; t < NT; t++) uv[t] = *(const v4f*)(U + ucol[t]);
+#pragma unroll
+                for (int q = 0; q < RT; q++) h[q] = (v4f)(0.f);
 #pragma unroll
                 for (int g = 0; g < KG; g++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) h = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[g][c], av[g][c], h, 0, 0, 0);
+                    for (int c = 0; c < 4; c++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) sH[(4 * lq + r) * 20 + lr] = h[r] * sc;
+                        for (int q = 0; q < RT; q++) h[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[q][g][c], av[g][c], h[q], 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < RT; q++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) sH[(16 * q + 4 * lq + r) * 20 + lr] = h[q][r] * sc;
                 turn();
-                v4f hv = *(const v4f*)(sH + lr * 20 + 4 * lq);
+                const int left = (int)d.rank - j0;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    if (4 * c >= left) break;
+#pragma unroll
+                    for (int q = 0; q < RT; q++) {
+                        const float hv = sH[(16 * q + lr) * 20 + 4 * c + lq];
+                        const float hc = (rows >> (16 * q + lr)) & 1 && 4 * c + lq < left ? hv : 0.f;
+#pragma unroll
+                        for (int t = 0; t < NT; t++) acc[q][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(hc, uv[t][c], acc[q][t], 0, 0, 0);
+                    }
+                }
                 __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (int c = 0; c < 4; c++) if (!mine || j + c >= d.rank) hv[c] = 0.f;
-#pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(hv[c], uv[t][c], acc[t], 0, 0, 0);
             }
         }
-        const long m = m0;
+        float* y = Y + m0 * N;                                                                 // uniform
+        const int n = B - m0 < ROWS ? (int)(B - m0) : ROWS;
         m0 += step;
         if (m0 < B) fetch(m0);
+        const float alpha = d.alpha;
+        fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
+            for (int h = 0; h < RT; h++)
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (m + 4 * lq + r < B && 16 * t + lr < d.N) Y[(m + 4 * lq + r) * d.N + 16 * t + lr] = fortis_act_any(acc[t][r] + bv[t], d.act, d.alpha);
-        }
+                for (int r = 0; r < 4; r++) {
+                    const int m = 16 * h + 4 * lq + r;
+                    if (m >= n) continue;
+                    float* row = y + m * N + lr;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+                        if (16 * t + lr < N) row[16 * t] = fortis_act_any(acc[h][t][r] + bv[t], decltype(act)::value, alpha);
+                }
+        });
     }
 }
-template <int KG, int NT, bool SC>
+template <int KG, int NT, int RT, bool SC>
 static void launch_narrow(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, hipStream_t s)
 {
-    const size_t shmem = (size_t)(16 * NT * (16 * KG + 4) + (AD_THREADS / 64) * NARROW_WAVE_FLOATS(KG, SC)) * 4;
+    const size_t shmem = (size_t)(16 * NT * (16 * KG + 4) + (AD_THREADS / 64) * NARROW_WAVE_FLOATS(KG, RT, SC)) * 4;
     static bool set = false;
-    if (!set) { HIP_OK(hipFuncSetAttribute((const void*)adapt_narrow_kernel<KG, NT, SC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem)); set = true; }
-    const long wgs = cdiv(B, 16 * (AD_THREADS / 64));
-    hipLaunchKernelGGL((adapt_narrow_kernel<KG, NT, SC>), dim3((unsigned)(wgs < 1536 ? wgs : 1536)), dim3(AD_THREADS), shmem, s, d, X, index, Y, B, fortis_fast_div((unsigned)d.K));
+    if (!set) { HIP_OK(hipFuncSetAttribute((const void*)adapt_narrow_kernel<KG, NT, RT, SC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem)); set = true; }
+    const long wgs = cdiv(B, 16 * RT * (AD_THREADS / 64));
+    hipLaunchKernelGGL((adapt_narrow_kernel<KG, NT, RT, SC>), dim3((unsigned)(wgs < 1024 ? wgs : 1024)), dim3(AD_THREADS), shmem, s, d, X, index, Y, B, fortis_fast_div((unsigned)d.K));
 }
 template <int KG, bool SC>
 static void narrow_by_columns(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, hipStream_t s)
 {
-    if (d.N <= 16) launch_narrow<KG, 1, SC>(d, X, index, Y, B, s);
-    else if (d.N <= 32) launch_narrow<KG, 2, SC>(d, X, index, Y, B, s);
-    else if (d.N <= 64) launch_narrow<KG, 4, SC>(d, X, index, Y, B, s);
-    else launch_narrow<KG, 8, SC>(d, X, index, Y, B, s);
+    // 32 rows a wave where that still gives every SIMD a wave
+    const bool two = B >= 32 * 1024;
+    if constexpr (KG <= 4) {
+        if (two && d.N <= 64) {
+            if (d.N <= 16) launch_narrow<KG, 1, 2, SC>(d, X, index, Y, B, s);
+            else if (d.N <= 32) launch_narrow<KG, 2, 2, SC>(d, X, index, Y, B, s);
+            else launch_narrow<KG, 4, 2, SC>(d, X, index, Y, B, s);
+            return;
+        }
+    }
+    if (d.N <= 16) launch_narrow<KG, 1, 1, SC>(d, X, index, Y, B, s);
+    else if (d.N <= 32) launch_narrow<KG, 2, 1, SC>(d, X, index, Y, B, s);
+    else if (d.N <= 64) launch_narrow<KG, 4, 1, SC>(d, X, index, Y, B, s);
+    else launch_narrow<KG, 8, 1, SC>(d, X, index, Y, B, s);
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------------------
@@ -525,15 +569,14 @@ long fortis_adapters_workspace(const AdaptDesc& d, long B)
 template <bool SC>
 static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {
-    // (an adapter with an infinity or a NaN in U would reach other rows through 0 times U)
-    if (d.finite && d.K <= NARROW_K && d.N <= NARROW_N && d.rank <= NARROW_RANK) {
+    if (d.p.narrow) {
         if (d.K <= 16) narrow_by_columns<1, SC>(d, X, index, Y, B, s);
         else if (d.K <= 32) narrow_by_columns<2, SC>(d, X, index, Y, B, s);
         else if (d.K <= 64) narrow_by_columns<4, SC>(d, X, index, Y, B, s);
         else narrow_by_columns<8, SC>(d, X, index, Y, B, s);
         return;
     }
-    if (B <= AD_FEW_ROWS || !d.finite) {
+    if (B <= AD_FEW_ROWS || !d.p.finite) {
         float* H = (float*)ws;
         hipLaunchKernelGGL((adapt_low_rows_kernel<SC>), dim3((unsigned)cdiv(B * (d.p.Rp / 4), AD_THREADS / 64)), dim3(AD_THREADS), 0, s, d, X, index, H, B);
         hipLaunchKernelGGL((adapt_few_kernel<SC>), dim3((unsigned)(cdiv(B, 16) * cdiv(d.N, 16))), dim3(64 * FEW_WAVES), 0, s, d, X, index, (const float*)H, Y, B);

@@ -4,6 +4,7 @@
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
+#include <type_traits>
 #include "../../include/fortis_rt.h"
 #include "../../include/fortis_step.h"
 
@@ -122,14 +123,17 @@ long fortis_norm_workspace(const NormDesc& d);          // bytes fortis_launch_g
 void fortis_launch_group_norm(const NormDesc& d, const float* x, float* y, void* ws, hipStream_t s);
 
 // ---- projection with an adapter per row (adapters.hip) -------------------------------------
-struct AdaptPitch { long ldw, Ka, R16, Rp; };   // floats a row of W, of A; rows of A an adapter; floats a row of U and of the low-rank rows
-AdaptPitch fortis_adapters_pitch(long K, long rank);
+struct AdaptPitch {
+    long ldw, Ka, R16, Rp;      // floats a row of W, of A; rows of A an adapter; floats a row of U and of the low-rank rows
+    int narrow, finite;         // the one-launch form for narrow layers; every value of U is finite
+};
+AdaptPitch fortis_adapters_pitch(long K, long N, long rank, bool finite);
+long fortis_adapters_place(const AdaptPitch& p, long j);       // where rank j lies in a row of U
 struct AdaptDesc {
     long K, N, nadapt, rank;
     int act;
     float alpha;
     AdaptPitch p;
-    int finite;                 // every value of U is
     const float *W, *bias;      // device, padded with zeros: W [N][ldw]; bias may be null
     const float *A, *U, *scale; // [nadapt][R16][Ka], [nadapt][N][Rp], [nadapt]
 };
@@ -178,6 +182,14 @@ __device__ __forceinline__ float fortis_act_any(float v, int act, float alpha)
         return v * (v >= 0.f ? hi : lo);
     }
     return v;
+}
+// Runs body(ACT) with the activation as a compile-time constant (std::integral_constant): one test a kernel, not one a value.
+template <class F> __device__ __forceinline__ void fortis_with_act(int act, F&& body)
+{
+    if (act == FORTIS_ACT_RELU) body(std::integral_constant<int, FORTIS_ACT_RELU>());
+    else if (act == FORTIS_ACT_LEAKY) body(std::integral_constant<int, FORTIS_ACT_LEAKY>());
+    else if (act == FORTIS_ACT_SILU) body(std::integral_constant<int, FORTIS_ACT_SILU>());
+    else body(std::integral_constant<int, FORTIS_ACT_NONE>());
 }
 // n / d for n < 2^31 by one multiplication: with 2^l the power of two at or above d, m = ceil(2^(31 + l) / d) is at most
 // 2^32 - 1 and n m >> (31 + l) is the quotient.

@@ -98,6 +98,7 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
 #pragma unroll
             for (int c = 0; c < V; c++) { v[k].v[c] -= mean; const float t = have[k] ? v[k].v[c] : 0.f; s = fmaf(t, t, s); }
         const float rstd = 1.f / sqrtf(sum_lanes<L>(s) * inv + d.eps);
+        fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
             if (!have[k]) continue;
@@ -113,9 +114,10 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
                 if (d.beta) be = ld<V>(d.beta + ch[k]);
             }
 #pragma unroll
-            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, ga.v[c], be.v[c]), d.act, d.alpha);
+            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, ga.v[c], be.v[c]), decltype(act)::value, d.alpha);
             st<V>(a.y + at[k], o);
         }
+        });
     }
 }
 
@@ -174,6 +176,7 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
 #pragma unroll
             for (int c = 0; c < V; c++) { v[k].v[c] -= mean; const float t = threadIdx.x + k * T < nv ? v[k].v[c] : 0.f; s = fmaf(t, t, s); }
         const float rstd = 1.f / sqrtf(sum_block<T>(s, red) * inv + d.eps);
+        fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
             unsigned e = threadIdx.x + k * T, ch;
@@ -185,10 +188,11 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
 #pragma unroll
             for (int c = 0; c < V; c++) {
                 const unsigned i = ch + (d.first ? 0 : c);
-                o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, d.gamma ? d.gamma[i] : 1.f, d.beta ? d.beta[i] : 0.f), d.act, d.alpha);
+                o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, d.gamma ? d.gamma[i] : 1.f, d.beta ? d.beta[i] : 0.f), decltype(act)::value, d.alpha);
             }
             st<V>(y + at, o);
         }
+        });
     }
 }
 // Channels last, `gs` neighbouring groups of one sample per workgroup (together up to a 128-byte line of channels or a little
@@ -242,14 +246,16 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
         Vals<V> ga, be;
 #pragma unroll
         for (int c = 0; c < V; c++) { ga.v[c] = d.gamma ? d.gamma[c0 + c] : 1.f; be.v[c] = d.beta ? d.beta[c0 + c] : 0.f; }
+        fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
             if (row + k * rows >= d.S) continue;
             Vals<V> o;
 #pragma unroll
-            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, ga.v[c], be.v[c]), d.act, d.alpha);
+            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, ga.v[c], be.v[c]), decltype(act)::value, d.alpha);
             st<V>(a.y + base + (long)(row + k * rows) * d.C, o);
         }
+        });
     }
 }
 
@@ -434,6 +440,7 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, Spli
     const long r0 = chunk * h.per, r1 = r0 + h.per < d.S ? r0 + h.per : d.S;
     const long off = n * d.S * d.C + c0;
     if (r0 + row >= r1) return;
+    fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
     for (long r = r0 + row + (r1 - 1 - r0 - row) / rows * rows; r >= r0; r -= GS_AHEAD * rows) {
         Vals<V> v[GS_AHEAD];
 #pragma unroll
@@ -443,10 +450,11 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, Spli
         for (int k = 0; k < GS_AHEAD; k++) {
             if (r - k * rows < r0) break;
 #pragma unroll
-            for (int c = 0; c < V; c++) v[k].v[c] = fortis_act_any(fmaf((v[k].v[c] - hi[c]) - lo[c], sc[c], be[c]), d.act, d.alpha);
+            for (int c = 0; c < V; c++) v[k].v[c] = fortis_act_any(fmaf((v[k].v[c] - hi[c]) - lo[c], sc[c], be[c]), decltype(act)::value, d.alpha);
             st<V>(a.y + off + (r - k * rows) * d.C, v[k]);
         }
     }
+    });
 }
 template <int V>
 __global__ __launch_bounds__(GS_THREADS) void norm_apply_first_kernel(NormArgs a, SplitShape h, const double2* __restrict__ in)
@@ -467,6 +475,7 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_first_kernel(NormArgs a
     const long nv = a.count / V, e0 = chunk * h.per, e1 = e0 + h.per < nv ? e0 + h.per : nv;
     const bool small = nv < (1L << 31);
     if (e0 + tid >= e1) return;
+    fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
     for (long e = e0 + tid + (e1 - 1 - e0 - tid) / GS_THREADS * GS_THREADS; e >= e0; e -= GS_AHEAD * GS_THREADS) {
         Vals<V> v[GS_AHEAD];
         float sc[GS_AHEAD], be[GS_AHEAD];
@@ -484,10 +493,11 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_first_kernel(NormArgs a
             const long i = e - k * GS_THREADS;
             if (i < e0) break;
 #pragma unroll
-            for (int c = 0; c < V; c++) v[k].v[c] = fortis_act_any(fmaf((v[k].v[c] - s.hi) - s.lo, sc[k], be[k]), d.act, d.alpha);
+            for (int c = 0; c < V; c++) v[k].v[c] = fortis_act_any(fmaf((v[k].v[c] - s.hi) - s.lo, sc[k], be[k]), decltype(act)::value, d.alpha);
             st<V>(y + i * V, v[k]);
         }
     }
+    });
 }
 
 // ---- choice ------------------------------------------------------------------------------------------------------

@@ -702,16 +702,22 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
                 if (o.has_v[0]) ex.norm.gamma = (const float*)upload(p, o.v0.data(), o.v0.size() * 4);
                 if (o.has_v[1]) ex.norm.beta = (const float*)upload(p, o.v1.data(), o.v1.size() * 4);
                 break;
-            case OP_ADAPT:
+            case OP_ADAPT: {
                 ex.kind = EX_ADAPT; ex.side = o.side; ex.rows = ex.rows_cap = o.B;
-                ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, fortis_adapters_pitch(o.K, o.D), 1, nullptr, nullptr, nullptr, nullptr, nullptr };
-                for (float u : o.v1) if (!std::isfinite(u)) ex.adapt.finite = 0;
-                ex.adapt.W = upload_padded(p, o.w, 1, o.N, o.K, o.N, ex.adapt.p.ldw);
+                bool finite = true;
+                for (float u : o.v1) finite = finite && std::isfinite(u);
+                const AdaptPitch pitch = fortis_adapters_pitch(o.K, o.N, o.D, finite);
+                ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, pitch, nullptr, nullptr, nullptr, nullptr, nullptr };
+                ex.adapt.W = upload_padded(p, o.w, 1, o.N, o.K, o.N, pitch.ldw);
                 ex.adapt.bias = o.has_bias ? (const float*)upload(p, o.b.data(), o.b.size() * 4) : nullptr;
-                ex.adapt.A = upload_padded(p, o.v0, o.F, o.D, o.K, ex.adapt.p.R16, ex.adapt.p.Ka);
-                ex.adapt.U = upload_padded(p, o.v1, o.F, o.N, o.D, o.N, ex.adapt.p.Rp);
+                ex.adapt.A = upload_padded(p, o.v0, o.F, o.D, o.K, pitch.R16, pitch.Ka);
+                std::vector<float> U((size_t)(o.F * o.N * pitch.Rp), 0.f);
+                for (long r = 0; r < o.F * o.N; r++)
+                    for (long j = 0; j < o.D; j++) U[(size_t)(r * pitch.Rp + fortis_adapters_place(pitch, j))] = o.v1[(size_t)(r * o.D + j)];
+                ex.adapt.U = (const float*)upload(p, U.data(), U.size() * 4);
                 ex.adapt.scale = (const float*)upload(p, o.v2.data(), o.v2.size() * 4);
                 break;
+            }
             case OP_RECUR:
                 ex.kind = EX_RECUR; ex.side = o.side; ex.h_in = o.h_in; ex.h_out = o.h_out;
                 break;
