@@ -19,7 +19,7 @@
 
 #define AD_THREADS 256
 #define AD_WINDOW 2048          // rows sorted together; a multiple of the tile's 128
-#define AD_FEW_ROWS 512
+#define AD_FEW_ROWS 1024
 
 static inline long up(long n, long m) { return (n + m - 1) / m * m; }
 
@@ -38,11 +38,14 @@ AdaptPitch fortis_adapters_pitch(long K, long N, long rank, bool finite)
 // multiplies ranks 4 c .. 4 c + 3 and which leaves out the instructions behind the last rank.
 long fortis_adapters_place(const AdaptPitch& p, long j) { return p.narrow ? j / 16 * 16 + j % 4 * 4 + j % 16 / 4 : j; }
 
-// Element k .. k + 3 of a row of K floats at p; what lies at or beyond K is 0.  SC: K is no multiple of 4.
-template <bool SC> __device__ __forceinline__ v4f load_row4(const float* p, long k, long K)
+// Elements k .. k + 3 of a row of K floats at p; what lies at or beyond K is 0.  How rows lie: ROW4 K is a multiple of 4; ROWANY
+// rows start at any float and K is at least 4: the 16 bytes are loaded where they are; ROWTINY K < 4.
+enum { ROW4 = 0, ROWANY = 1, ROWTINY = 2 };
+template <int ROW> __device__ __forceinline__ v4f load_row4(const float* p, long k, long K)
 {
+    if constexpr (ROW == ROWANY) return shift_row4(*(const v4f_any*)(p + (k <= K - 4 ? k : K - 4)), k, K);
     v4f v;
-    if constexpr (SC) {
+    if constexpr (ROW == ROWTINY) {
 #pragma unroll
         for (int c = 0; c < 4; c++) { const float t = p[k + c < K ? k + c : K - 1]; v[c] = k + c < K ? t : 0.f; }
     } else {
@@ -54,7 +57,7 @@ template <bool SC> __device__ __forceinline__ v4f load_row4(const float* p, long
 
 // ---- few rows ----------------------------------------------------------------------------------------------------
 // H[r][4 q .. 4 q + 3], one wave each: lanes stride over k.
-template <bool SC>
+template <int ROW>
 __global__ __launch_bounds__(AD_THREADS) void adapt_low_rows_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
                                                                     float* __restrict__ H, long B)
 {
@@ -68,7 +71,7 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_low_rows_kernel(AdaptDesc d,
     const float* a = d.A + ((long)i * d.p.R16 + 4 * q) * d.p.Ka;
     float s[4] = { 0.f, 0.f, 0.f, 0.f };
     for (long k = lane * 4; k < d.p.Ka; k += 256) {
-        const v4f xv = load_row4<SC>(x, k, d.K);
+        const v4f xv = load_row4<ROW>(x, k, d.K);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const v4f av = *(const v4f*)(a + j * d.p.Ka + k);
@@ -89,7 +92,7 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_low_rows_kernel(AdaptDesc d,
 // and of W as one 16-byte load each and feeds four matrix instructions: instruction c multiplies k = 16 g + 4 q + c for lane
 // quarter q on both sides.
 #define FEW_WAVES 8
-template <bool SC>
+template <int ROW>
 __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
                                                                    const float* __restrict__ H, float* __restrict__ Y, long B)
 {
@@ -106,8 +109,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             const long k = (g + u * FEW_WAVES) * 16 + 4 * lq;
-            xv[u] = load_row4<SC>(x, k, d.K);
-            wv[u] = load_row4<false>(w, k, d.p.ldw);
+            xv[u] = load_row4<ROW>(x, k, d.K);
+            wv[u] = load_row4<ROW4>(w, k, d.p.ldw);
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; u++)
@@ -170,7 +173,7 @@ __global__ __launch_bounds__(AD_THREADS, KG * RT <= 4 && NT <= 4 ? 3 : 2) void a
 #pragma unroll
             for (int h = 0; h < RT; h++)
 #pragma unroll
-                for (int g = 0; g < KG; g++) xv[h][g] = load_row4<false>(p + (16 * h + lr < n ? 16 * h + lr : n - 1) * K, 16 * g + 4 * lq, K);
+                for (int g = 0; g < KG; g++) xv[h][g] = load_row4<ROW4>(p + (16 * h + lr < n ? 16 * h + lr : n - 1) * K, 16 * g + 4 * lq, K);
         }
     };
     if (m0 < B) fetch(m0);
@@ -186,7 +189,7 @@ __global__ __launch_bounds__(AD_THREADS, KG * RT <= 4 && NT <= 4 ? 3 : 2) void a
     }
     for (int e = threadIdx.x; e < 16 * NT * 4 * KG; e += AD_THREADS) {
         const int n = e / (4 * KG), k = e % (4 * KG) * 4;
-        *(v4f*)(sW + n * LDW + k) = load_row4<false>(d.W + (n < N ? n : N - 1) * d.p.ldw, k, d.p.ldw);
+        *(v4f*)(sW + n * LDW + k) = load_row4<ROW4>(d.W + (n < N ? n : N - 1) * d.p.ldw, k, d.p.ldw);
     }
     __syncthreads();
     auto turn = [&]() __attribute__((always_inline)) {         // the wave's LDS writes before its reads
@@ -359,13 +362,13 @@ __global__ __launch_bounds__(1024) void adapt_sort_kernel(const int* __restrict_
     }
 }
 
-// H of 32 sorted rows: the four waves divide the 16-wide k groups, 16 ranks at a time; per adapter among the rows all 32 are
+// H of 32 sorted rows: KS waves divide the 16-wide k groups, 16 ranks at a time; per adapter among the rows all 32 are
 // multiplied with its A and its own rows kept.
-template <bool SC>
-__global__ __launch_bounds__(AD_THREADS) void adapt_low_sorted_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ perm,
+template <int KS, bool SC>
+__global__ __launch_bounds__(64 * KS) void adapt_low_sorted_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ perm,
                                                                       const int* __restrict__ key, float* __restrict__ H, long B)
 {
-    __shared__ float part[4][32][17];
+    __shared__ float part[KS][32][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
     const long p0 = (long)blockIdx.x * 32, base = p0 / AD_WINDOW * AD_WINDOW;
     const int kk = p0 + (lane & 31) < B ? key[p0 + (lane & 31)] : -1;
@@ -376,7 +379,7 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_low_sorted_kernel(AdaptDesc 
         x[h] = X + (base + perm[p]) * d.K;
     }
     const long groups = d.p.Ka / 16;
-    constexpr int AHEAD = 4;
+    constexpr int AHEAD = 6;
     unsigned live = (unsigned)__ballot(kk >= 0);
     while (live) {
         const int a = __builtin_amdgcn_readlane(kk, __builtin_ctz(live));
@@ -386,14 +389,14 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_low_sorted_kernel(AdaptDesc 
         for (long j0 = 0; j0 < d.rank; j0 += 16) {
             const float* w = d.A + ((long)a * d.p.R16 + j0 + lr) * d.p.Ka;
             v4f acc[2] = { (v4f)(0.f), (v4f)(0.f) };
-            for (long g = wave; g < groups; g += 4 * AHEAD) {
+            for (long g = wave; g < groups; g += KS * AHEAD) {
                 v4f xv[2][AHEAD], wv[AHEAD];
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++) {
-                    const long k = (g + u * 4) * 16 + 4 * lq;
-                    xv[0][u] = load_row4<SC>(x[0], k, d.K);
-                    xv[1][u] = load_row4<SC>(x[1], k, d.K);
-                    wv[u] = load_row4<false>(w, k, d.p.Ka);
+                    const long k = (g + u * KS) * 16 + 4 * lq;
+                    xv[0][u] = load_row4<SC ? ROWANY : ROW4>(x[0], k, d.K);
+                    xv[1][u] = load_row4<SC ? ROWANY : ROW4>(x[1], k, d.K);
+                    wv[u] = load_row4<ROW4>(w, k, d.p.Ka);
                 }
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++)
@@ -409,11 +412,12 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_low_sorted_kernel(AdaptDesc 
 #pragma unroll
                 for (int r = 0; r < 4; r++) part[wave][16 * h + 4 * lq + r][lr] = acc[h][r];
             __syncthreads();
-#pragma unroll
-            for (int e = threadIdx.x; e < 512; e += AD_THREADS) {
+            for (int e = threadIdx.x; e < 512; e += 64 * KS) {
                 const int m = e >> 4, j = e & 15;
                 if (!((rows >> m) & 1) || j0 + j >= d.p.Rp) continue;
-                const float v = ((part[0][m][j] + part[1][m][j]) + part[2][m][j]) + part[3][m][j];
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < KS; w++) v += part[w][m][j];
                 H[(p0 + m) * d.p.Rp + j0 + j] = j0 + j < d.rank ? v * sc : 0.f;
             }
         }
@@ -422,7 +426,7 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_low_sorted_kernel(AdaptDesc 
 
 // The GEMM tile over sorted rows.
 template <bool SC> struct AdaptRows {
-    static constexpr bool kPlain = false, kScalar = SC;
+    static constexpr bool kPlain = false, kAnyRow = SC;
     const int *perm, *key;
     const float *H, *U;
     long ldw, B, N, Rp;
@@ -566,6 +570,13 @@ long fortis_adapters_workspace(const AdaptDesc& d, long B)
 {
     return up(B, AD_WINDOW) * 8 + B * d.p.Rp * 4;
 }
+template <int ROW>
+static void launch_few(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
+{
+    float* H = (float*)ws;
+    hipLaunchKernelGGL((adapt_low_rows_kernel<ROW>), dim3((unsigned)cdiv(B * (d.p.Rp / 4), AD_THREADS / 64)), dim3(AD_THREADS), 0, s, d, X, index, H, B);
+    hipLaunchKernelGGL((adapt_few_kernel<ROW>), dim3((unsigned)(cdiv(B, 16) * cdiv(d.N, 16))), dim3(64 * FEW_WAVES), 0, s, d, X, index, (const float*)H, Y, B);
+}
 template <bool SC>
 static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {
@@ -576,18 +587,19 @@ static void launch_adapters(const AdaptDesc& d, const float* X, const int* index
         else narrow_by_columns<8, SC>(d, X, index, Y, B, s);
         return;
     }
-    if (B <= AD_FEW_ROWS || !d.p.finite) {
-        float* H = (float*)ws;
-        hipLaunchKernelGGL((adapt_low_rows_kernel<SC>), dim3((unsigned)cdiv(B * (d.p.Rp / 4), AD_THREADS / 64)), dim3(AD_THREADS), 0, s, d, X, index, H, B);
-        hipLaunchKernelGGL((adapt_few_kernel<SC>), dim3((unsigned)(cdiv(B, 16) * cdiv(d.N, 16))), dim3(64 * FEW_WAVES), 0, s, d, X, index, (const float*)H, Y, B);
-        return;
-    }
+    if (d.K < 4) { launch_few<ROWTINY>(d, X, index, Y, B, ws, s); return; }
+    if (B <= AD_FEW_ROWS || !d.p.finite) { launch_few<SC ? ROWANY : ROW4>(d, X, index, Y, B, ws, s); return; }
     const long Bw = up(B, AD_WINDOW);
     int *perm = (int*)ws, *key = perm + Bw;
     float* H = (float*)(key + Bw);
     hipLaunchKernelGGL(adapt_sort_kernel, dim3((unsigned)(Bw / AD_WINDOW)), dim3(1024), (size_t)(d.nadapt + 1 + 16) * 4, s, index, perm, key, B, (int)d.nadapt);
-    hipLaunchKernelGGL((adapt_low_sorted_kernel<SC>), dim3((unsigned)cdiv(B, 32)), dim3(AD_THREADS), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
-    launch_adapt_gemm<SC>(d, X, Y, B, { perm, key, H, d.U, d.p.ldw, B, d.N, d.p.Rp }, s);
+    // as many waves as leave each the six groups that it loads at once
+    const dim3 blocks((unsigned)cdiv(B, 32));
+    if (d.p.Ka <= 12 * 16) hipLaunchKernelGGL((adapt_low_sorted_kernel<1, SC>), blocks, dim3(64), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
+    else if (d.p.Ka <= 24 * 16) hipLaunchKernelGGL((adapt_low_sorted_kernel<2, SC>), blocks, dim3(128), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
+    else hipLaunchKernelGGL((adapt_low_sorted_kernel<8, SC>), blocks, dim3(512), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
+    const AdaptRows<SC> ext = { perm, key, H, d.U, d.p.ldw, B, d.N, d.p.Rp };
+    launch_adapt_gemm<SC>(d, X, Y, B, ext, s);
 }
 void fortis_launch_linear_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {

@@ -8,6 +8,19 @@ typedef float v4f __attribute__((ext_vector_type(4)));   // native vector: selec
 
 #define GM_THREADS 256
 
+// Four floats from any float on, and what a load from the last four floats of a row of K has to become to stand for k .. k + 3.
+typedef v4f v4f_any __attribute__((aligned(4)));
+__device__ __forceinline__ v4f shift_row4(v4f t, long k, long K)
+{
+    const int s = k <= K - 4 ? 0 : (int)(k - (K - 4));
+    v4f v;
+    v[0] = s == 0 ? t[0] : s == 1 ? t[1] : s == 2 ? t[2] : s == 3 ? t[3] : 0.f;
+    v[1] = s == 0 ? t[1] : s == 1 ? t[2] : s == 2 ? t[3] : 0.f;
+    v[2] = s == 0 ? t[2] : s == 1 ? t[3] : 0.f;
+    v[3] = s == 0 ? t[3] : 0.f;
+    return v;
+}
+
 struct GemmEpi {
     const float* bias;
     const float* out_scale;
@@ -75,10 +88,10 @@ __device__ __forceinline__ void lds_barrier()
 // one (kPlain false) gives
 //   base(m0), rel(m)   A's row of tile row m is base(m0) + rel(m)
 //   ldw                pitch of W's rows
-//   kScalar            A is read float by float (K no multiple of 4; ldw is one, W's rows end in zeros)
+//   kAnyRow            A's rows start at any float (K no multiple of 4 but at least 4; ldw is one, W's rows end in zeros)
 //   add(acc, ...)      sums that join before the epilogue
 //   store(acc, ...)    the epilogue
-struct GemmPlain { static constexpr bool kPlain = true, kScalar = false; };
+struct GemmPlain { static constexpr bool kPlain = true, kAnyRow = false; };
 template <int TM, int TN, int GM_BK, class Ext>
 __device__ __forceinline__ void gemm_tile(const float* __restrict__ A, const float* __restrict__ W,
                                           float* __restrict__ C, long B, long N, long K,
@@ -122,7 +135,7 @@ __device__ __forceinline__ void gemm_tile(const float* __restrict__ A, const flo
         for (int t = 0; t < LA; t++) {
             const int f = tid + t * GM_THREADS, row = f / F4R, kq = f % F4R;
             if constexpr (Ext::kPlain) oa[t] = ((unsigned)(row < lastm ? row : lastm) * (unsigned)K + kq * 4) * 4u;
-            else oa[t] = (ext.rel(mt + (row < lastm ? row : lastm)) * (unsigned)K + (Ext::kScalar ? 0 : kq * 4)) * 4u;
+            else oa[t] = (ext.rel(mt + (row < lastm ? row : lastm)) * (unsigned)K + (Ext::kAnyRow ? 0 : kq * 4)) * 4u;
         }
 #pragma unroll
         for (int t = 0; t < LW; t++) {
@@ -139,15 +152,11 @@ __device__ __forceinline__ void gemm_tile(const float* __restrict__ A, const flo
     // A chunk at or beyond K reads the row's chunk 0 instead (a valid address) and is zeroed when stored.
     auto load_slab = [&](const float* Ab, const float* Wb, const unsigned (&oa)[LA], const unsigned (&ow)[LW], long k0) __attribute__((always_inline)) {
         const char* wb = (const char*)(Wb + k0);
-        if constexpr (Ext::kScalar) {
-            // element k of a row; one at or beyond K reads the row's last instead and is zeroed when stored
-            unsigned ok[4];
+        if constexpr (Ext::kAnyRow) {
+            // from the row's last four floats at most; moved into place when stored
+            const unsigned ok = (unsigned)(k0 + kq4 <= K - 4 ? k0 + kq4 : K - 4) * 4u;
 #pragma unroll
-            for (int c = 0; c < 4; c++) ok[c] = (unsigned)(k0 + kq4 + c < K ? k0 + kq4 + c : K - 1) * 4u;
-#pragma unroll
-            for (int t = 0; t < LA; t++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) ra[t][c] = *(const float*)((const char*)Ab + oa[t] + ok[c]);
+            for (int t = 0; t < LA; t++) ra[t] = *(const v4f_any*)((const char*)Ab + oa[t] + ok);
         } else {
             const char* ab = (const char*)(Ab + k0);
 #pragma unroll
@@ -162,7 +171,7 @@ __device__ __forceinline__ void gemm_tile(const float* __restrict__ A, const flo
         if (k0 + GM_BK > K) {
             asm volatile("" ::: "memory");               // stays a branch
             const unsigned adj = k0 + kq4 < K ? 0u : (unsigned)kq4 * 4u;
-            if constexpr (!Ext::kScalar) {
+            if constexpr (!Ext::kAnyRow) {
 #pragma unroll
                 for (int t = 0; t < LA; t++) oa[t] -= adj;
             }
@@ -185,11 +194,11 @@ __device__ __forceinline__ void gemm_tile(const float* __restrict__ A, const flo
 #pragma unroll
                 for (int t = 0; t < LW; t++) rw[t] = zero;
             }
-            if constexpr (Ext::kScalar) {
+            if constexpr (Ext::kAnyRow) {
+                if (k0 + kq4 < K) {
 #pragma unroll
-                for (int t = 0; t < LA; t++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) ra[t][c] = k0 + kq4 + c < K ? ra[t][c] : 0.f;
+                    for (int t = 0; t < LA; t++) ra[t] = shift_row4(ra[t], k0 + kq4, K);
+                }
             }
         }
 #pragma unroll
