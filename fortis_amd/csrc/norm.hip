@@ -53,7 +53,10 @@ struct NormArgs {
     float* y;
     long cg, count;             // channels a group, values an instance
     FastDiv row;                // vectors of an instance's row (channels last), or of a channel (channels first)
+    FastDiv group;              // groups of a sample
 };
+// (64-bit divisions take a hundred instructions each; counts that reach 2^31 are rare enough to pay for them)
+__device__ __forceinline__ long div_up31(long n, const FastDiv& f) { return n < (1L << 31) ? (long)fortis_div((unsigned)n, f) : n / (long)f.d; }
 
 // ---- lanes form --------------------------------------------------------------------------------------------------
 // Element e (vectors of V) of an instance: position e / (cg / V), channel V * (e % (cg / V)); channels first: V values of
@@ -68,7 +71,7 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
     for (long first = (long)blockIdx.x * (256 / L); first < total; first += step) {
         const long inst = first + threadIdx.x / L;
         const bool on = inst < total;
-        const long n = on ? inst / d.G : 0;
+        const long n = on ? div_up31(inst, a.group) : 0;
         const int g = on ? (int)(inst - n * d.G) : 0;
         const long base = d.first ? (n * d.C + g * a.cg) * d.S : n * d.S * d.C + g * a.cg;
         Vals<V> v[E];
@@ -142,7 +145,7 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
     const NormDesc& d = a.d;
     const unsigned nv = (unsigned)(a.count / V);
     for (long inst = blockIdx.x; inst < total; inst += gridDim.x) {
-        const long n = inst / d.G;
+        const long n = div_up31(inst, a.group);
         const int g = (int)(inst - n * d.G);
         const float* x = a.x + (d.first ? (n * d.C + g * a.cg) * d.S : n * d.S * d.C + g * a.cg);
         float* y = a.y + (x - a.x);
@@ -198,14 +201,14 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
 // Channels last, `gs` neighbouring groups of one sample per workgroup (together up to a 128-byte line of channels or a little
 // more): a thread keeps its column of V channels, which lie in one group, and takes every rows-th position.
 template <int V, int T, int E>
-__global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs, int slices, long total)
+__global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs, FastDiv slices, long total)
 {
     __shared__ float part[T], sums[T];
     const NormDesc& d = a.d;
     const int tid = threadIdx.x;
     for (long item = blockIdx.x; item < total; item += gridDim.x) {
-        const long n = item / slices;
-        const int g0 = (int)(item - n * slices) * gs, ng = d.G - g0 < gs ? (int)(d.G - g0) : gs;
+        const long n = div_up31(item, slices);
+        const int g0 = (int)(item - n * slices.d) * gs, ng = d.G - g0 < gs ? (int)(d.G - g0) : gs;
         const int cgv = (int)(a.cg / V), wv = ng * cgv, rows = T / wv;
         const int col = tid % wv, row = tid / wv, gl = col / cgv;
         const bool on = row < rows;
@@ -261,14 +264,36 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
 
 // ---- split form --------------------------------------------------------------------------------------------------
 #define GS_THREADS 1024
-#define GS_AHEAD 4             // loads a thread has in flight while it normalises
+#define GS_AHEAD 8             // loads a thread has in flight
 struct SplitShape {
     long chunks, per;        // chunks of a sample (an instance with channels first), positions (vectors) a chunk
     int V;                   // floats a thread loads at a time
     int gs, slices;          // channels last: groups and workgroups across the channels
     int blocks;              // workgroups across one group's channels (1 unless a group is wider than 1024 vectors)
     long parts;              // partial sums an instance has
+    FastDiv by_chunks, by_across, by_blocks, by_cg;
 };
+// Where a workgroup of the split form stands (channels last).
+struct SplitPlace { long n, c_lo; int chunk, g0, ng, wv, rows, col, row, bl; };
+template <int V> __device__ __forceinline__ SplitPlace split_place(const NormArgs& a, const SplitShape& h)
+{
+    SplitPlace p;
+    const NormDesc& d = a.d;
+    const unsigned rest = fortis_div(blockIdx.x, h.by_chunks), n = fortis_div(rest, h.by_across), across = rest - n * h.by_across.d;
+    const unsigned sl = fortis_div(across, h.by_blocks);
+    p.chunk = (int)(blockIdx.x - rest * h.by_chunks.d);
+    p.n = n;
+    p.bl = (int)(across - sl * h.by_blocks.d);
+    p.g0 = (int)sl * h.gs;
+    p.ng = d.G - p.g0 < h.gs ? (int)(d.G - p.g0) : h.gs;
+    p.c_lo = (long)p.g0 * a.cg + (long)p.bl * GS_THREADS * V;                  // first channel of the workgroup
+    const long c_hi = h.blocks > 1 ? ((long)p.g0 + 1) * a.cg : (long)(p.g0 + p.ng) * a.cg;
+    p.wv = (int)((c_hi - p.c_lo) / V < GS_THREADS ? (c_hi - p.c_lo) / V : GS_THREADS);
+    p.rows = (int)((unsigned)GS_THREADS / (unsigned)p.wv);
+    p.row = (int)(threadIdx.x / (unsigned)p.wv);
+    p.col = (int)threadIdx.x - p.row * p.wv;
+    return p;
+}
 
 // Partial sums of `n` values about P: a1 = sum(v - P), a2 = sum((v - P)^2), from sums about a pivot of the thread's own.
 __device__ __forceinline__ void about(float pivot, int n, float s1, float s2, double P, double& a1, double& a2)
@@ -276,9 +301,10 @@ __device__ __forceinline__ void about(float pivot, int n, float s1, float s2, do
     const double dn = (double)n;
     a1 = a2 = 0.0;
     if (n == 0) return;
-    const double t1 = dn * ((double)pivot - P) + (double)s1;
-    const double m2 = (double)s2 - (double)s1 * (double)s1 / dn;       // centred, of this thread's values
-    a1 = t1; a2 = m2 + t1 * t1 / dn;
+    // centred, s2 - s1^2 / n, and moved to P, + t1^2 / n, where t1 - s1 = n (pivot - P): no division
+    const double d = (double)pivot - P;
+    a1 = dn * d + (double)s1;
+    a2 = (double)s2 + d * ((double)s1 + a1);
 }
 __device__ __forceinline__ double sum_wave(double v)
 {
@@ -294,66 +320,85 @@ __global__ __launch_bounds__(GS_THREADS) void norm_sums_kernel(NormArgs a, Split
     __shared__ double2 part[GS_THREADS];
     const NormDesc& d = a.d;
     const int tid = threadIdx.x;
-    const long chunk = blockIdx.x % h.chunks, rest = blockIdx.x / h.chunks;
-    const int across = h.slices * h.blocks;
-    const long n = rest / across;
-    const int sl = (int)(rest - n * across) / h.blocks, bl = (int)(rest - n * across) % h.blocks;
-    const int g0 = sl * h.gs, ng = d.G - g0 < h.gs ? (int)(d.G - g0) : h.gs;
-    const long c_lo = (long)g0 * a.cg + (long)bl * GS_THREADS * V;                    // first channel of the workgroup
-    const long c_hi = h.blocks > 1 ? ((long)g0 + 1) * a.cg : (long)(g0 + ng) * a.cg;
-    const int wv = (int)((c_hi - c_lo) / V < GS_THREADS ? (c_hi - c_lo) / V : GS_THREADS), rows = GS_THREADS / wv;
-    const int col = tid % wv, row = tid / wv;
-    const long r0 = chunk * h.per, r1 = r0 + h.per < d.S ? r0 + h.per : d.S;
-    const float* x = a.x + (n * d.S) * d.C + c_lo + col * V;
+    const SplitPlace w = split_place<V>(a, h);
+    const long r0 = (long)w.chunk * h.per, r1 = r0 + h.per < d.S ? r0 + h.per : d.S;
+    const float* xs = a.x + w.n * d.S * d.C;
+    // a column's V channels lie in one group unless the slice is all channels and V does not divide cg
+    const bool one = a.cg % V == 0;
+    int g[V];
+    float P[V];                                 // the groups' first values: what the sums are joined about
+#pragma unroll
+    for (int c = 0; c < V; c++) {
+        g[c] = h.blocks > 1 ? w.g0 : (int)fortis_div((unsigned)(w.c_lo + w.col * V + c), h.by_cg);
+        P[c] = xs[g[c] * a.cg];
+    }
     float p[V], s1[V], s2[V];
     int cnt = 0;
 #pragma unroll
     for (int c = 0; c < V; c++) p[c] = s1[c] = s2[c] = 0.f;
-    if (row < rows && r0 + row < r1) {
-        const Vals<V> f = ld<V>(x + (r0 + row) * d.C);
+    auto take = [&](const Vals<V>& v) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < V; c++) p[c] = f.v[c];
-#pragma unroll 4
-        for (long r = r0 + row; r < r1; r += rows) {
-            const Vals<V> v = ld<V>(x + r * d.C);
+        for (int c = 0; c < V; c++) { const float t = v.v[c] - p[c]; s1[c] += t; s2[c] = fmaf(t, t, s2[c]); }
+    };
+    // whole passes of the workgroup over `rows` positions: uniform base + a 32-bit offset of the thread's own
+    const unsigned off = ((unsigned)w.row * (unsigned)d.C + (unsigned)w.col * V) * 4u;
+    const char* base = (const char*)(xs + w.c_lo + r0 * d.C);
+    const long pass = (long)w.rows * d.C * 4;
+    int left = (int)(r1 - r0);
+    if (w.row < w.rows) {
+        if (w.row < left) {
+            const Vals<V> f = ld<V>((const float*)(base + off));
 #pragma unroll
-            for (int c = 0; c < V; c++) { const float t = v.v[c] - p[c]; s1[c] += t; s2[c] = fmaf(t, t, s2[c]); }
-            cnt++;
+            for (int c = 0; c < V; c++) p[c] = f.v[one ? 0 : c];
         }
+        while (left >= GS_AHEAD * w.rows) {
+            Vals<V> v[GS_AHEAD];
+#pragma unroll
+            for (int k = 0; k < GS_AHEAD; k++) v[k] = ld<V>((const float*)(base + k * pass + off));
+#pragma unroll
+            for (int k = 0; k < GS_AHEAD; k++) take(v[k]);
+            cnt += GS_AHEAD;
+            base += GS_AHEAD * pass;
+            left -= GS_AHEAD * w.rows;
+        }
+        Vals<V> v[GS_AHEAD];
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++)
+            if (w.row + k * w.rows < left) v[k] = ld<V>((const float*)(base + k * pass + off));
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++)
+            if (w.row + k * w.rows < left) { take(v[k]); cnt++; }
     }
-    // join: a column's V channels lie in one group unless the slice is all channels and V does not divide cg
-    const int gfirst = h.blocks > 1 ? g0 : (int)((c_lo + col * V) / a.cg);
-    const bool one = a.cg % V == 0;
     for (int c = 0; c < (one ? 1 : V); c++) {
         double a1 = 0, a2 = 0;
         if (one) {
-            const double P = a.x[n * d.S * d.C + gfirst * a.cg];
 #pragma unroll
-            for (int k = 0; k < V; k++) { double b1, b2; about(p[k], cnt, s1[k], s2[k], P, b1, b2); a1 += b1; a2 += b2; }
+            for (int k = 1; k < V; k++) { s1[0] += s1[k]; s2[0] += s2[k]; }
+            about(p[0], V * cnt, s1[0], s2[0], (double)P[0], a1, a2);
         } else {
             // component c of every column; the groups then take the components one after the other
-            const int g = (int)((c_lo + col * V + c) / a.cg);
-            float pc = 0, s1c = 0, s2c = 0;
+            float pc = 0, s1c = 0, s2c = 0, Pc = 0;
 #pragma unroll
-            for (int k = 0; k < V; k++) if (k == c) { pc = p[k]; s1c = s1[k]; s2c = s2[k]; }
-            about(pc, cnt, s1c, s2c, (double)a.x[n * d.S * d.C + g * a.cg], a1, a2);
+            for (int k = 0; k < V; k++) if (k == c) { pc = p[k]; s1c = s1[k]; s2c = s2[k]; Pc = P[k]; }
+            about(pc, cnt, s1c, s2c, (double)Pc, a1, a2);
         }
         __syncthreads();
         part[tid] = make_double2(a1, a2);
         __syncthreads();
-        for (int g = tid >> 6; g < ng; g += GS_THREADS / 64) {
-            // columns that hold a channel of group g0 + g in component c (any component when V divides cg)
-            const long lo = h.blocks > 1 ? 0 : (long)g * a.cg, hi = h.blocks > 1 ? (long)wv * V : lo + a.cg;
-            const int k0 = one ? (int)(lo / V) : (int)((lo - c + V - 1 + V) / V - 1), k1 = one ? (int)(hi / V) : (int)((hi - c + V - 1 + V) / V - 1);
+        for (int q = tid >> 6; q < w.ng; q += GS_THREADS / 64) {
+            // columns that hold a channel of group g0 + q in component c (any component when V divides cg)
+            const int lo = h.blocks > 1 ? 0 : (int)(q * a.cg), hi = h.blocks > 1 ? w.wv * V : lo + (int)a.cg;
+            const int k0 = one ? lo / V : (lo - c + V - 1 + V) / V - 1, k1 = one ? hi / V : (hi - c + V - 1 + V) / V - 1;
             double t1 = 0, t2 = 0;
-            const int w = k1 - k0;
-            for (int i = tid & 63; i < rows * w; i += 64) {
-                const double2 q = part[(i / w) * wv + k0 + i % w];
-                t1 += q.x; t2 += q.y;
+            const int width = k1 - k0;
+            for (int i = tid & 63; i < w.rows * width; i += 64) {
+                const int r = (int)((unsigned)i / (unsigned)width);
+                const double2 t = part[r * w.wv + k0 + i - r * width];
+                t1 += t.x; t2 += t.y;
             }
             t1 = sum_wave(t1); t2 = sum_wave(t2);
             if ((tid & 63) == 0) {
-                double2* o = out + (n * d.G + g0 + g) * h.parts + chunk * h.blocks + bl;
+                double2* o = out + (w.n * d.G + w.g0 + q) * h.parts + w.chunk * h.blocks + w.bl;
                 if (c == 0) *o = make_double2(t1, t2);
                 else *o = make_double2(o->x + t1, o->y + t2);
             }
@@ -366,29 +411,44 @@ __global__ __launch_bounds__(GS_THREADS) void norm_sums_first_kernel(NormArgs a,
 {
     __shared__ double2 part[GS_THREADS / 64];
     const int tid = threadIdx.x;
-    const long chunk = blockIdx.x % h.chunks, inst = blockIdx.x / h.chunks;
+    const unsigned inst = fortis_div(blockIdx.x, h.by_chunks), chunk = blockIdx.x - inst * h.by_chunks.d;
     const float* x = a.x + inst * a.count;
     const long nv = a.count / V, e0 = chunk * h.per, e1 = e0 + h.per < nv ? e0 + h.per : nv;
+    const float P = x[0];
     float p = 0.f, s1 = 0.f, s2 = 0.f;
     int cnt = 0;
-    if (e0 + tid < e1) {
-        p = x[(e0 + tid) * V];
-#pragma unroll 4
-        for (long e = e0 + tid; e < e1; e += GS_THREADS) {
-            const Vals<V> v = ld<V>(x + e * V);
+    auto take = [&](const Vals<V>& v) __attribute__((always_inline)) {
 #pragma unroll
-            for (int c = 0; c < V; c++) { const float t = v.v[c] - p; s1 += t; s2 = fmaf(t, t, s2); }
-            cnt += V;
-        }
+        for (int c = 0; c < V; c++) { const float t = v.v[c] - p; s1 += t; s2 = fmaf(t, t, s2); }
+        cnt += V;
+    };
+    const float* base = x + e0 * V;
+    long left = e1 - e0;
+    if (tid < left) p = base[tid * V];
+    for (; left >= GS_AHEAD * GS_THREADS; left -= GS_AHEAD * GS_THREADS, base += GS_AHEAD * GS_THREADS * V) {
+        Vals<V> v[GS_AHEAD];
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++) v[k] = ld<V>(base + (k * GS_THREADS + tid) * V);
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++) take(v[k]);
+    }
+    {
+        Vals<V> v[GS_AHEAD];
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++)
+            if (k * GS_THREADS + tid < left) v[k] = ld<V>(base + (k * GS_THREADS + tid) * V);
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++)
+            if (k * GS_THREADS + tid < left) take(v[k]);
     }
     double a1, a2;
-    about(p, cnt, s1, s2, (double)x[0], a1, a2);
+    about(p, cnt, s1, s2, (double)P, a1, a2);
     a1 = sum_wave(a1); a2 = sum_wave(a2);
     if ((tid & 63) == 0) part[tid >> 6] = make_double2(a1, a2);
     __syncthreads();
     if (tid == 0) {
         for (int w = 1; w < GS_THREADS / 64; w++) { a1 += part[w].x; a2 += part[w].y; }
-        out[inst * h.parts + chunk] = make_double2(a1, a2);
+        out[(long)inst * h.parts + chunk] = make_double2(a1, a2);
     }
 }
 
@@ -403,57 +463,65 @@ __device__ __forceinline__ Stat join(const double2* part, long parts, double piv
     if (var < 0) var = 0;                                  // a NaN stays one
     const double mean = pivot + t1;
     Stat s;
-    s.hi = (float)mean; s.lo = (float)(mean - (double)s.hi); s.rstd = (float)(1.0 / sqrt(var + (double)eps)); s.pad = 0.f;
+    s.hi = (float)mean; s.lo = (float)(mean - (double)s.hi); s.rstd = 1.f / sqrtf((float)(var + (double)eps)); s.pad = 0.f;
     return s;
 }
-// Channels last: the same chunks and columns as the sums, last position first (what the caches still hold).
+// Channels last: the same chunks and columns as the sums, last position first (what the caches still hold).  The first loads
+// travel while the sums are joined.
 template <int V>
 __global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, SplitShape h, const double2* __restrict__ in)
 {
     __shared__ Stat stat[GS_THREADS];
     const NormDesc& d = a.d;
-    const int tid = threadIdx.x;
-    const long chunk = blockIdx.x % h.chunks, rest = blockIdx.x / h.chunks;
-    const int across = h.slices * h.blocks;
-    const long n = rest / across;
-    const int sl = (int)(rest - n * across) / h.blocks, bl = (int)(rest - n * across) % h.blocks;
-    const int g0 = sl * h.gs, ng = d.G - g0 < h.gs ? (int)(d.G - g0) : h.gs;
-    const long c_lo = (long)g0 * a.cg + (long)bl * GS_THREADS * V;
-    const long c_hi = h.blocks > 1 ? ((long)g0 + 1) * a.cg : (long)(g0 + ng) * a.cg;
-    const int wv = (int)((c_hi - c_lo) / V < GS_THREADS ? (c_hi - c_lo) / V : GS_THREADS), rows = GS_THREADS / wv;
-    for (int g = tid >> 6; g < ng; g += GS_THREADS / 64) {
-        const Stat s = join(in + (n * d.G + g0 + g) * h.parts, h.parts, (double)a.x[n * d.S * d.C + (g0 + g) * a.cg], (double)a.count, d.eps);
-        if ((tid & 63) == 0) stat[g] = s;
+    const SplitPlace w = split_place<V>(a, h);
+    const long r0 = (long)w.chunk * h.per, r1 = r0 + h.per < d.S ? r0 + h.per : d.S, c0 = w.c_lo + w.col * V;
+    const bool on = w.row < w.rows;
+    // passes of the workgroup over `rows` positions, GS_AHEAD at a time, the last ones first
+    const unsigned off = ((unsigned)w.row * (unsigned)d.C + (unsigned)w.col * V) * 4u;
+    const long pass = (long)w.rows * d.C * 4, first = (w.n * d.S + r0) * d.C + w.c_lo;
+    const int batch = GS_AHEAD * w.rows, total = (int)(r1 - r0);
+    int at = (total - 1) / batch * batch;                    // first position of the batch
+    const char* x = (const char*)(a.x + first) + (long)(at / w.rows) * pass;
+    char* y = (char*)(a.y + first) + (long)(at / w.rows) * pass;
+    Vals<V> v[GS_AHEAD];
+    if (on) {                                                // the last batch may be short
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++)
+            if (at + w.row + k * w.rows < total) v[k] = ld<V>((const float*)(x + k * pass + off));
+    }
+    for (int q = threadIdx.x >> 6; q < w.ng; q += GS_THREADS / 64) {
+        const Stat s = join(in + (w.n * d.G + w.g0 + q) * h.parts, h.parts, (double)a.x[w.n * d.S * d.C + (w.g0 + q) * a.cg], (double)a.count, d.eps);
+        if ((threadIdx.x & 63) == 0) stat[q] = s;
     }
     __syncthreads();
-    const int col = tid % wv, row = tid / wv;
-    if (row >= rows) return;
-    const long c0 = c_lo + col * V;
+    if (!on) return;
     float hi[V], lo[V], sc[V], be[V];
 #pragma unroll
     for (int c = 0; c < V; c++) {
-        const Stat s = stat[h.blocks > 1 ? 0 : (int)((c0 + c) / a.cg) - g0];
+        const Stat s = stat[h.blocks > 1 ? 0 : (int)fortis_div((unsigned)(c0 + c), h.by_cg) - w.g0];
         hi[c] = s.hi; lo[c] = s.lo;
         sc[c] = s.rstd * (d.gamma ? d.gamma[c0 + c] : 1.f);
         be[c] = d.beta ? d.beta[c0 + c] : 0.f;
     }
-    const long r0 = chunk * h.per, r1 = r0 + h.per < d.S ? r0 + h.per : d.S;
-    const long off = n * d.S * d.C + c0;
-    if (r0 + row >= r1) return;
+    const float alpha = d.alpha;
     fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
-    for (long r = r0 + row + (r1 - 1 - r0 - row) / rows * rows; r >= r0; r -= GS_AHEAD * rows) {
-        Vals<V> v[GS_AHEAD];
+        auto put = [&](int k) __attribute__((always_inline)) {
+            Vals<V> o;
+#pragma unroll
+            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf((v[k].v[c] - hi[c]) - lo[c], sc[c], be[c]), decltype(act)::value, alpha);
+            st<V>((float*)(y + k * pass + off), o);
+        };
 #pragma unroll
         for (int k = 0; k < GS_AHEAD; k++)
-            if (r - k * rows >= r0) v[k] = ld<V>(a.x + off + (r - k * rows) * d.C);
+            if (at + w.row + k * w.rows < total) put(k);
+        while ((at -= batch) >= 0) {
+            x -= GS_AHEAD * pass;
+            y -= GS_AHEAD * pass;
 #pragma unroll
-        for (int k = 0; k < GS_AHEAD; k++) {
-            if (r - k * rows < r0) break;
+            for (int k = 0; k < GS_AHEAD; k++) v[k] = ld<V>((const float*)(x + k * pass + off));
 #pragma unroll
-            for (int c = 0; c < V; c++) v[k].v[c] = fortis_act_any(fmaf((v[k].v[c] - hi[c]) - lo[c], sc[c], be[c]), decltype(act)::value, d.alpha);
-            st<V>(a.y + off + (r - k * rows) * d.C, v[k]);
+            for (int k = 0; k < GS_AHEAD; k++) put(k);
         }
-    }
     });
 }
 template <int V>
@@ -462,41 +530,49 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_first_kernel(NormArgs a
     __shared__ Stat stat;
     const NormDesc& d = a.d;
     const int tid = threadIdx.x;
-    const long chunk = blockIdx.x % h.chunks, inst = blockIdx.x / h.chunks;
-    const long g = inst % d.G;
+    const unsigned inst = fortis_div(blockIdx.x, h.by_chunks), chunk = blockIdx.x - inst * h.by_chunks.d;
+    const unsigned g = inst - fortis_div(inst, a.group) * a.group.d;
     const float* x = a.x + inst * a.count;
     float* y = a.y + inst * a.count;
+    const long nv = a.count / V, e0 = chunk * h.per, e1 = e0 + h.per < nv ? e0 + h.per : nv;
+    const bool small = nv < (1L << 31);
+    const long total = e1 - e0;
+    long at = (total - 1) / (GS_AHEAD * GS_THREADS) * (GS_AHEAD * GS_THREADS);       // first vector of the batch, the last one first
+    const float* xb = x + (e0 + at) * V;
+    float* yb = y + (e0 + at) * V;
+    Vals<V> v[GS_AHEAD];
+#pragma unroll
+    for (int k = 0; k < GS_AHEAD; k++)
+        if (at + k * GS_THREADS + tid < total) v[k] = ld<V>(xb + (k * GS_THREADS + tid) * V);
     if (tid < 64) {
-        const Stat s = join(in + inst * h.parts, h.parts, (double)x[0], (double)a.count, d.eps);
+        const Stat s = join(in + (long)inst * h.parts, h.parts, (double)x[0], (double)a.count, d.eps);
         if (tid == 0) stat = s;
     }
     __syncthreads();
     const Stat s = stat;
-    const long nv = a.count / V, e0 = chunk * h.per, e1 = e0 + h.per < nv ? e0 + h.per : nv;
-    const bool small = nv < (1L << 31);
-    if (e0 + tid >= e1) return;
+    const float alpha = d.alpha;
+    const long c0 = g * a.cg;
     fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
-    for (long e = e0 + tid + (e1 - 1 - e0 - tid) / GS_THREADS * GS_THREADS; e >= e0; e -= GS_AHEAD * GS_THREADS) {
-        Vals<V> v[GS_AHEAD];
-        float sc[GS_AHEAD], be[GS_AHEAD];
+        auto put = [&](int k) __attribute__((always_inline)) {
+            const long e = e0 + at + k * GS_THREADS + tid;
+            const long c = c0 + (small ? (long)fortis_div((unsigned)e, a.row) : e / (d.S / V));
+            const float sc = s.rstd * (d.gamma ? d.gamma[c] : 1.f), be = d.beta ? d.beta[c] : 0.f;
+            Vals<V> o;
 #pragma unroll
-        for (int k = 0; k < GS_AHEAD; k++) {
-            const long i = e - k * GS_THREADS;
-            if (i < e0) break;
-            v[k] = ld<V>(x + i * V);
-            const long c = g * a.cg + (small ? (long)fortis_div((unsigned)i, a.row) : i / (d.S / V));
-            sc[k] = s.rstd * (d.gamma ? d.gamma[c] : 1.f);
-            be[k] = d.beta ? d.beta[c] : 0.f;
+            for (int q = 0; q < V; q++) o.v[q] = fortis_act_any(fmaf((v[k].v[q] - s.hi) - s.lo, sc, be), decltype(act)::value, alpha);
+            st<V>(yb + (k * GS_THREADS + tid) * V, o);
+        };
+#pragma unroll
+        for (int k = 0; k < GS_AHEAD; k++)
+            if (at + k * GS_THREADS + tid < total) put(k);
+        while ((at -= GS_AHEAD * GS_THREADS) >= 0) {
+            xb -= GS_AHEAD * GS_THREADS * V;
+            yb -= GS_AHEAD * GS_THREADS * V;
+#pragma unroll
+            for (int k = 0; k < GS_AHEAD; k++) v[k] = ld<V>(xb + (k * GS_THREADS + tid) * V);
+#pragma unroll
+            for (int k = 0; k < GS_AHEAD; k++) put(k);
         }
-#pragma unroll
-        for (int k = 0; k < GS_AHEAD; k++) {
-            const long i = e - k * GS_THREADS;
-            if (i < e0) break;
-#pragma unroll
-            for (int c = 0; c < V; c++) v[k].v[c] = fortis_act_any(fmaf((v[k].v[c] - s.hi) - s.lo, sc[k], be[k]), decltype(act)::value, d.alpha);
-            st<V>(y + i * V, v[k]);
-        }
-    }
     });
 }
 
@@ -521,6 +597,7 @@ static SplitShape split_shape(const NormDesc& d)
         h.chunks = cdiv(nv, h.per);
         h.gs = h.slices = h.blocks = 1;
         h.parts = h.chunks;
+        h.by_chunks = fortis_fast_div((unsigned)h.chunks);
         return h;
     }
     h.V = d.C % 4 == 0 && d.C <= 4 * GS_THREADS ? 4 : cg % 4 == 0 ? 4 : cg % 2 == 0 ? 2 : 1;
@@ -536,6 +613,10 @@ static SplitShape split_shape(const NormDesc& d)
     h.per = cdiv(d.S, h.chunks);
     h.chunks = cdiv(d.S, h.per);
     h.parts = h.chunks * h.blocks;
+    h.by_chunks = fortis_fast_div((unsigned)h.chunks);
+    h.by_across = fortis_fast_div((unsigned)(h.slices * h.blocks));
+    h.by_blocks = fortis_fast_div((unsigned)h.blocks);
+    h.by_cg = fortis_fast_div((unsigned)cg);
     return h;
 }
 
@@ -577,8 +658,8 @@ template <int V> static void launch_block(const NormArgs& a, int gs, hipStream_t
         if constexpr (V == 1) if (nv > 1024 * 16) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 32>), grid, dim3(1024), 0, s, a, total);
         return;
     }
-    const int slices = (int)cdiv(d.G, gs);
-    const long total = d.NB * slices;
+    const long nslices = cdiv(d.G, gs), total = d.NB * nslices;
+    const FastDiv slices = fortis_fast_div((unsigned)nslices);
     const long wv = gs * a.cg / V;
     const dim3 grid((unsigned)(total < 65536 ? total : 65536));
     if (wv <= 256 && d.S <= 256 / wv * 4) hipLaunchKernelGGL((norm_block_groups_kernel<V, 256, 4>), grid, dim3(256), 0, s, a, gs, slices, total);
@@ -602,7 +683,7 @@ template <int V> static void launch_split(const NormArgs& a, const SplitShape& h
 
 void fortis_launch_group_norm(const NormDesc& in, const float* x, float* y, void* ws, hipStream_t s)
 {
-    NormArgs a = { norm_normal(in), x, y, in.C / in.G, in.S * (in.C / in.G), {} };
+    NormArgs a = { norm_normal(in), x, y, in.C / in.G, in.S * (in.C / in.G), {}, fortis_fast_div((unsigned)in.G) };
     const NormDesc& d = a.d;
     if (a.count > GN_BLOCK_MAX) {
         const SplitShape h = split_shape(d);
