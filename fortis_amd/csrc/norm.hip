@@ -28,16 +28,19 @@ template <int V> __device__ __forceinline__ Vals<V> ld(const float* p)
     __builtin_memcpy(r.v, &t, sizeof t);
     return r;
 }
-template <int V> __device__ __forceinline__ void st(float* p, const Vals<V>& r)
+template <int V, bool STREAM = false> __device__ __forceinline__ void st(float* p, const Vals<V>& r)
 {
     typename VecOf<V>::T t;
     __builtin_memcpy(&t, r.v, sizeof t);
-    *(typename VecOf<V>::T*)p = t;
+    if constexpr (STREAM) __builtin_nontemporal_store(t, (typename VecOf<V>::T*)p);
+    else *(typename VecOf<V>::T*)p = t;
 }
 
-#define GN_LANES_MAX 2048      // values of an instance in the lanes form
-#define GN_BLOCK_MAX 32768     // in the block form: 1024 threads x 32
-#define GN_BLOCK_EDGE 32       // channels whose floats fill a 128-byte line
+#define GN_LANES_VECS 512      // vectors of an instance in the lanes form: 64 lanes x 8
+#define GN_BLOCK_VALUES 32768  // values of a workgroup in the block form: 1024 threads x 32
+#define GN_BLOCK_ALONE 8192    // up to this many the block form is taken however few workgroups there are
+#define GN_BLOCK_FULL 256      // workgroups that keep every compute unit busy
+#define GN_LINE 32             // channels whose floats fill a 128-byte line
 
 // Sum over the 2^k lanes around this one (L = 2^k).
 template <int L> __device__ __forceinline__ float sum_lanes(float v)
@@ -198,8 +201,7 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
         });
     }
 }
-// Channels last, `gs` neighbouring groups of one sample per workgroup (together up to a 128-byte line of channels or a little
-// more): a thread keeps its column of V channels, which lie in one group, and takes every rows-th position.
+// Channels last, `gs` neighbouring groups of one sample per workgroup: a thread keeps its column of V channels, which lie in one group, and takes every rows-th position.
 template <int V, int T, int E>
 __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs, FastDiv slices, long total)
 {
@@ -209,8 +211,8 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
     for (long item = blockIdx.x; item < total; item += gridDim.x) {
         const long n = div_up31(item, slices);
         const int g0 = (int)(item - n * slices.d) * gs, ng = d.G - g0 < gs ? (int)(d.G - g0) : gs;
-        const int cgv = (int)(a.cg / V), wv = ng * cgv, rows = T / wv;
-        const int col = tid % wv, row = tid / wv, gl = col / cgv;
+        const int cgv = (int)(a.cg / V), wv = ng * cgv, rows = (int)((unsigned)T / (unsigned)wv);
+        const int row = (int)((unsigned)tid / (unsigned)wv), col = tid - row * wv, gl = (int)((unsigned)col / (unsigned)cgv);
         const bool on = row < rows;
         const unsigned c0 = (unsigned)(g0 * a.cg) + col * V;
         const long base = n * d.S * d.C + c0;
@@ -225,8 +227,10 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
             __syncthreads();
             for (int g = tid >> 6; g < ng; g += T / 64) {
                 float t = 0.f;
-                for (int r = 0; r < rows; r++)
-                    for (int c = tid & 63; c < cgv; c += 64) t += part[r * wv + g * cgv + c];
+                for (unsigned i = tid & 63; i < (unsigned)(rows * cgv); i += 64) {
+                    const unsigned r = i / (unsigned)cgv;
+                    t += part[r * wv + g * cgv + i - r * cgv];
+                }
                 t = sum_lanes<64>(t);
                 if ((tid & 63) == 0) sums[g] = t;
             }
@@ -264,7 +268,7 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
 
 // ---- split form --------------------------------------------------------------------------------------------------
 #define GS_THREADS 1024
-#define GS_AHEAD 8             // loads a thread has in flight
+#define GS_AHEAD 4             // loads a thread has in flight
 struct SplitShape {
     long chunks, per;        // chunks of a sample (an instance with channels first), positions (vectors) a chunk
     int V;                   // floats a thread loads at a time
@@ -457,7 +461,13 @@ struct Stat { float hi, lo, rstd, pad; };
 __device__ __forceinline__ Stat join(const double2* part, long parts, double pivot, double count, float eps)
 {
     double t1 = 0, t2 = 0;
-    for (long i = threadIdx.x & 63; i < parts; i += 64) { const double2 q = part[i]; t1 += q.x; t2 += q.y; }
+    for (long i = threadIdx.x & 63; i < parts; i += 256) {         // four loads at once: one after the other they take 3 us for 256
+        double2 q[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) q[k] = part[i + 64 * k < parts ? i + 64 * k : i];
+#pragma unroll
+        for (int k = 0; k < 4; k++) if (i + 64 * k < parts) { t1 += q[k].x; t2 += q[k].y; }
+    }
     t1 = sum_wave(t1) / count; t2 = sum_wave(t2) / count;
     double var = t2 - t1 * t1;
     if (var < 0) var = 0;                                  // a NaN stays one
@@ -468,7 +478,7 @@ __device__ __forceinline__ Stat join(const double2* part, long parts, double piv
 }
 // Channels last: the same chunks and columns as the sums, last position first (what the caches still hold).  The first loads
 // travel while the sums are joined.
-template <int V>
+template <int V, bool STREAM>
 __global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, SplitShape h, const double2* __restrict__ in)
 {
     __shared__ Stat stat[GS_THREADS];
@@ -509,7 +519,7 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, Spli
             Vals<V> o;
 #pragma unroll
             for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf((v[k].v[c] - hi[c]) - lo[c], sc[c], be[c]), decltype(act)::value, alpha);
-            st<V>((float*)(y + k * pass + off), o);
+            st<V, STREAM>((float*)(y + k * pass + off), o);
         };
 #pragma unroll
         for (int k = 0; k < GS_AHEAD; k++)
@@ -524,7 +534,7 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, Spli
         }
     });
 }
-template <int V>
+template <int V, bool STREAM>
 __global__ __launch_bounds__(GS_THREADS) void norm_apply_first_kernel(NormArgs a, SplitShape h, const double2* __restrict__ in)
 {
     __shared__ Stat stat;
@@ -560,7 +570,7 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_first_kernel(NormArgs a
             Vals<V> o;
 #pragma unroll
             for (int q = 0; q < V; q++) o.v[q] = fortis_act_any(fmaf((v[k].v[q] - s.hi) - s.lo, sc, be), decltype(act)::value, alpha);
-            st<V>(yb + (k * GS_THREADS + tid) * V, o);
+            st<V, STREAM>(yb + (k * GS_THREADS + tid) * V, o);
         };
 #pragma unroll
         for (int k = 0; k < GS_AHEAD; k++)
@@ -620,10 +630,39 @@ static SplitShape split_shape(const NormDesc& d)
     return h;
 }
 
+// Which form a problem takes.  S = 1 may be re-sized to other row counts later and is decided by the width of a group alone.
+enum NormKind { NORM_LANES, NORM_BLOCK, NORM_GROUPS, NORM_SPLIT };
+struct NormForm { NormKind kind; int V, gs; };
+static NormForm norm_form(const NormDesc& d)
+{
+    const long cg = d.C / d.G, count = d.S * cg;
+    // a vector stays inside a group and a position (channels last) or inside a channel (channels first)
+    const long along = d.first ? d.S : cg;
+    NormForm f = { NORM_LANES, along % 4 == 0 ? 4 : along % 2 == 0 ? 2 : 1, 1 };
+    if (d.first || d.S == 1 || cg >= 4 * GN_LINE) {
+        // instances whose memory comes in long pieces
+        if (count <= GN_LANES_VECS * f.V) return f;
+        f.kind = count <= GN_BLOCK_ALONE || (count <= GN_BLOCK_VALUES && (d.S == 1 || d.NB * d.G >= GN_BLOCK_FULL)) ? NORM_BLOCK : NORM_SPLIT;
+        return f;
+    }
+    // Channels last and narrow groups: neighbouring groups share lines.  Instances of a few values are left to lanes all the
+    // same (a sample's are next to each other in a wave); otherwise a workgroup takes the groups of one line, or more of them
+    // as long as there are workgroups enough: 512 samples of 128 x 256 in groups of 32 channels, a group each: 36 us, the
+    // whole sample: see the figures at the top.
+    if (count <= 256) return f;
+    auto fits = [&](long gs) { return gs * cg / f.V <= 1024 && d.S <= 1024 / (gs * cg / f.V) * 8; };
+    f.gs = (int)cdiv(GN_LINE, cg);
+    if (f.gs > d.G) f.gs = (int)d.G;
+    while (2 * f.gs <= d.G && fits(2 * f.gs) && d.NB * cdiv(d.G, 2 * f.gs) >= 2 * GN_BLOCK_FULL) f.gs *= 2;
+    const bool enough = d.S * f.gs * cg <= GN_BLOCK_ALONE || d.NB * cdiv(d.G, f.gs) >= GN_BLOCK_FULL;
+    f.kind = fits(f.gs) && enough ? NORM_GROUPS : NORM_SPLIT;
+    return f;
+}
+
 long fortis_norm_workspace(const NormDesc& in)
 {
     const NormDesc d = norm_normal(in);
-    if (d.S * (d.C / d.G) <= GN_BLOCK_MAX) return 0;
+    if (norm_form(d).kind != NORM_SPLIT) return 0;
     return d.NB * d.G * split_shape(d).parts * (long)sizeof(double2);
 }
 
@@ -644,10 +683,10 @@ template <int V> static void launch_lanes(const NormArgs& a, long total, hipStre
     else GN_LANES(64, 8);
 #undef GN_LANES
 }
-template <int V> static void launch_block(const NormArgs& a, int gs, hipStream_t s)
+template <int V> static void launch_block(const NormArgs& a, NormKind kind, int gs, hipStream_t s)
 {
     const NormDesc& d = a.d;
-    if (gs == 1) {
+    if (kind == NORM_BLOCK) {
         const long total = d.NB * d.G, nv = a.count / V;
         const dim3 grid((unsigned)(total < 65536 ? total : 65536));
         if (nv <= 256 * 4) hipLaunchKernelGGL((norm_block_kernel<V, 256, 4>), grid, dim3(256), 0, s, a, total);
@@ -670,47 +709,43 @@ template <int V> static void launch_split(const NormArgs& a, const SplitShape& h
 {
     const NormDesc& d = a.d;
     double2* part = (double2*)ws;
+    // An output that the eight L2s (32 MB) cannot hold is written past them: it would only push out the input that the second
+    // launch is about to read (287496 x 64, 74 MB: 49.7 us through the caches, 40.5 us past them; 65536 x 32, 8 MB: no difference,
+    // and the next kernel finds it there).
+    const bool stream = d.NB * d.S * d.C * 4 > (32L << 20);
     if (d.first) {
         const dim3 grid((unsigned)(d.NB * d.G * h.chunks));
         hipLaunchKernelGGL((norm_sums_first_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, part);
-        hipLaunchKernelGGL((norm_apply_first_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+        if (stream) hipLaunchKernelGGL((norm_apply_first_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+        else hipLaunchKernelGGL((norm_apply_first_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
         return;
     }
     const dim3 grid((unsigned)(d.NB * h.slices * h.blocks * h.chunks));
     hipLaunchKernelGGL((norm_sums_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, part);
-    hipLaunchKernelGGL((norm_apply_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+    if (stream) hipLaunchKernelGGL((norm_apply_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+    else hipLaunchKernelGGL((norm_apply_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
 }
 
 void fortis_launch_group_norm(const NormDesc& in, const float* x, float* y, void* ws, hipStream_t s)
 {
     NormArgs a = { norm_normal(in), x, y, in.C / in.G, in.S * (in.C / in.G), {}, fortis_fast_div((unsigned)in.G) };
     const NormDesc& d = a.d;
-    if (a.count > GN_BLOCK_MAX) {
+    const NormForm f = norm_form(d);
+    if (f.kind == NORM_SPLIT) {
         const SplitShape h = split_shape(d);
         if (d.first && d.S / h.V < (1L << 31)) a.row = fortis_fast_div((unsigned)(d.S / h.V));
         if (h.V == 4) launch_split<4>(a, h, ws, s);
         else if (h.V == 2) launch_split<2>(a, h, ws, s);
         else launch_split<1>(a, h, ws, s);
-        HIP_OK(hipGetLastError());
-        return;
+    } else {
+        a.row = fortis_fast_div((unsigned)((d.first ? d.S : a.cg) / f.V));
+        if (f.kind == NORM_LANES) {
+            if (f.V == 4) launch_lanes<4>(a, d.NB * d.G, s);
+            else if (f.V == 2) launch_lanes<2>(a, d.NB * d.G, s);
+            else launch_lanes<1>(a, d.NB * d.G, s);
+        } else if (f.V == 4) launch_block<4>(a, f.kind, f.gs, s);
+        else if (f.V == 2) launch_block<2>(a, f.kind, f.gs, s);
+        else launch_block<1>(a, f.kind, f.gs, s);
     }
-    // a vector stays inside a group and a position (channels last) or inside a channel (channels first)
-    const long along = d.first ? d.S : a.cg;
-    const int V = along % 4 == 0 ? 4 : along % 2 == 0 ? 2 : 1;
-    a.row = fortis_fast_div((unsigned)(along / V));
-    // channels last and narrow groups over several positions: the groups whose channels share lines go to one workgroup
-    int gs = 1;
-    if (!d.first && d.S > 1 && a.cg < GN_BLOCK_EDGE && a.count > GN_LANES_MAX / 8) {
-        gs = (int)((GN_BLOCK_EDGE + a.cg - 1) / a.cg);
-        if (gs > d.G) gs = (int)d.G;
-        while (gs > 1 && d.S > 1024 / (gs * a.cg / V) * 8) gs--;       // what a workgroup's registers hold
-    }
-    if (gs == 1 && a.count <= (V == 4 ? GN_LANES_MAX : GN_LANES_MAX / 4 * V)) {
-        if (V == 4) launch_lanes<4>(a, d.NB * d.G, s);
-        else if (V == 2) launch_lanes<2>(a, d.NB * d.G, s);
-        else launch_lanes<1>(a, d.NB * d.G, s);
-    } else if (V == 4) launch_block<4>(a, gs, s);
-    else if (V == 2) launch_block<2>(a, gs, s);
-    else launch_block<1>(a, gs, s);
     HIP_OK(hipGetLastError());
 }
