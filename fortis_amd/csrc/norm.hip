@@ -639,7 +639,7 @@ static NormForm norm_form(const NormDesc& d)
     // a vector stays inside a group and a position (channels last) or inside a channel (channels first)
     const long along = d.first ? d.S : cg;
     NormForm f = { NORM_LANES, along % 4 == 0 ? 4 : along % 2 == 0 ? 2 : 1, 1 };
-    if (d.first || d.S == 1 || cg >= 4 * GN_LINE) {
+    if (d.first || d.S == 1 || d.G == 1 || cg >= 4 * GN_LINE) {
         // instances whose memory comes in long pieces
         if (count <= GN_LANES_VECS * f.V) return f;
         f.kind = count <= GN_BLOCK_ALONE || (count <= GN_BLOCK_VALUES && (d.S == 1 || d.NB * d.G >= GN_BLOCK_FULL)) ? NORM_BLOCK : NORM_SPLIT;

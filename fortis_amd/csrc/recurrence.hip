@@ -10,13 +10,11 @@
 #include "common.h"
 
 #define RC_THREADS 256
-#define RC_AHEAD 8              // steps whose loads are in flight together
+#define RC_AHEAD 4              // steps whose loads are in flight together
 
-typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 template <int V> struct VecOf { typedef float T; };
 template <> struct VecOf<2> { typedef v2f T; };
-template <> struct VecOf<4> { typedef v4f T; };
 
 struct RecurArgs {
     RecurDesc d;
@@ -34,11 +32,12 @@ template <int V> __device__ __forceinline__ void load(float (&o)[V], const float
     const typename VecOf<V>::T t = *(const typename VecOf<V>::T*)p;
     __builtin_memcpy(o, &t, sizeof t);
 }
-template <int V> __device__ __forceinline__ void store(float* p, const float (&o)[V])
+template <int V, bool STREAM> __device__ __forceinline__ void store(float* p, const float (&o)[V])
 {
     typename VecOf<V>::T t;
     __builtin_memcpy(&t, o, sizeof t);
-    *(typename VecOf<V>::T*)p = t;
+    if constexpr (STREAM) __builtin_nontemporal_store(t, (typename VecOf<V>::T*)p);
+    else *(typename VecOf<V>::T*)p = t;
 }
 __device__ __forceinline__ long steps_of(const RecurArgs& a, long s)
 {
@@ -49,7 +48,7 @@ __device__ __forceinline__ long steps_of(const RecurArgs& a, long s)
 
 // One lane, V channels, the steps of one chunk.  APPLY: from the state in front, writing every step; otherwise the map of the
 // chunk's steps.
-template <int V, bool APPLY>
+template <int V, bool APPLY, bool STREAM>
 __global__ __launch_bounds__(RC_THREADS) void recurrence_walk_kernel(RecurArgs a)
 {
     const RecurDesc& d = a.d;
@@ -79,37 +78,52 @@ __global__ __launch_bounds__(RC_THREADS) void recurrence_walk_kernel(RecurArgs a
         const float* p = a.src + (row0 + t0 * rstep) * 2 * d.ch + c;
         float* q = a.dst + (row0 + t0 * rstep) * d.ch + c;
         const long ps = dir * 2 * d.ch, qs = dir * d.ch, n = i1 - i0;
-        float g[RC_AHEAD][V], x[RC_AHEAD][V];
-        for (long i = 0; i < n; i += RC_AHEAD, p += RC_AHEAD * ps, q += RC_AHEAD * qs) {
-            if (i + RC_AHEAD <= n) {
+        float g[2][RC_AHEAD][V], x[2][RC_AHEAD][V];
+        auto step = [&](int set, int u, float* at) __attribute__((always_inline)) {
 #pragma unroll
-                for (int u = 0; u < RC_AHEAD; u++) { load<V>(g[u], p + u * ps); load<V>(x[u], p + u * ps + d.ch); }
-            } else {
-                const long last = (n - 1 - i) * ps;              // places behind the last step read it again
-#pragma unroll
-                for (int u = 0; u < RC_AHEAD; u++) {
-                    const long o = i + u < n ? u * ps : last;
-                    load<V>(g[u], p + o);
-                    load<V>(x[u], p + o + d.ch);
-                }
+            for (int v = 0; v < V; v++) {
+                float hi, lo;
+                const float gv = g[set][u][v];
+                fortis_sigmoids(gv, hi, lo);
+                const float f = gv >= 0.f ? hi : lo, b = (gv >= 0.f ? lo : hi) * x[set][u][v];
+                h[v] = fmaf(f, h[v], b);
+                if (!APPLY) F[v] *= f;
             }
+            if (APPLY) store<V, STREAM>(at, h);
+        };
+        // Two register sets: a batch's loads are issued before the batch in front of it is worked on.  No branch goes round a load
+        // in this loop (the last round reads its own first batch again): one would make every wait a wait for all loads in flight.
+        auto fetch = [&](int set, const float* at) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < RC_AHEAD; u++) {
-                if (i + u >= n) break;
+            for (int u = 0; u < RC_AHEAD; u++) { load<V>(g[set][u], at + u * ps); load<V>(x[set][u], at + u * ps + d.ch); }
+        };
+        const long rounds = n / (2 * RC_AHEAD);
+        if (rounds > 0) fetch(0, p);
+        for (long r = 0; r < rounds; r++) {
+            fetch(1, p + RC_AHEAD * ps);
 #pragma unroll
-                for (int v = 0; v < V; v++) {
-                    float hi, lo;
-                    fortis_sigmoids(g[u][v], hi, lo);
-                    const float f = g[u][v] >= 0.f ? hi : lo, b = (g[u][v] >= 0.f ? lo : hi) * x[u][v];
-                    h[v] = fmaf(f, h[v], b);
-                    if (!APPLY) F[v] *= f;
-                }
-                if (APPLY) store<V>(q + u * qs, h);
-            }
+            for (int u = 0; u < RC_AHEAD; u++) step(0, u, q + u * qs);
+            const float* next = r + 1 < rounds ? p + 2 * RC_AHEAD * ps : p;
+            fetch(0, next);
+#pragma unroll
+            for (int u = 0; u < RC_AHEAD; u++) step(1, u, q + (RC_AHEAD + u) * qs);
+            p += 2 * RC_AHEAD * ps;
+            q += 2 * RC_AHEAD * qs;
         }
+        const int rest = (int)(n - rounds * 2 * RC_AHEAD);
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int u = 0; u < RC_AHEAD; u++)
+                if (k * RC_AHEAD + u < rest) { load<V>(g[k][u], p + (k * RC_AHEAD + u) * ps); load<V>(x[k][u], p + (k * RC_AHEAD + u) * ps + d.ch); }
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int u = 0; u < RC_AHEAD; u++)
+                if (k * RC_AHEAD + u < rest) step(k, u, q + (k * RC_AHEAD + u) * qs);
     }
     if (APPLY) {
-        if (a.chunks == 1 && a.h_out) store<V>(a.h_out + e, h);
+        if (a.chunks == 1 && a.h_out) store<V, false>(a.h_out + e, h);
     } else {
 #pragma unroll
         for (int v = 0; v < V; v++) a.maps[(e + v) * a.chunks + k] = make_float2(F[v], h[v]);
@@ -149,7 +163,9 @@ static RecurShape recur_shape(const RecurDesc& d)
 {
     RecurShape r;
     const long values = d.nseq * d.ch, full = 256 * 8 * 64;      // lanes that fill the chip: eight waves a compute unit
-    r.V = d.ch % 4 == 0 && values / 4 >= full / 2 ? 4 : d.ch % 2 == 0 && values / 2 >= full / 2 ? 2 : 1;
+    // One channel a lane until two leave four lanes in flight for every one that computes: 4736 x 64 values over 15 and 60 levels
+    // take 8.0 and 43.5 us with one, 9.4 and 45.7 with two.
+    r.V = d.ch % 2 == 0 && values / 2 >= 2 * full ? 2 : 1;
     r.chunks = 1;
     if (values / r.V < full / 2) r.chunks = cdiv(full, values / r.V);
     if (r.chunks > cdiv(d.len, 32)) r.chunks = cdiv(d.len, 32);
@@ -168,17 +184,18 @@ template <int V> static void launch_walks(const RecurArgs& a, hipStream_t s)
 {
     const dim3 grid((unsigned)cdiv(a.d.nseq * a.d.ch / V * a.chunks, RC_THREADS)), block(RC_THREADS);
     if (a.chunks > 1) {
-        hipLaunchKernelGGL((recurrence_walk_kernel<V, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((recurrence_walk_kernel<V, false, false>), grid, block, 0, s, a);
         hipLaunchKernelGGL(recurrence_scan_kernel, dim3((unsigned)cdiv(a.d.nseq * a.d.ch, RC_THREADS / 64)), block, 0, s, a);
     }
-    hipLaunchKernelGGL((recurrence_walk_kernel<V, true>), grid, block, 0, s, a);
+    // an output that the eight L2s (32 MB) cannot hold is written past them
+    if (a.d.nseq * a.d.len * a.d.ch * 4 > (32L << 20)) hipLaunchKernelGGL((recurrence_walk_kernel<V, true, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((recurrence_walk_kernel<V, true, false>), grid, block, 0, s, a);
 }
 void fortis_launch_recurrence(const RecurDesc& d, const float* src, float* dst, const float* h_in, float* h_out, const int* lengths, void* ws, hipStream_t s)
 {
     const RecurShape r = recur_shape(d);
     const RecurArgs a = { d, src, dst, h_in, h_out, lengths, (float2*)ws, r.chunks, r.per };
-    if (r.V == 4) launch_walks<4>(a, s);
-    else if (r.V == 2) launch_walks<2>(a, s);
+    if (r.V == 2) launch_walks<2>(a, s);
     else launch_walks<1>(a, s);
     HIP_OK(hipGetLastError());
 }
