@@ -91,27 +91,68 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_low_rows_kernel(AdaptDesc d,
 // 16 rows x 16 columns of Y; wave w takes the 16-wide k groups w, w + 8, ...  A lane reads four consecutive k of a row of X
 // and of W as one 16-byte load each and feeds four matrix instructions: instruction c multiplies k = 16 g + 4 q + c for lane
 // quarter q on both sides.
+// What the outputs' adapters add is formed while those loads travel.  FUSED (a few products at most, FEW_FUSED): every
+// workgroup forms H of its rows itself, one product a wave at a time, and the launch in front is not needed.
 #define FEW_WAVES 8
-template <int ROW>
+#define FEW_FUSED 32            // rows x ranks
+template <int ROW, bool FUSED>
 __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
                                                                    const float* __restrict__ H, float* __restrict__ Y, long B)
 {
     __shared__ float part[FEW_WAVES][16][17];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
-    const long tn = (d.N + 15) / 16, m0 = blockIdx.x / tn * 16, n0 = blockIdx.x % tn * 16;
+    __shared__ __attribute__((aligned(16))) float sH[FUSED ? FEW_FUSED : 4];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, lr = lane & 15, lq = lane >> 4;
+    const unsigned tn = (unsigned)(d.N + 15) / 16;
+    const long m0 = (long)(blockIdx.x / tn) * 16, n0 = (long)(blockIdx.x % tn) * 16;
+    // this thread's output (the first 256 threads)
+    const long m = m0 + t / 16, n = n0 + t % 16;
+    const bool out = t < 256 && m < B && n < d.N;
+    int i = out ? index[m] : -1;
+    const float bias = out && d.bias ? d.bias[n] : 0.f;
     const float* x = X + (m0 + lr < B ? m0 + lr : B - 1) * d.K;
     const float* w = d.W + (n0 + lr < d.N ? n0 + lr : d.N - 1) * d.p.ldw;
-    v4f acc = (v4f)(0.f);
-    const long groups = d.p.Ka / 16;
+    const int groups = (int)d.p.Ka / 16, Rp = (int)d.p.Rp;
     constexpr int AHEAD = 6;
-    for (long g = wave; g < groups; g += FEW_WAVES * AHEAD) {
-        v4f xv[AHEAD], wv[AHEAD];
+    v4f xv[AHEAD], wv[AHEAD];
+    auto fetch = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
-            const long k = (g + u * FEW_WAVES) * 16 + 4 * lq;
+            const int k = (g + u * FEW_WAVES) * 16 + 4 * lq;
             xv[u] = load_row4<ROW>(x, k, d.K);
             wv[u] = load_row4<ROW4>(w, k, d.p.ldw);
         }
+    };
+    fetch(wave);
+    if constexpr (FUSED) {
+        for (int e = wave; e < (int)B * Rp; e += FEW_WAVES) {
+            const int r = e / Rp, j = e - r * Rp, a = index[r];
+            float s = 0.f;
+            if (a >= 0 && a < d.nadapt && j < d.rank) {
+                const float *xr = X + r * d.K, *ar = d.A + ((long)a * d.p.R16 + j) * d.p.Ka;
+                for (int k = lane * 4; k < (int)d.p.Ka; k += 256) {
+                    const v4f p = load_row4<ROW>(xr, k, d.K), q = *(const v4f*)(ar + k);
+                    s = fmaf(p[3], q[3], fmaf(p[2], q[2], fmaf(p[1], q[1], fmaf(p[0], q[0], s))));
+                }
+                s *= d.scale[a];
+#pragma unroll
+                for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+            }
+            if (lane == 0) sH[e] = s;
+        }
+    }
+    if (i >= d.nadapt) i = -1;
+    const float* u = d.U + ((long)(i < 0 ? 0 : i) * d.N + n) * Rp;
+    float low = 0.f;
+    if (!FUSED && i >= 0) {
+        const float* h = H + m * Rp;
+        for (int j = 0; j < Rp; j += 4) {
+            const v4f hv = *(const v4f*)(h + j), uv = *(const v4f*)(u + j);
+            low = fmaf(hv[3], uv[3], fmaf(hv[2], uv[2], fmaf(hv[1], uv[1], fmaf(hv[0], uv[0], low))));
+        }
+    }
+    v4f acc = (v4f)(0.f);
+    for (int g = wave; g < groups; g += FEW_WAVES * AHEAD) {
+        if (g > wave) fetch(g);
 #pragma unroll
         for (int u = 0; u < AHEAD; u++)
 #pragma unroll
@@ -120,22 +161,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
 #pragma unroll
     for (int r = 0; r < 4; r++) part[wave][4 * lq + r][lr] = acc[r];
     __syncthreads();
-    const int t = threadIdx.x;
-    if (t >= 256) return;
-    const long m = m0 + t / 16, n = n0 + t % 16;
-    if (m >= B || n >= d.N) return;
+    if (!out) return;
     float v = 0.f;
 #pragma unroll
     for (int k = 0; k < FEW_WAVES; k++) v += part[k][t / 16][t % 16];
-    const int i = index[m];
-    if (i >= 0 && i < d.nadapt) {
-        const float *h = H + m * d.p.Rp, *u = d.U + ((long)i * d.N + n) * d.p.Rp;
-        for (long j = 0; j < d.p.Rp; j += 4) {
+    if (FUSED && i >= 0) {
+        const float* h = sH + m * Rp;
+        for (int j = 0; j < Rp; j += 4) {
             const v4f hv = *(const v4f*)(h + j), uv = *(const v4f*)(u + j);
-            v = fmaf(hv[3], uv[3], fmaf(hv[2], uv[2], fmaf(hv[1], uv[1], fmaf(hv[0], uv[0], v))));
+            low = fmaf(hv[3], uv[3], fmaf(hv[2], uv[2], fmaf(hv[1], uv[1], fmaf(hv[0], uv[0], low))));
         }
     }
-    Y[m * d.N + n] = fortis_act_any(v + (d.bias ? d.bias[n] : 0.f), d.act, d.alpha);
+    Y[m * d.N + n] = fortis_act_any(v + low + bias, d.act, d.alpha);
 }
 
 // ---- narrow layers -----------------------------------------------------------------------------------------------
@@ -574,8 +611,13 @@ template <int ROW>
 static void launch_few(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {
     float* H = (float*)ws;
+    const dim3 grid((unsigned)(cdiv(B, 16) * cdiv(d.N, 16))), block(64 * FEW_WAVES);
+    if (B * d.p.Rp <= FEW_FUSED) {
+        hipLaunchKernelGGL((adapt_few_kernel<ROW, true>), grid, block, 0, s, d, X, index, (const float*)H, Y, B);
+        return;
+    }
     hipLaunchKernelGGL((adapt_low_rows_kernel<ROW>), dim3((unsigned)cdiv(B * (d.p.Rp / 4), AD_THREADS / 64)), dim3(AD_THREADS), 0, s, d, X, index, H, B);
-    hipLaunchKernelGGL((adapt_few_kernel<ROW>), dim3((unsigned)(cdiv(B, 16) * cdiv(d.N, 16))), dim3(64 * FEW_WAVES), 0, s, d, X, index, (const float*)H, Y, B);
+    hipLaunchKernelGGL((adapt_few_kernel<ROW, false>), grid, block, 0, s, d, X, index, (const float*)H, Y, B);
 }
 template <bool SC>
 static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
