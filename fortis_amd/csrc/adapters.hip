@@ -415,9 +415,21 @@ __global__ __launch_bounds__(64 * KS) void adapt_low_sorted_kernel(AdaptDesc d, 
         const long p = p0 + 16 * h + lr < B ? p0 + 16 * h + lr : B - 1;
         x[h] = X + (base + perm[p]) * d.K;
     }
-    const long groups = d.p.Ka / 16;
+    const int groups = (int)d.p.Ka / 16;
     constexpr int AHEAD = 6;
+    v4f xv[2][AHEAD];
+    auto fetch = [&](int g) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            const int k = (g + u * KS) * 16 + 4 * lq;
+            xv[0][u] = load_row4<SC ? ROWANY : ROW4>(x[0], k, d.K);
+            xv[1][u] = load_row4<SC ? ROWANY : ROW4>(x[1], k, d.K);
+        }
+    };
+    // rows that one set of loads holds whole are read once for all their adapters
+    const bool whole = groups <= KS * AHEAD;
     unsigned live = (unsigned)__ballot(kk >= 0);
+    if (whole && live) fetch(wave);
     while (live) {
         const int a = __builtin_amdgcn_readlane(kk, __builtin_ctz(live));
         const unsigned rows = (unsigned)__ballot(kk == a);
@@ -426,15 +438,11 @@ __global__ __launch_bounds__(64 * KS) void adapt_low_sorted_kernel(AdaptDesc d, 
         for (long j0 = 0; j0 < d.rank; j0 += 16) {
             const float* w = d.A + ((long)a * d.p.R16 + j0 + lr) * d.p.Ka;
             v4f acc[2] = { (v4f)(0.f), (v4f)(0.f) };
-            for (long g = wave; g < groups; g += KS * AHEAD) {
-                v4f xv[2][AHEAD], wv[AHEAD];
+            for (int g = wave; g < groups; g += KS * AHEAD) {
+                v4f wv[AHEAD];
 #pragma unroll
-                for (int u = 0; u < AHEAD; u++) {
-                    const long k = (g + u * KS) * 16 + 4 * lq;
-                    xv[0][u] = load_row4<SC ? ROWANY : ROW4>(x[0], k, d.K);
-                    xv[1][u] = load_row4<SC ? ROWANY : ROW4>(x[1], k, d.K);
-                    wv[u] = load_row4<ROW4>(w, k, d.p.Ka);
-                }
+                for (int u = 0; u < AHEAD; u++) wv[u] = load_row4<ROW4>(w, (g + u * KS) * 16 + 4 * lq, d.p.Ka);
+                if (!whole) fetch(g);
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++)
 #pragma unroll
