@@ -4,6 +4,7 @@
 // second call and replay afterwards, with an eager fallback.
 #include <atomic>
 #include <cmath>
+#include <new>
 #include <condition_variable>
 #include <mutex>
 #include <functional>
@@ -313,7 +314,7 @@ int fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma,
 {
     if (!p || p->finalized) return bad("plan is null or already finalized");
     const long need = bytes_of(NB, S, C);
-    if (need < 0 || G <= 0 || C % G || !(eps >= 0.f)) return bad("group_norm: bad shape, groups or eps");
+    if (need < 0 || C >= (1L << 20) || G <= 0 || C % G || !(eps >= 0.f)) return bad("group_norm: bad shape, groups or eps");
     if (act < 0 || act > FORTIS_ACT_SILU) return bad("group_norm: unknown activation");
     if (!tensor_ok(p, src, need) || !tensor_ok(p, dst, need) || overlap(p, src, dst)) return bad("group_norm: tensors too small or overlapping");
     Op o; o.kind = OP_NORM; o.src = src; o.dst = dst; o.B = NB; o.H = S; o.C = C; o.F = G; o.flag = channels_first ? 1 : 0;
@@ -337,12 +338,14 @@ int fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, con
         overlap(p, index, src))
         return bad("linear_adapters: tensors too small or overlapping");
     Op o; o.kind = OP_ADAPT; o.src = src; o.dst = dst; o.side = index; o.B = B; o.K = K; o.N = N; o.F = nadapt; o.D = rank; o.act = act; o.alpha = alpha;
-    o.w.assign(W, W + N * K);
-    if (bias) { o.b.assign(bias, bias + N); o.has_bias = true; }
-    o.v0.assign(A, A + nadapt * rank * K);
-    o.v1.assign(U, U + nadapt * N * rank);
-    if (scale) o.v2.assign(scale, scale + nadapt); else o.v2.assign(nadapt, 1.f);
-    p->ops.push_back(std::move(o));
+    try {
+        o.w.assign(W, W + N * K);
+        if (bias) { o.b.assign(bias, bias + N); o.has_bias = true; }
+        o.v0.assign(A, A + nadapt * rank * K);
+        o.v1.assign(U, U + nadapt * N * rank);
+        if (scale) o.v2.assign(scale, scale + nadapt); else o.v2.assign(nadapt, 1.f);
+        p->ops.push_back(std::move(o));
+    } catch (const std::bad_alloc&) { return bad("linear_adapters: out of host memory"); }
     return 0;
 }
 int fortis_plan_recurrence(fortis_plan* p, int src, int dst, int h_in, int h_out, int lengths, long nseq, long len, long ch,
@@ -369,8 +372,10 @@ int fortis_plan_recurrence(fortis_plan* p, int src, int dst, int h_in, int h_out
 // ---- finalize: fusion + uploads -----------------------------------------------------------------
 static int uses_of(const fortis_plan* p, int t)
 {
-    int n = (t == p->out_t) ? 1 : 0;
-    for (const Op& o : p->ops) n += (o.src == t) + (o.res == t) + (o.side == t) + (o.h_in == t);
+    // (a window of t, or the tensor that t is a window of, counts: its reader reads t)
+    auto is = [&](int r) { return r >= 0 && overlap(p, r, t) ? 1 : 0; };
+    int n = is(p->out_t);
+    for (const Op& o : p->ops) n += is(o.src) + is(o.res) + is(o.side) + is(o.h_in);
     return n;
 }
 
@@ -687,7 +692,8 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
                     ops[i + 1].src == o.dst && ops[i + 1].KD == 3 && ops[i + 1].pad == 1 && ops[i + 1].F >= 16 && out_t != o.dst) {
                     bool other = false;
                     for (size_t j = 0; j < ops.size(); j++)
-                        if (j != i + 1 && (ops[j].src == o.dst || ops[j].res == o.dst || ops[j].side == o.dst || ops[j].h_in == o.dst)) other = true;
+                        if (j != i + 1)
+                            for (int r : { ops[j].src, ops[j].res, ops[j].side, ops[j].h_in }) other = other || (r >= 0 && overlap(p, r, o.dst));
                     if (ops[i + 1].res == o.dst) other = true;
                     if (!other) { fuse_ups_src = o.src; p->exec_skip++; i += 1; continue; }
                 }
@@ -704,18 +710,20 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
                 break;
             case OP_ADAPT: {
                 ex.kind = EX_ADAPT; ex.side = o.side; ex.rows = ex.rows_cap = o.B;
-                bool finite = true;
-                for (float u : o.v1) finite = finite && std::isfinite(u);
-                const AdaptPitch pitch = fortis_adapters_pitch(o.K, o.N, o.D, finite);
-                ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, pitch, nullptr, nullptr, nullptr, nullptr, nullptr };
-                ex.adapt.W = upload_padded(p, o.w, 1, o.N, o.K, o.N, pitch.ldw);
-                ex.adapt.bias = o.has_bias ? (const float*)upload(p, o.b.data(), o.b.size() * 4) : nullptr;
-                ex.adapt.A = upload_padded(p, o.v0, o.F, o.D, o.K, pitch.R16, pitch.Ka);
-                std::vector<float> U((size_t)(o.F * o.N * pitch.Rp), 0.f);
-                for (long r = 0; r < o.F * o.N; r++)
-                    for (long j = 0; j < o.D; j++) U[(size_t)(r * pitch.Rp + fortis_adapters_place(pitch, j))] = o.v1[(size_t)(r * o.D + j)];
-                ex.adapt.U = (const float*)upload(p, U.data(), U.size() * 4);
-                ex.adapt.scale = (const float*)upload(p, o.v2.data(), o.v2.size() * 4);
+                try {
+                    bool finite = true;
+                    for (float u : o.v1) finite = finite && std::isfinite(u);
+                    const AdaptPitch pitch = fortis_adapters_pitch(o.K, o.N, o.D, finite);
+                    ex.adapt = { o.K, o.N, o.F, o.D, o.act, o.alpha, pitch, nullptr, nullptr, nullptr, nullptr, nullptr };
+                    ex.adapt.W = upload_padded(p, o.w, 1, o.N, o.K, o.N, pitch.ldw);
+                    ex.adapt.bias = o.has_bias ? (const float*)upload(p, o.b.data(), o.b.size() * 4) : nullptr;
+                    ex.adapt.A = upload_padded(p, o.v0, o.F, o.D, o.K, pitch.R16, pitch.Ka);
+                    std::vector<float> U((size_t)(o.F * o.N * pitch.Rp), 0.f);
+                    for (long r = 0; r < o.F * o.N; r++)
+                        for (long j = 0; j < o.D; j++) U[(size_t)(r * pitch.Rp + fortis_adapters_place(pitch, j))] = o.v1[(size_t)(r * o.D + j)];
+                    ex.adapt.U = (const float*)upload(p, U.data(), U.size() * 4);
+                    ex.adapt.scale = (const float*)upload(p, o.v2.data(), o.v2.size() * 4);
+                } catch (const std::bad_alloc&) { p->upload_failed = true; fprintf(stderr, "fortis_plan: out of host memory for padded weights\n"); }
                 break;
             }
             case OP_RECUR:

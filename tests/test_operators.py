@@ -38,6 +38,18 @@ def test_group_norm_refusals(plan, capfd):
     plan.group_norm(**ok)                                      # and the call they all vary is accepted
 
 
+def test_sizes_the_kernels_do_not_address_are_refused(plan):
+    x, y = plan.tensor(1 << 20), plan.tensor(1 << 20)
+    with pytest.raises(ValueError):
+        plan.group_norm(x, y, 1, 1, 1 << 20, 1)                # channels
+    plan.group_norm(x, y, 1, 1, (1 << 20) - 1, 1)
+    i, one = plan.tensor(4), plan.tensor(4)
+    with pytest.raises(ValueError):
+        plan.linear_adapters(x, one, i, _f(1, 1 << 19), None, _f(1, 1, 1 << 19), _f(1, 1, 1), 1)
+    with pytest.raises(ValueError):
+        plan.linear_adapters(one, x, i, _f(1 << 19, 1), None, _f(1, 1, 1), _f(1, 1 << 19, 1), 1)
+
+
 def test_overlapping_windows_are_refused(plan):
     base = plan.tensor(400)
     a, b, c = plan.view(base, 0, 120), plan.view(base, 116, 120), plan.view(base, 240, 120)
