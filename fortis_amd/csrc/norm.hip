@@ -50,6 +50,19 @@ template <int L> __device__ __forceinline__ float sum_lanes(float v)
     return v;
 }
 
+// The values of an instance held in registers, less their mean, in two steps.  The first mean is summed about a pivot, the instance's
+// first value, which may lie far outside (sqrt(n) spreads): it is off by some u |pivot - mean|.  It is subtracted as a pair
+// (hi, lo), and what the differences still sum to corrects it.
+struct Centre { float hi, lo; };
+__device__ __forceinline__ Centre centre(float pivot, float mean)       // pivot + mean to twice float32's digits
+{
+    Centre c;
+    c.hi = pivot + mean;
+    const float b = c.hi - pivot;
+    c.lo = (pivot - (c.hi - b)) + (mean - b);
+    return c;
+}
+
 struct NormArgs {
     NormDesc d;
     const float* x;
@@ -96,14 +109,20 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
 #pragma unroll
         for (int k = 0; k < E; k++)
 #pragma unroll
-            for (int c = 0; c < V; c++) { v[k].v[c] -= pivot; s += have[k] ? v[k].v[c] : 0.f; }
-        const float mean = sum_lanes<L>(s) * inv;
+            for (int c = 0; c < V; c++) s += have[k] ? v[k].v[c] - pivot : 0.f;
+        const Centre mid = centre(pivot, sum_lanes<L>(s) * inv);
+        float s2 = 0.f;
         s = 0.f;
 #pragma unroll
         for (int k = 0; k < E; k++)
 #pragma unroll
-            for (int c = 0; c < V; c++) { v[k].v[c] -= mean; const float t = have[k] ? v[k].v[c] : 0.f; s = fmaf(t, t, s); }
-        const float rstd = 1.f / sqrtf(sum_lanes<L>(s) * inv + d.eps);
+            for (int c = 0; c < V; c++) {
+                v[k].v[c] = (v[k].v[c] - mid.hi) - mid.lo;
+                const float t = have[k] ? v[k].v[c] : 0.f;
+                s += t;
+                s2 = fmaf(t, t, s2);
+            }
+        const float off = sum_lanes<L>(s) * inv, rstd = 1.f / sqrtf(fmaf(-off, off, sum_lanes<L>(s2) * inv) + d.eps);
         fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
@@ -120,7 +139,7 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
                 if (d.beta) be = ld<V>(d.beta + ch[k]);
             }
 #pragma unroll
-            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, ga.v[c], be.v[c]), decltype(act)::value, d.alpha);
+            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf((v[k].v[c] - off) * rstd, ga.v[c], be.v[c]), decltype(act)::value, d.alpha);
             st<V>(a.y + at[k], o);
         }
         });
@@ -128,15 +147,15 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
 }
 
 // ---- block form --------------------------------------------------------------------------------------------------
-// Sum of one float per thread over the workgroup's T threads, the same order in every call; red: T / 64 floats.
-template <int T> __device__ __forceinline__ float sum_block(float v, float* red)
+// Sums of two floats per thread over the workgroup's T threads, the same order in every call; red: T / 64 pairs.
+template <int T> __device__ __forceinline__ float2 sum_block(float v, float w, float2* red)
 {
-    v = sum_lanes<64>(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    v = sum_lanes<64>(v); w = sum_lanes<64>(w);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = make_float2(v, w);
     __syncthreads();
-    float s = 0.f;
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < T / 64; w++) s += red[w];
+    for (int k = 0; k < T / 64; k++) { s.x += red[k].x; s.y += red[k].y; }
     __syncthreads();
     return s;
 }
@@ -144,7 +163,7 @@ template <int T> __device__ __forceinline__ float sum_block(float v, float* red)
 template <int V, int T, int E>
 __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
 {
-    __shared__ float red[T / 64];
+    __shared__ float2 red[T / 64];
     const NormDesc& d = a.d;
     const unsigned nv = (unsigned)(a.count / V);
     for (long inst = blockIdx.x; inst < total; inst += gridDim.x) {
@@ -174,14 +193,21 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
 #pragma unroll
         for (int k = 0; k < E; k++)
 #pragma unroll
-            for (int c = 0; c < V; c++) { v[k].v[c] -= pivot; s += threadIdx.x + k * T < nv ? v[k].v[c] : 0.f; }
-        const float mean = sum_block<T>(s, red) * inv;
+            for (int c = 0; c < V; c++) s += threadIdx.x + k * T < nv ? v[k].v[c] - pivot : 0.f;
+        const Centre mid = centre(pivot, sum_block<T>(s, 0.f, red).x * inv);
+        float s2 = 0.f;
         s = 0.f;
 #pragma unroll
         for (int k = 0; k < E; k++)
 #pragma unroll
-            for (int c = 0; c < V; c++) { v[k].v[c] -= mean; const float t = threadIdx.x + k * T < nv ? v[k].v[c] : 0.f; s = fmaf(t, t, s); }
-        const float rstd = 1.f / sqrtf(sum_block<T>(s, red) * inv + d.eps);
+            for (int c = 0; c < V; c++) {
+                v[k].v[c] = (v[k].v[c] - mid.hi) - mid.lo;
+                const float t = threadIdx.x + k * T < nv ? v[k].v[c] : 0.f;
+                s += t;
+                s2 = fmaf(t, t, s2);
+            }
+        const float2 sums = sum_block<T>(s, s2, red);
+        const float off = sums.x * inv, rstd = 1.f / sqrtf(fmaf(-off, off, sums.y * inv) + d.eps);
         fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
@@ -194,7 +220,7 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
 #pragma unroll
             for (int c = 0; c < V; c++) {
                 const unsigned i = ch + (d.first ? 0 : c);
-                o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, d.gamma ? d.gamma[i] : 1.f, d.beta ? d.beta[i] : 0.f), decltype(act)::value, d.alpha);
+                o.v[c] = fortis_act_any(fmaf((v[k].v[c] - off) * rstd, d.gamma ? d.gamma[i] : 1.f, d.beta ? d.beta[i] : 0.f), decltype(act)::value, d.alpha);
             }
             st<V>(y + at, o);
         }
@@ -205,7 +231,7 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
 template <int V, int T, int E>
 __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs, FastDiv slices, long total)
 {
-    __shared__ float part[T], sums[T];
+    __shared__ float2 part[T], sums[T];
     const NormDesc& d = a.d;
     const int tid = threadIdx.x;
     for (long item = blockIdx.x; item < total; item += gridDim.x) {
@@ -222,17 +248,18 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
             if (on && row + k * rows < d.S) v[k] = ld<V>(a.x + base + (long)(row + k * rows) * d.C);
         const float pivot = a.x[n * d.S * d.C + (g0 + gl) * a.cg], inv = 1.f / (float)a.count;
         // the group's sum: its threads are (row, columns gl cgv .. + cgv); one wave adds each group's partial sums
-        auto group_sum = [&](float s) __attribute__((always_inline)) {
-            part[tid] = on ? s : 0.f;
+        auto group_sum = [&](float s, float s2) __attribute__((always_inline)) {
+            part[tid] = on ? make_float2(s, s2) : make_float2(0.f, 0.f);
             __syncthreads();
             for (int g = tid >> 6; g < ng; g += T / 64) {
-                float t = 0.f;
+                float t = 0.f, t2 = 0.f;
                 for (unsigned i = tid & 63; i < (unsigned)(rows * cgv); i += 64) {
                     const unsigned r = i / (unsigned)cgv;
-                    t += part[r * wv + g * cgv + i - r * cgv];
+                    const float2 q = part[r * wv + g * cgv + i - r * cgv];
+                    t += q.x; t2 += q.y;
                 }
-                t = sum_lanes<64>(t);
-                if ((tid & 63) == 0) sums[g] = t;
+                t = sum_lanes<64>(t); t2 = sum_lanes<64>(t2);
+                if ((tid & 63) == 0) sums[g] = make_float2(t, t2);
             }
             __syncthreads();
             return sums[gl];
@@ -241,14 +268,21 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
 #pragma unroll
         for (int k = 0; k < E; k++)
 #pragma unroll
-            for (int c = 0; c < V; c++) { v[k].v[c] -= pivot; s += on && row + k * rows < d.S ? v[k].v[c] : 0.f; }
-        const float mean = group_sum(s) * inv;
+            for (int c = 0; c < V; c++) s += on && row + k * rows < d.S ? v[k].v[c] - pivot : 0.f;
+        const Centre mid = centre(pivot, group_sum(s, 0.f).x * inv);
+        float s2 = 0.f;
         s = 0.f;
 #pragma unroll
         for (int k = 0; k < E; k++)
 #pragma unroll
-            for (int c = 0; c < V; c++) { v[k].v[c] -= mean; const float t = on && row + k * rows < d.S ? v[k].v[c] : 0.f; s = fmaf(t, t, s); }
-        const float rstd = 1.f / sqrtf(group_sum(s) * inv + d.eps);
+            for (int c = 0; c < V; c++) {
+                v[k].v[c] = (v[k].v[c] - mid.hi) - mid.lo;
+                const float t = on && row + k * rows < d.S ? v[k].v[c] : 0.f;
+                s += t;
+                s2 = fmaf(t, t, s2);
+            }
+        const float2 both = group_sum(s, s2);
+        const float off = both.x * inv, rstd = 1.f / sqrtf(fmaf(-off, off, both.y * inv) + d.eps);
         if (!on) continue;
         Vals<V> ga, be;
 #pragma unroll
@@ -259,7 +293,7 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
             if (row + k * rows >= d.S) continue;
             Vals<V> o;
 #pragma unroll
-            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf(v[k].v[c] * rstd, ga.v[c], be.v[c]), decltype(act)::value, d.alpha);
+            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf((v[k].v[c] - off) * rstd, ga.v[c], be.v[c]), decltype(act)::value, d.alpha);
             st<V>(a.y + base + (long)(row + k * rows) * d.C, o);
         }
         });
@@ -268,6 +302,7 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
 
 // ---- split form --------------------------------------------------------------------------------------------------
 #define GS_THREADS 1024
+#define GS_FOLD 16             // batches of loads between two moves of a thread's float32 sums into its float64 ones
 #define GS_AHEAD 4             // loads a thread has in flight
 struct SplitShape {
     long chunks, per;        // chunks of a sample (an instance with channels first), positions (vectors) a chunk
@@ -300,15 +335,15 @@ template <int V> __device__ __forceinline__ SplitPlace split_place(const NormArg
 }
 
 // Partial sums of `n` values about P: a1 = sum(v - P), a2 = sum((v - P)^2), from sums about a pivot of the thread's own.
-__device__ __forceinline__ void about(float pivot, int n, float s1, float s2, double P, double& a1, double& a2)
+__device__ __forceinline__ void about(float pivot, long n, double s1, double s2, double P, double& a1, double& a2)
 {
     const double dn = (double)n;
     a1 = a2 = 0.0;
     if (n == 0) return;
     // centred, s2 - s1^2 / n, and moved to P, + t1^2 / n, where t1 - s1 = n (pivot - P): no division
     const double d = (double)pivot - P;
-    a1 = dn * d + (double)s1;
-    a2 = (double)s2 + d * ((double)s1 + a1);
+    a1 = dn * d + s1;
+    a2 = s2 + d * (s1 + a1);
 }
 __device__ __forceinline__ double sum_wave(double v)
 {
@@ -317,8 +352,9 @@ __device__ __forceinline__ double sum_wave(double v)
     return v;
 }
 
-// Channels last.  The slice's columns (V channels each) by rows of the chunk; a thread keeps its column.
-template <int V>
+// Channels last.  The slice's columns (V channels each) by rows of the chunk; a thread keeps its column.  ONE: a column's V
+// channels lie in one group (they do unless the slice is all channels and V does not divide cg) and are summed together.
+template <int V, bool ONE>
 __global__ __launch_bounds__(GS_THREADS) void norm_sums_kernel(NormArgs a, SplitShape h, double2* __restrict__ out)
 {
     __shared__ double2 part[GS_THREADS];
@@ -327,35 +363,40 @@ __global__ __launch_bounds__(GS_THREADS) void norm_sums_kernel(NormArgs a, Split
     const SplitPlace w = split_place<V>(a, h);
     const long r0 = (long)w.chunk * h.per, r1 = r0 + h.per < d.S ? r0 + h.per : d.S;
     const float* xs = a.x + w.n * d.S * d.C;
-    // a column's V channels lie in one group unless the slice is all channels and V does not divide cg
-    const bool one = a.cg % V == 0;
-    int g[V];
-    float P[V];                                 // the groups' first values: what the sums are joined about
+    constexpr int D = ONE ? 1 : V;              // sums a thread keeps
+    float P[D];                                 // the groups' first values: what the sums are joined about
 #pragma unroll
-    for (int c = 0; c < V; c++) {
-        g[c] = h.blocks > 1 ? w.g0 : (int)fortis_div((unsigned)(w.c_lo + w.col * V + c), h.by_cg);
-        P[c] = xs[g[c] * a.cg];
+    for (int c = 0; c < D; c++) {
+        const int g = h.blocks > 1 ? w.g0 : (int)fortis_div((unsigned)(w.c_lo + w.col * V + c), h.by_cg);
+        P[c] = xs[g * a.cg];
     }
-    float p[V], s1[V], s2[V];
-    int cnt = 0;
+    float p[D], s1[V], s2[V];
+    double d1[D], d2[D];
+    long cnt = 0;
 #pragma unroll
-    for (int c = 0; c < V; c++) p[c] = s1[c] = s2[c] = 0.f;
+    for (int c = 0; c < V; c++) s1[c] = s2[c] = 0.f;
+#pragma unroll
+    for (int c = 0; c < D; c++) { p[c] = 0.f; d1[c] = d2[c] = 0; }
     auto take = [&](const Vals<V>& v) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < V; c++) { const float t = v.v[c] - p[c]; s1[c] += t; s2[c] = fmaf(t, t, s2[c]); }
+        for (int c = 0; c < V; c++) { const float t = v.v[c] - p[ONE ? 0 : c]; s1[c] += t; s2[c] = fmaf(t, t, s2[c]); }
+    };
+    auto fold = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < V; c++) { d1[ONE ? 0 : c] += (double)s1[c]; d2[ONE ? 0 : c] += (double)s2[c]; s1[c] = s2[c] = 0.f; }
     };
     // whole passes of the workgroup over `rows` positions: uniform base + a 32-bit offset of the thread's own
     const unsigned off = ((unsigned)w.row * (unsigned)d.C + (unsigned)w.col * V) * 4u;
     const char* base = (const char*)(xs + w.c_lo + r0 * d.C);
     const long pass = (long)w.rows * d.C * 4;
-    int left = (int)(r1 - r0);
+    long left = r1 - r0;
     if (w.row < w.rows) {
         if (w.row < left) {
             const Vals<V> f = ld<V>((const float*)(base + off));
 #pragma unroll
-            for (int c = 0; c < V; c++) p[c] = f.v[one ? 0 : c];
+            for (int c = 0; c < D; c++) p[c] = f.v[c];
         }
-        while (left >= GS_AHEAD * w.rows) {
+        for (int batch = 1; left >= GS_AHEAD * w.rows; batch++) {
             Vals<V> v[GS_AHEAD];
 #pragma unroll
             for (int k = 0; k < GS_AHEAD; k++) v[k] = ld<V>((const float*)(base + k * pass + off));
@@ -364,6 +405,7 @@ __global__ __launch_bounds__(GS_THREADS) void norm_sums_kernel(NormArgs a, Split
             cnt += GS_AHEAD;
             base += GS_AHEAD * pass;
             left -= GS_AHEAD * w.rows;
+            if (batch % GS_FOLD == 0) fold();
         }
         Vals<V> v[GS_AHEAD];
 #pragma unroll
@@ -372,27 +414,20 @@ __global__ __launch_bounds__(GS_THREADS) void norm_sums_kernel(NormArgs a, Split
 #pragma unroll
         for (int k = 0; k < GS_AHEAD; k++)
             if (w.row + k * w.rows < left) { take(v[k]); cnt++; }
+        fold();
     }
-    for (int c = 0; c < (one ? 1 : V); c++) {
+    for (int c = 0; c < D; c++) {
+        // component c of every column; the groups then take the components one after the other
         double a1 = 0, a2 = 0;
-        if (one) {
 #pragma unroll
-            for (int k = 1; k < V; k++) { s1[0] += s1[k]; s2[0] += s2[k]; }
-            about(p[0], V * cnt, s1[0], s2[0], (double)P[0], a1, a2);
-        } else {
-            // component c of every column; the groups then take the components one after the other
-            float pc = 0, s1c = 0, s2c = 0, Pc = 0;
-#pragma unroll
-            for (int k = 0; k < V; k++) if (k == c) { pc = p[k]; s1c = s1[k]; s2c = s2[k]; Pc = P[k]; }
-            about(pc, cnt, s1c, s2c, (double)Pc, a1, a2);
-        }
+        for (int k = 0; k < D; k++) if (k == c) about(p[k], ONE ? V * cnt : cnt, d1[k], d2[k], (double)P[k], a1, a2);
         __syncthreads();
         part[tid] = make_double2(a1, a2);
         __syncthreads();
         for (int q = tid >> 6; q < w.ng; q += GS_THREADS / 64) {
-            // columns that hold a channel of group g0 + q in component c (any component when V divides cg)
+            // columns that hold a channel of group g0 + q in component c (ONE: in any)
             const int lo = h.blocks > 1 ? 0 : (int)(q * a.cg), hi = h.blocks > 1 ? w.wv * V : lo + (int)a.cg;
-            const int k0 = one ? lo / V : (lo - c + V - 1 + V) / V - 1, k1 = one ? hi / V : (hi - c + V - 1 + V) / V - 1;
+            const int k0 = ONE ? lo / V : (lo - c + V - 1 + V) / V - 1, k1 = ONE ? hi / V : (hi - c + V - 1 + V) / V - 1;
             double t1 = 0, t2 = 0;
             const int width = k1 - k0;
             for (int i = tid & 63; i < w.rows * width; i += 64) {
@@ -420,12 +455,14 @@ __global__ __launch_bounds__(GS_THREADS) void norm_sums_first_kernel(NormArgs a,
     const long nv = a.count / V, e0 = chunk * h.per, e1 = e0 + h.per < nv ? e0 + h.per : nv;
     const float P = x[0];
     float p = 0.f, s1 = 0.f, s2 = 0.f;
-    int cnt = 0;
+    double d1 = 0, d2 = 0;
+    long cnt = 0;
     auto take = [&](const Vals<V>& v) __attribute__((always_inline)) {
 #pragma unroll
         for (int c = 0; c < V; c++) { const float t = v.v[c] - p; s1 += t; s2 = fmaf(t, t, s2); }
         cnt += V;
     };
+    auto fold = [&]() __attribute__((always_inline)) { d1 += (double)s1; d2 += (double)s2; s1 = s2 = 0.f; };
     const float* base = x + e0 * V;
     long left = e1 - e0;
     if (tid < left) p = base[tid * V];
@@ -435,6 +472,7 @@ __global__ __launch_bounds__(GS_THREADS) void norm_sums_first_kernel(NormArgs a,
         for (int k = 0; k < GS_AHEAD; k++) v[k] = ld<V>(base + (k * GS_THREADS + tid) * V);
 #pragma unroll
         for (int k = 0; k < GS_AHEAD; k++) take(v[k]);
+        if (cnt % 64 == 0) fold();
     }
     {
         Vals<V> v[GS_AHEAD];
@@ -444,9 +482,10 @@ __global__ __launch_bounds__(GS_THREADS) void norm_sums_first_kernel(NormArgs a,
 #pragma unroll
         for (int k = 0; k < GS_AHEAD; k++)
             if (k * GS_THREADS + tid < left) take(v[k]);
+        fold();
     }
     double a1, a2;
-    about(p, cnt, s1, s2, (double)P, a1, a2);
+    about(p, cnt, d1, d2, (double)P, a1, a2);
     a1 = sum_wave(a1); a2 = sum_wave(a2);
     if ((tid & 63) == 0) part[tid >> 6] = make_double2(a1, a2);
     __syncthreads();
@@ -721,7 +760,8 @@ template <int V> static void launch_split(const NormArgs& a, const SplitShape& h
         return;
     }
     const dim3 grid((unsigned)(d.NB * h.slices * h.blocks * h.chunks));
-    hipLaunchKernelGGL((norm_sums_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, part);
+    if (a.cg % V == 0) hipLaunchKernelGGL((norm_sums_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, part);
+    else if constexpr (V > 1) hipLaunchKernelGGL((norm_sums_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, part);
     if (stream) hipLaunchKernelGGL((norm_apply_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
     else hipLaunchKernelGGL((norm_apply_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
 }

@@ -98,6 +98,27 @@ def test_group_norm_of_constant_groups_and_of_one_value(L, gpu):
     assert bits_equal(y, np.broadcast_to(beta, y.shape))
 
 
+@pytest.mark.parametrize("first", [False, True])
+def test_group_norm_of_a_large_array_sums_no_worse(L, gpu, first):
+    """32 million values in four groups: a thread's float32 sums are moved on before they grow, so the bound is that of small ones."""
+    rng = np.random.default_rng(12)
+    x = rng.standard_normal((1, 8, 4000000) if first else (1, 4000000, 8), dtype=np.float32)
+    x += np.float32(3)
+    within(run_norm(x, 4, first=first), *R.group_norm(x, 4, None, None, 1e-5, None, 0, first))
+
+
+def test_a_fill_value_in_front_of_a_group(L, gpu):
+    """The first value of every sample is far outside (a land cell's -9999): it is the pivot of the sums and costs no digits."""
+    rng = np.random.default_rng(13)
+    for shape in ((2, 500, 16), (1, 70000, 16)):
+        x = rng.standard_normal(shape).astype(np.float32)
+        x[:, 0] = -9999.0
+        y, e = R.group_norm(x, 2, None, None, 1e-5, None, 0, False)
+        got = run_norm(x, 2)
+        # of the values other than the outlier only the spread among them is at stake: 1e-4 of the sample's spread
+        assert np.abs(got[:, 1:] - y[:, 1:]).max() < 2e-6 and np.abs(got[:, 0] / y[:, 0] - 1).max() < 1e-5
+
+
 def test_group_norm_is_the_same_from_pass_to_pass(L, gpu):
     x = np.random.default_rng(2).standard_normal((1, 50000, 32)).astype(np.float32)
     assert bits_equal(run_norm(x, 8), run_norm(x, 8, fill=np.nan))
@@ -139,7 +160,9 @@ class Adapted:
 ADAPT_SHAPES = [(1, 1, 1, 1, 1), (1, 768, 768, 64, 8), (1, 27, 64, 3, 4), (2, 64, 3, 2, 1), (3, 556, 368, 7, 12), (5, 9, 700, 40, 31), (16, 768, 100, 64, 16),
                 (17, 100, 100, 5, 3), (33, 768, 768, 64, 16), (48, 555, 129, 11, 5), (64, 64, 64, 1, 64), (127, 130, 66, 200, 2), (200, 256, 256, 9, 33),
                 (513, 96, 48, 4, 8), (1000, 27, 64, 15, 4), (1500, 556, 368, 7, 12), (3000, 61, 148, 1000, 6), (4099, 128, 132, 24, 16),
-                (700, 300, 33, 3, 256), (2500, 5, 2, 4, 3), (40, 1000, 1, 6, 7), (9000, 64, 256, 4096, 4), (300, 37, 501, 2, 100)]
+                (700, 300, 33, 3, 256), (2500, 5, 2, 4, 3), (40, 1000, 1, 6, 7), (9000, 64, 256, 4096, 4), (300, 37, 501, 2, 100),
+                (9, 3, 700, 4, 3), (3000, 2, 200, 5, 70), (1300, 133, 200, 6, 9), (1100, 131, 129, 40, 17), (1, 5, 300, 2, 32), (4, 770, 9, 3, 8),
+                (35000, 20, 30, 9, 5), (33000, 62, 61, 3, 20), (32768, 16, 64, 4, 64), (1024, 129, 20, 3, 4), (1025, 129, 20, 3, 4), (2049, 1100, 65, 5, 40)]
 
 
 @pytest.mark.parametrize("B,K,N,nadapt,rank", ADAPT_SHAPES)
@@ -506,3 +529,101 @@ def test_two_plans_interleaved_share_nothing(L, gpu):
         y = pl.read(blk.y, blk.shapes[1])
         assert np.abs(y[valid] - ry[valid]).max() < BLOCK_TOL * np.abs(ry[valid]).max()
         pl.close()
+
+
+def test_a_window_of_a_tensor_that_would_be_folded_away(L, gpu):
+    """linear -> scale fold into one kernel that does not store the tensor between them, unless a window of it is read too."""
+    rng = np.random.default_rng(1)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    X, W, v = f(64, 16), f(300, 16), f(300)
+    p = P.Plan()
+    t, h, s, z, o = p.tensor(64 * 16), p.tensor(64 * 300), p.tensor(64 * 300), p.tensor(32 * 300), p.tensor(32 * 300)
+    low = p.view(h, 32 * 300, 32 * 300)
+    p.linear(t, h, W, None, 64)
+    p.scale(h, s, v, 64, divide=False)
+    p.group_norm(low, z, 32, 1, 300, 3)
+    p.concat_copy(z, o, 32, 300, 0, 32)
+    p.finalize(t, o)
+    y = p.forward(X, (32, 300))
+    r = (X.astype(np.float64) @ W.T)[32:]
+    ref, bound = R.group_norm(r[:, None], 3, None, None, 1e-5, None, 0, False)
+    assert np.abs(y - ref[:, 0]).max() < 1e-5                  # 16-term sums, 16 u of their terms, and the norm's own bound
+    p.close()
+
+
+# ---- offsets beyond 32 bits: the same block again and again, results have to repeat to the bit -----------------
+def _repeat(L, ptr, block_bytes, copies):
+    done = 1
+    while done < copies:
+        n = min(done, copies - done)
+        L.fortis_d2d(ptr + done * block_bytes, ptr, n * block_bytes)
+        done += n
+
+
+def _block(L, ptr, shape):
+    out = np.empty(shape, np.float32)
+    L.fortis_d2h(_vp(out), ptr, out.nbytes)
+    return out
+
+
+@pytest.mark.parametrize("K,N,block,copies", [(27, 3, 1 << 16, 640), (556, 40, 1 << 13, 260)])
+def test_adapters_beyond_four_gigabytes(L, gpu, K, N, block, copies):
+    a = Adapted(block, K, N, 5, 4)
+    B = block * copies
+    assert B * K * 4 > 1 << 32
+    p = P.Plan()
+    t, i, o = p.tensor(B * K), p.tensor(B), p.tensor(B * N)
+    p.linear_adapters(t, o, i, a.W, a.bias, a.A, a.U, B, a.scale, "relu")
+    p.finalize(t, o)
+    p.write(t, a.X)
+    p.write(i, a.index)
+    _repeat(L, p.ptr(t), block * K * 4, copies)
+    _repeat(L, p.ptr(i), block * 4, copies)
+    p.run()
+    first, last = _block(L, p.ptr(o), (block, N)), _block(L, p.ptr(o) + (copies - 1) * block * N * 4, (block, N))
+    a.act = "relu"
+    within(first, *a.ref())
+    assert bits_equal(last, first)
+    p.close()
+    L.fortis_pool_trim()
+
+
+@pytest.mark.parametrize("NB,S,Cc,G,first", [(1 << 14, 1, 80, 4, False), (6, 20000, 64, 8, False), (6, 20000, 64, 8, True), (512, 64, 32, 2, False)])
+def test_group_norm_beyond_four_gigabytes(L, gpu, NB, S, Cc, G, first):
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((NB, Cc, S) if first else (NB, S, Cc)).astype(np.float32)
+    copies = (5 << 30) // x.nbytes
+    p = P.Plan()
+    t, o = p.tensor(x.size * copies), p.tensor(x.size * copies)
+    p.group_norm(t, o, NB * copies, S, Cc, G, channels_first=first, act="silu")
+    p.finalize(t, o)
+    p.write(t, x)
+    _repeat(L, p.ptr(t), x.nbytes, copies)
+    p.run()
+    a, b = _block(L, p.ptr(o), x.shape), _block(L, p.ptr(o) + (copies - 1) * x.nbytes, x.shape)
+    within(a, *R.group_norm(x, G, None, None, 1e-5, "silu", 0, first))
+    assert bits_equal(a, b)
+    p.close()
+    L.fortis_pool_trim()
+
+
+@pytest.mark.parametrize("q,n,c", [(64, 100, 40), (2, 3000, 8)])
+def test_recurrence_beyond_four_gigabytes(L, gpu, q, n, c):
+    """Sequence-major: a block of sequences again and again."""
+    rng = np.random.default_rng(4)
+    src = rng.standard_normal((q * n, 2 * c)).astype(np.float32)
+    copies = (5 << 30) // src.nbytes
+    p = P.Plan()
+    t, o, h = p.tensor(src.size * copies), p.tensor(q * n * c * copies), p.tensor(q * c * copies)
+    p.recurrence(t, o, q * copies, n, c, h_out=h, time_major=False)
+    p.finalize(t, o)
+    p.write(t, src)
+    _repeat(L, p.ptr(t), src.nbytes, copies)
+    p.run()
+    a, b = _block(L, p.ptr(o), (q * n, c)), _block(L, p.ptr(o) + (copies - 1) * q * n * c * 4, (q * n, c))
+    ry, rh, ey, eh = R.recurrence(src, None, None, q, n, c, False, False, np.zeros((q * n, c)))
+    within(a, ry, ey)
+    assert bits_equal(a, b)
+    assert bits_equal(_block(L, p.ptr(h) + (copies - 1) * q * c * 4, (q, c)), _block(L, p.ptr(h), (q, c)))
+    p.close()
+    L.fortis_pool_trim()
