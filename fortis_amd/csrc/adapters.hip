@@ -6,7 +6,7 @@
 // low-rank rows H[r] = s_i X[r] A_i^T with a wave per row and four ranks, a second the outputs: a workgroup owns 16 rows
 // by 16 columns and its eight waves divide K, so that all of a wave's loads are in flight at once.
 //
-// Narrow layers (K and N up to 128): bound by reading X and writing Y.  One launch does it all: W lies in LDS, a wave
+// Narrow layers (K and N up to 64, ranks up to 16): bound by reading X and writing Y.  One launch does it all: W lies in LDS, a wave
 // takes 16 rows at a time from X to Y.
 //
 // Many rows: bound by the matrix pipes.  Rows are sorted by adapter inside windows of AD_WINDOW rows (one launch), H is
@@ -19,15 +19,20 @@
 
 #define AD_THREADS 256
 #define AD_WINDOW 2048          // rows sorted together; a multiple of the tile's 128
+// Few rows against sorted ones, us at K = N = 768, rank 16: 513 rows with 64 adapters 29 against 62, with 4 adapters 28 against 39;
+// 1024 rows with 64 adapters 49 against 52, with 8 adapters 47 against 41; 2048 rows with 24 adapters 90 against 55.
 #define AD_FEW_ROWS 1024
 
 static inline long up(long n, long m) { return (n + m - 1) / m * m; }
 
 // ---- weights, laid out once --------------------------------------------------------------------------------------
 // W [N][ldw], A [nadapt][R16][Ka], U [nadapt][N][Rp], padded with zeros.
-#define NARROW_K 128
-#define NARROW_N 128
-#define NARROW_RANK 64
+// Where one launch pays, us for the narrow form / the others: 24576 rows of 64 -> 64, rank 8 with 8 adapters in any order 18 / 31 (sorted
+// rows), 27 -> 64 13 / 32, but 128 -> 128 41 / 37 and 128 -> 128 with rank 64 and 24 adapters 207 / 84 (every adapter among 16 rows is a
+// product of its own); 500 rows of 128 -> 128 24 / 9 (few rows).
+#define NARROW_K 64
+#define NARROW_N 64
+#define NARROW_RANK 16
 AdaptPitch fortis_adapters_pitch(long K, long N, long rank, bool finite)
 {
     // (an adapter with an infinity or a NaN in U would reach other rows through 0 times U in all forms but the few-rows one)
@@ -36,7 +41,9 @@ AdaptPitch fortis_adapters_pitch(long K, long N, long rank, bool finite)
 }
 // Where rank j of a row of U lies: in order, but 4 x 4 transposed within sixteen for the narrow form, whose instruction c then
 // multiplies ranks 4 c .. 4 c + 3 and which leaves out the instructions behind the last rank.
-long fortis_adapters_place(const AdaptPitch& p, long j) { return p.narrow ? j / 16 * 16 + j % 4 * 4 + j % 16 / 4 : j; }
+// (H of the few-rows form lies alike.)
+__host__ __device__ __forceinline__ static int adapt_place(int narrow, int j) { return narrow ? j / 16 * 16 + j % 4 * 4 + j % 16 / 4 : j; }
+long fortis_adapters_place(const AdaptPitch& p, long j) { return adapt_place(p.narrow, (int)j); }
 
 // Elements k .. k + 3 of a row of K floats at p; what lies at or beyond K is 0.  How rows lie: ROW4 K is a multiple of 4; ROWANY
 // rows start at any float and K is at least 4: the 16 bytes are loaded where they are; ROWTINY K < 4.
@@ -84,7 +91,7 @@ __global__ __launch_bounds__(AD_THREADS) void adapt_low_rows_kernel(AdaptDesc d,
         for (int o = 32; o >= 1; o >>= 1) s[j] += __shfl_xor(s[j], o, 64);
     if (lane < 4) {
         const float v = lane == 0 ? s[0] : lane == 1 ? s[1] : lane == 2 ? s[2] : s[3];
-        H[r * d.p.Rp + 4 * q + lane] = 4 * q + lane < d.rank ? v * d.scale[i] : 0.f;
+        H[r * d.p.Rp + adapt_place(d.p.narrow, (int)(4 * q) + lane)] = 4 * q + lane < d.rank ? v * d.scale[i] : 0.f;
     }
 }
 
@@ -137,7 +144,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
 #pragma unroll
                 for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
             }
-            if (lane == 0) sH[e] = s;
+            if (lane == 0) sH[r * Rp + adapt_place(d.p.narrow, j)] = s;
         }
     }
     if (i >= d.nadapt) i = -1;
@@ -176,25 +183,25 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
 }
 
 // ---- narrow layers -----------------------------------------------------------------------------------------------
-// A wave owns RT times 16 rows: their X as KG operands of four k (k = 16 g + 4 q + c, as above).  Per adapter among the rows: all
-// are multiplied with its A, 16 ranks at a time, the products change places through the wave's own piece of LDS into
+// A wave owns 16 rows: their X as KG operands of four k (k = 16 g + 4 q + c, as above).  Per adapter among the rows: all
+// are multiplied with its A, the products change places through the wave's own piece of LDS into
 // operands of the second product, where those of other adapters' rows are zeros.  Loads of X start before W is brought to LDS.
-#define NARROW_WAVE_FLOATS(KG, RT, SC) (16 * (RT) * 20 + ((SC) ? 16 * (RT) * (16 * (KG) + 4) : 0))
-template <int KG, int NT, int RT, bool SC>
-__global__ __launch_bounds__(AD_THREADS, KG * RT <= 4 && NT <= 4 ? 3 : 2) void adapt_narrow_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
+#define NARROW_WAVE_FLOATS(KG, SC) (16 * 20 + ((SC) ? 16 * (16 * (KG) + 4) : 0))
+template <int KG, int NT, bool SC>
+__global__ __launch_bounds__(AD_THREADS, 3) void adapt_narrow_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
                                                                   float* __restrict__ Y, long B, FastDiv byK)
 {
     extern __shared__ float4 smem4[];
-    constexpr int LDW = 16 * KG + 4, ROWS = 16 * RT;
+    constexpr int LDW = 16 * KG + 4, ROWS = 16;
     float* sW = (float*)smem4;                                                                 // [16 NT][LDW]
-    float* sH = sW + 16 * NT * LDW + (threadIdx.x >> 6) * NARROW_WAVE_FLOATS(KG, RT, SC);      // [ROWS][20] for this wave
+    float* sH = sW + 16 * NT * LDW + (threadIdx.x >> 6) * NARROW_WAVE_FLOATS(KG, SC);      // [ROWS][20] for this wave
     float* sX = sH + ROWS * 20;                                                                // SC: [ROWS][LDW], zeros behind K
     const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4;
     const int K = (int)d.K, N = (int)d.N;
     const long step = (long)gridDim.x * (AD_THREADS / 64) * ROWS;
     long m0 = ((long)blockIdx.x * (AD_THREADS / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * ROWS;
-    v4f xv[RT][KG];
-    int i = -1;                                                                                // adapter of row lane % ROWS
+    v4f xv[KG];
+    int i = -1;                                                                                // adapter of row lane % 16
     auto fetch = [&](long m) __attribute__((always_inline)) {
         const int n = B - m < ROWS ? (int)(B - m) : ROWS, row = lane & (ROWS - 1);
         i = row < n ? index[m + row] : -1;
@@ -202,15 +209,13 @@ __global__ __launch_bounds__(AD_THREADS, KG * RT <= 4 && NT <= 4 ? 3 : 2) void a
         if constexpr (SC) {
             // the rows' floats in the order of memory, whatever K is
 #pragma unroll
-            for (int u = 0; u < 4 * KG * RT; u++) {
+            for (int u = 0; u < 4 * KG; u++) {
                 const int e = lane + 64 * u;
-                xv[u / (4 * KG)][u / 4 % KG][u % 4] = p[e < n * K ? e : n * K - 1];
+                xv[u / 4][u % 4] = p[e < n * K ? e : n * K - 1];
             }
         } else {
 #pragma unroll
-            for (int h = 0; h < RT; h++)
-#pragma unroll
-                for (int g = 0; g < KG; g++) xv[h][g] = load_row4<ROW4>(p + (16 * h + lr < n ? 16 * h + lr : n - 1) * K, 16 * g + 4 * lq, K);
+            for (int g = 0; g < KG; g++) xv[g] = load_row4<ROW4>(p + (lr < n ? lr : n - 1) * K, 16 * g + 4 * lq, K);
         }
     };
     if (m0 < B) fetch(m0);
@@ -235,76 +240,59 @@ __global__ __launch_bounds__(AD_THREADS, KG * RT <= 4 && NT <= 4 ? 3 : 2) void a
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
     while (m0 < B) {
-        v4f acc[RT][NT];
+        v4f acc[NT];
         if (i >= d.nadapt) i = -1;
         unsigned live = (unsigned)__ballot(i >= 0) & (unsigned)((1ull << ROWS) - 1);
         if constexpr (SC) {
 #pragma unroll
-            for (int u = 0; u < 4 * KG * RT; u++) {
+            for (int u = 0; u < 4 * KG; u++) {
                 const unsigned e = lane + 64 * u, r = fortis_div(e, byK);
-                if (e < (unsigned)(ROWS * K)) sX[r * LDW + e - r * K] = xv[u / (4 * KG)][u / 4 % KG][u % 4];
+                if (e < (unsigned)(ROWS * K)) sX[r * LDW + e - r * K] = xv[u / 4][u % 4];
             }
             turn();
 #pragma unroll
-            for (int h = 0; h < RT; h++)
-#pragma unroll
-                for (int g = 0; g < KG; g++) xv[h][g] = *(const v4f*)(sX + (16 * h + lr) * LDW + 16 * g + 4 * lq);
+            for (int g = 0; g < KG; g++) xv[g] = *(const v4f*)(sX + lr * LDW + 16 * g + 4 * lq);
             __builtin_amdgcn_wave_barrier();
         }
 #pragma unroll
-        for (int h = 0; h < RT; h++)
-#pragma unroll
-            for (int t = 0; t < NT; t++) acc[h][t] = (v4f)(0.f);
+        for (int t = 0; t < NT; t++) acc[t] = (v4f)(0.f);
 #pragma unroll
         for (int g = 0; g < KG; g++)
 #pragma unroll
             for (int t = 0; t < NT; t++) {
                 const v4f w = *(const v4f*)(sW + (16 * t + lr) * LDW + 16 * g + 4 * lq);
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-#pragma unroll
-                    for (int h = 0; h < RT; h++) acc[h][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[h][g][c], w[c], acc[h][t], 0, 0, 0);
+                for (int c = 0; c < 4; c++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[g][c], w[c], acc[t], 0, 0, 0);
             }
         while (live) {
             const int a = __builtin_amdgcn_readlane(i, __builtin_ctz(live));
             const unsigned rows = (unsigned)__ballot(i == a) & (unsigned)((1ull << ROWS) - 1);
             live &= ~rows;
             const float sc = d.scale[a];
-            for (int j0 = 0; j0 < d.rank; j0 += 16) {
-                const float* A = d.A + ((long)a * d.p.R16 + j0) * d.p.Ka;                       // uniform
-                const float* U = d.U + (long)a * N * d.p.Rp + j0;
-                v4f h[RT], av[KG], uv[NT];
+            const int rank = (int)d.rank;
+            const float* A = d.A + (long)a * d.p.R16 * d.p.Ka;                                  // uniform
+            const float* U = d.U + (long)a * N * d.p.Rp;
+            v4f h = (v4f)(0.f), av[KG], uv[NT];
 #pragma unroll
-                for (int g = 0; g < KG; g++) av[g] = 16 * g < d.p.Ka ? *(const v4f*)(A + lr * (int)d.p.Ka + 4 * lq + 16 * g) : (v4f)(0.f);
+            for (int g = 0; g < KG; g++) av[g] = 16 * g < d.p.Ka ? *(const v4f*)(A + lr * (int)d.p.Ka + 4 * lq + 16 * g) : (v4f)(0.f);
 #pragma unroll
-                for (int t = 0; t < NT; t++) uv[t] = *(const v4f*)(U + ucol[t]);
+            for (int t = 0; t < NT; t++) uv[t] = *(const v4f*)(U + ucol[t]);
 #pragma unroll
-                for (int q = 0; q < RT; q++) h[q] = (v4f)(0.f);
+            for (int g = 0; g < KG; g++)
 #pragma unroll
-                for (int g = 0; g < KG; g++)
+                for (int c = 0; c < 4; c++) h = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[g][c], av[g][c], h, 0, 0, 0);
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
+            for (int r = 0; r < 4; r++) sH[(4 * lq + r) * 20 + lr] = h[r] * sc;
+            turn();
 #pragma unroll
-                        for (int q = 0; q < RT; q++) h[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[q][g][c], av[g][c], h[q], 0, 0, 0);
+            for (int c = 0; c < 4; c++) {
+                if (4 * c >= rank) break;
+                const float hv = sH[lr * 20 + 4 * c + lq];
+                const float hc = (rows >> lr) & 1 && 4 * c + lq < rank ? hv : 0.f;
 #pragma unroll
-                for (int q = 0; q < RT; q++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) sH[(16 * q + 4 * lq + r) * 20 + lr] = h[q][r] * sc;
-                turn();
-                const int left = (int)d.rank - j0;
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    if (4 * c >= left) break;
-#pragma unroll
-                    for (int q = 0; q < RT; q++) {
-                        const float hv = sH[(16 * q + lr) * 20 + 4 * c + lq];
-                        const float hc = (rows >> (16 * q + lr)) & 1 && 4 * c + lq < left ? hv : 0.f;
-#pragma unroll
-                        for (int t = 0; t < NT; t++) acc[q][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(hc, uv[t][c], acc[q][t], 0, 0, 0);
-                    }
-                }
-                __builtin_amdgcn_wave_barrier();
+                for (int t = 0; t < NT; t++) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(hc, uv[t][c], acc[t], 0, 0, 0);
             }
+            __builtin_amdgcn_wave_barrier();
         }
         float* y = Y + m0 * N;                                                                 // uniform
         const int n = B - m0 < ROWS ? (int)(B - m0) : ROWS;
@@ -313,45 +301,32 @@ __global__ __launch_bounds__(AD_THREADS, KG * RT <= 4 && NT <= 4 ? 3 : 2) void a
         const float alpha = d.alpha;
         fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
-            for (int h = 0; h < RT; h++)
+            for (int r = 0; r < 4; r++) {
+                const int m = 4 * lq + r;
+                if (m >= n) continue;
+                float* row = y + m * N + lr;
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int m = 16 * h + 4 * lq + r;
-                    if (m >= n) continue;
-                    float* row = y + m * N + lr;
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-                        if (16 * t + lr < N) row[16 * t] = fortis_act_any(acc[h][t][r] + bv[t], decltype(act)::value, alpha);
-                }
+                for (int t = 0; t < NT; t++)
+                    if (16 * t + lr < N) row[16 * t] = fortis_act_any(acc[t][r] + bv[t], decltype(act)::value, alpha);
+            }
         });
     }
 }
-template <int KG, int NT, int RT, bool SC>
+template <int KG, int NT, bool SC>
 static void launch_narrow(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, hipStream_t s)
 {
-    const size_t shmem = (size_t)(16 * NT * (16 * KG + 4) + (AD_THREADS / 64) * NARROW_WAVE_FLOATS(KG, RT, SC)) * 4;
+    const size_t shmem = (size_t)(16 * NT * (16 * KG + 4) + (AD_THREADS / 64) * NARROW_WAVE_FLOATS(KG, SC)) * 4;
     static bool set = false;
-    if (!set) { HIP_OK(hipFuncSetAttribute((const void*)adapt_narrow_kernel<KG, NT, RT, SC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem)); set = true; }
-    const long wgs = cdiv(B, 16 * RT * (AD_THREADS / 64));
-    hipLaunchKernelGGL((adapt_narrow_kernel<KG, NT, RT, SC>), dim3((unsigned)(wgs < 1024 ? wgs : 1024)), dim3(AD_THREADS), shmem, s, d, X, index, Y, B, fortis_fast_div((unsigned)d.K));
+    if (!set) { HIP_OK(hipFuncSetAttribute((const void*)adapt_narrow_kernel<KG, NT, SC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shmem)); set = true; }
+    const long wgs = cdiv(B, 16 * (AD_THREADS / 64));
+    hipLaunchKernelGGL((adapt_narrow_kernel<KG, NT, SC>), dim3((unsigned)(wgs < 2048 ? wgs : 2048)), dim3(AD_THREADS), shmem, s, d, X, index, Y, B, fortis_fast_div((unsigned)d.K));
 }
 template <int KG, bool SC>
 static void narrow_by_columns(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, hipStream_t s)
 {
-    // 32 rows a wave where that still gives every SIMD a wave
-    const bool two = B >= 32 * 1024;
-    if constexpr (KG <= 4) {
-        if (two && d.N <= 64) {
-            if (d.N <= 16) launch_narrow<KG, 1, 2, SC>(d, X, index, Y, B, s);
-            else if (d.N <= 32) launch_narrow<KG, 2, 2, SC>(d, X, index, Y, B, s);
-            else launch_narrow<KG, 4, 2, SC>(d, X, index, Y, B, s);
-            return;
-        }
-    }
-    if (d.N <= 16) launch_narrow<KG, 1, 1, SC>(d, X, index, Y, B, s);
-    else if (d.N <= 32) launch_narrow<KG, 2, 1, SC>(d, X, index, Y, B, s);
-    else if (d.N <= 64) launch_narrow<KG, 4, 1, SC>(d, X, index, Y, B, s);
-    else launch_narrow<KG, 8, 1, SC>(d, X, index, Y, B, s);
+    if (d.N <= 16) launch_narrow<KG, 1, SC>(d, X, index, Y, B, s);
+    else if (d.N <= 32) launch_narrow<KG, 2, SC>(d, X, index, Y, B, s);
+    else launch_narrow<KG, 4, SC>(d, X, index, Y, B, s);
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------------------
@@ -630,11 +605,10 @@ static void launch_few(const AdaptDesc& d, const float* X, const int* index, flo
 template <bool SC>
 static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {
-    if (d.p.narrow) {
+    if (B > AD_FEW_ROWS && d.p.narrow) {
         if (d.K <= 16) narrow_by_columns<1, SC>(d, X, index, Y, B, s);
         else if (d.K <= 32) narrow_by_columns<2, SC>(d, X, index, Y, B, s);
-        else if (d.K <= 64) narrow_by_columns<4, SC>(d, X, index, Y, B, s);
-        else narrow_by_columns<8, SC>(d, X, index, Y, B, s);
+        else narrow_by_columns<4, SC>(d, X, index, Y, B, s);
         return;
     }
     if (d.K < 4) { launch_few<ROWTINY>(d, X, index, Y, B, ws, s); return; }

@@ -2,17 +2,20 @@
 //     y = act(gamma_c (x - mean_{n,g}) / sqrt(var_{n,g} + eps) + beta_c)
 // over the S * C / G values of every (sample, group) -- an "instance" below -- channels last or first.
 //
-// Memory-bound: 8 bytes and about ten operations a value.  Three forms by the size of an instance:
-//   lanes    up to 2048 values: 1 to 64 lanes hold the instance in registers, one read, one write, no barrier;
+// Memory-bound: 8 bytes and about ten operations a value.  Three forms:
+//   lanes    up to 2048 values an instance (512 vectors): 1 to 64 lanes hold it in registers, one read, one write, no barrier.
+//            71040 rows of 64 in heads of 16: 9.7 us, 3.8 TB/s (a copy of as many bytes 5.4 us);
 //   block    up to 32768: one workgroup holds an instance (or the neighbouring instances whose channels share 128-byte
-//            lines) in registers, one read, one write;
-//   split    beyond: one launch sums over chunks of every sample, a second joins a sample's chunk sums and normalises.  The
-//            input is read twice, the second time from the caches as far as they hold it.
-// Sums.  Where the values stay in registers the mean comes first and the squares of what is left after it second, about
-// the instance's first value as a pivot (a pivot inside the data is at most sqrt(n) spreads from the mean), in float32.  The
-// split form has to take both sums in one read: every thread sums a few dozen values about the first one it meets, and from
-// there on everything is joined in float64 about the instance's first value, where cancellation costs digits that are there
-// to spare.  The mean is then subtracted as a float32 pair.
+//            lines) in registers, one read, one write.  512 x 8 instances of 16384, channels first: 102 us, 5.2 TB/s;
+//   split    beyond, and where few workgroups would have much each (a compute unit alone moves some 25 GB/s: eight instances of
+//            32768 take 8.3 us in the block form, 7.6 in two launches): one launch sums over chunks of every sample, a second joins
+//            a sample's chunk sums and normalises.  The input is read twice, the second time from the caches as far as they
+//            hold it.  287496 x 64 in 8 groups: 37.5 us, 13 of them the sums (the first read runs at what HBM gives), the rest
+//            the second at 6 TB/s; 65536 x 32: 11.1 us, both launches bound by their start, two barriers and the join.
+// Sums.  Where the values stay in registers the mean comes first, summed about the instance's first value as a pivot, and the
+// squares of what is left after it second, in float32.  The split form has to take both sums in one read: every thread sums at
+// most 64 values about the first one it meets, and from there on everything is joined in float64 about the instance's first
+// value, where cancellation costs digits that are there to spare.  The mean is subtracted as a float32 pair.
 #include "common.h"
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -686,8 +689,8 @@ static NormForm norm_form(const NormDesc& d)
     }
     // Channels last and narrow groups: neighbouring groups share lines.  Instances of a few values are left to lanes all the
     // same (a sample's are next to each other in a wave); otherwise a workgroup takes the groups of one line, or more of them
-    // as long as there are workgroups enough: 512 samples of 128 x 256 in groups of 32 channels, a group each: 36 us, the
-    // whole sample: see the figures at the top.
+    // as long as there are workgroups enough: 512 samples of 128 x 256 in groups of 32 channels take 36.1 us with a group
+    // each and 33.6 with four.
     if (count <= 256) return f;
     auto fits = [&](long gs) { return gs * cg / f.V <= 1024 && d.S <= 1024 / (gs * cg / f.V) * 8; };
     f.gs = (int)cdiv(GN_LINE, cg);

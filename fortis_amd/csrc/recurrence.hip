@@ -2,11 +2,16 @@
 //     f = 1 / (1 + exp(-g_t)),  h_t = f h_(t-1) + (1 - f) x_t
 // per sequence and channel, rows of 2 * ch features (g first, x behind).
 //
-// Memory-bound: 12 bytes and about 25 instructions a value.  A lane owns V neighbouring channels of a sequence and walks
-// steps with the next loads in flight.  Where sequences and channels alone do not fill the chip, every sequence is cut into
-// K chunks: a step is the map h -> f h + b, maps compose to (F, B), so one launch composes every chunk's steps, one wave per
-// sequence and channel scans the K compositions and leaves the state in front of every chunk, and a third launch walks the
-// chunks from there.  All compositions happen in a fixed order: results repeat bit for bit.
+// Memory-bound: 12 bytes and about 25 instructions a value.  A lane owns one or two neighbouring channels of a sequence and
+// walks its steps with two batches of loads in flight.  4736 columns of up to 15 levels of 64 channels: 7.6 us, 3.9 TB/s; one step:
+// 3.3 us, the launch; 4736 x 60 x 64: 43.5 us, 5.0 TB/s.
+// Where sequences and channels alone do not fill the chip, every sequence is cut into K chunks: a step is the map
+// h -> f h + b, maps compose to (F, B), so one launch composes every chunk's steps, one wave per sequence and channel scans the
+// K compositions and leaves the state in front of every chunk, and a third launch walks the chunks from there: 8 bytes a value
+// more.  2 x 32768 steps of 384 channels: 90 us = 37 (201 MB at 5.4 TB/s) + 5 + 48 (302 MB at 6.3, the input partly from the
+// memory-side cache); in one read it could not be under 57 us at a copy's rate.  Chunks that wait for the ones in front of them
+// would read once, but a wait between workgroups has no place in a library that runs beside others.
+// All compositions happen in a fixed order: results repeat bit for bit.
 #include "common.h"
 
 #define RC_THREADS 256
@@ -162,9 +167,9 @@ struct RecurShape { int V; long chunks, per; };
 static RecurShape recur_shape(const RecurDesc& d)
 {
     RecurShape r;
-    const long values = d.nseq * d.ch, full = 256 * 8 * 64;      // lanes that fill the chip: eight waves a compute unit
-    // One channel a lane until two leave four lanes in flight for every one that computes: 4736 x 64 values over 15 and 60 levels
-    // take 8.0 and 43.5 us with one, 9.4 and 45.7 with two.
+    const long values = d.nseq * d.ch, full = 256 * 8 * 64;      // lanes that keep the memory busy: eight waves a compute unit (twelve and sixteen: no faster)
+    // One channel a lane until two still give every SIMD four waves: 4736 x 64 values over 15 and 60 levels take 8.0 and 43.5 us with
+    // one, 9.4 and 45.7 with two (four: 10.6 and 54).
     r.V = d.ch % 2 == 0 && values / 2 >= 2 * full ? 2 : 1;
     r.chunks = 1;
     if (values / r.V < full / 2) r.chunks = cdiv(full, values / r.V);
@@ -187,7 +192,7 @@ template <int V> static void launch_walks(const RecurArgs& a, hipStream_t s)
         hipLaunchKernelGGL((recurrence_walk_kernel<V, false, false>), grid, block, 0, s, a);
         hipLaunchKernelGGL(recurrence_scan_kernel, dim3((unsigned)cdiv(a.d.nseq * a.d.ch, RC_THREADS / 64)), block, 0, s, a);
     }
-    // an output that the eight L2s (32 MB) cannot hold is written past them
+    // an output that the eight L2s (32 MB) cannot hold is written past them: 106 -> 96 us for 2 x 32768 x 384
     if (a.d.nseq * a.d.len * a.d.ch * 4 > (32L << 20)) hipLaunchKernelGGL((recurrence_walk_kernel<V, true, true>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((recurrence_walk_kernel<V, true, false>), grid, block, 0, s, a);
 }
