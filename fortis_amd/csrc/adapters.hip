@@ -374,31 +374,28 @@ __global__ __launch_bounds__(1024) void adapt_sort_kernel(const int* __restrict_
     }
 }
 
-// H of 32 sorted rows: KS waves divide the 16-wide k groups, 16 ranks at a time; per adapter among the rows all 32 are
-// multiplied with its A and its own rows kept.
+// H of 16 sorted rows: KS waves divide the 16-wide k groups, 16 ranks at a time; per adapter among the rows all 16 are
+// multiplied with its A and its own rows kept.  Bound by reading X, and by how many loads a compute unit holds: 24576 rows of 768 with 24
+// adapters of rank 16 (75 MB) 24 us behind the sort, 3.1 TB/s; with 32 rows a workgroup 27, and
+// 4099 rows of 556 9 instead of 7.5 (but 8192 x 2048 -> 512 with rank 32, whose X is read once per 16 ranks, 207 us in all instead of 220).
+#define LOW_ROWS 16
 template <int KS, bool SC>
 __global__ __launch_bounds__(64 * KS) void adapt_low_sorted_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ perm,
                                                                       const int* __restrict__ key, float* __restrict__ H, long B)
 {
-    __shared__ float part[KS][32][17];
+    __shared__ float part[KS][LOW_ROWS][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
-    const long p0 = (long)blockIdx.x * 32, base = p0 / AD_WINDOW * AD_WINDOW;
-    const int kk = p0 + (lane & 31) < B ? key[p0 + (lane & 31)] : -1;
-    const float* x[2];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const long p = p0 + 16 * h + lr < B ? p0 + 16 * h + lr : B - 1;
-        x[h] = X + (base + perm[p]) * d.K;
-    }
+    const long p0 = (long)blockIdx.x * LOW_ROWS, base = p0 / AD_WINDOW * AD_WINDOW;
+    const int kk = lane < LOW_ROWS && p0 + lane < B ? key[p0 + lane] : -1;
+    const float* x = X + (base + perm[p0 + lr < B ? p0 + lr : B - 1]) * d.K;
     const int groups = (int)d.p.Ka / 16;
     constexpr int AHEAD = 6;
-    v4f xv[2][AHEAD];
+    v4f xv[AHEAD];
     auto fetch = [&](int g) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
             const int k = (g + u * KS) * 16 + 4 * lq;
-            xv[0][u] = load_row4<SC ? ROWANY : ROW4>(x[0], k, d.K);
-            xv[1][u] = load_row4<SC ? ROWANY : ROW4>(x[1], k, d.K);
+            xv[u] = load_row4<SC ? ROWANY : ROW4>(x, k, d.K);
         }
     };
     // rows that one set of loads holds whole are read once for all their adapters
@@ -412,7 +409,7 @@ __global__ __launch_bounds__(64 * KS) void adapt_low_sorted_kernel(AdaptDesc d, 
         const float sc = d.scale[a];
         for (long j0 = 0; j0 < d.rank; j0 += 16) {
             const float* w = d.A + ((long)a * d.p.R16 + j0 + lr) * d.p.Ka;
-            v4f acc[2] = { (v4f)(0.f), (v4f)(0.f) };
+            v4f acc = (v4f)(0.f);
             for (int g = wave; g < groups; g += KS * AHEAD) {
                 v4f wv[AHEAD];
 #pragma unroll
@@ -421,18 +418,13 @@ __global__ __launch_bounds__(64 * KS) void adapt_low_sorted_kernel(AdaptDesc d, 
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        acc[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[0][u][c], wv[u][c], acc[0], 0, 0, 0);
-                        acc[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[1][u][c], wv[u][c], acc[1], 0, 0, 0);
-                    }
+                    for (int c = 0; c < 4; c++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[u][c], wv[u][c], acc, 0, 0, 0);
             }
             __syncthreads();
 #pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) part[wave][16 * h + 4 * lq + r][lr] = acc[h][r];
+            for (int r = 0; r < 4; r++) part[wave][4 * lq + r][lr] = acc[r];
             __syncthreads();
-            for (int e = threadIdx.x; e < 512; e += 64 * KS) {
+            for (int e = threadIdx.x; e < 16 * LOW_ROWS; e += 64 * KS) {
                 const int m = e >> 4, j = e & 15;
                 if (!((rows >> m) & 1) || j0 + j >= d.p.Rp) continue;
                 float v = 0.f;
@@ -618,7 +610,7 @@ static void launch_adapters(const AdaptDesc& d, const float* X, const int* index
     float* H = (float*)(key + Bw);
     hipLaunchKernelGGL(adapt_sort_kernel, dim3((unsigned)(Bw / AD_WINDOW)), dim3(1024), (size_t)(d.nadapt + 1 + 16) * 4, s, index, perm, key, B, (int)d.nadapt);
     // as many waves as leave each the six groups that it loads at once
-    const dim3 blocks((unsigned)cdiv(B, 32));
+    const dim3 blocks((unsigned)cdiv(B, LOW_ROWS));
     if (d.p.Ka <= 12 * 16) hipLaunchKernelGGL((adapt_low_sorted_kernel<1, SC>), blocks, dim3(64), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
     else if (d.p.Ka <= 24 * 16) hipLaunchKernelGGL((adapt_low_sorted_kernel<2, SC>), blocks, dim3(128), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
     else hipLaunchKernelGGL((adapt_low_sorted_kernel<8, SC>), blocks, dim3(512), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
