@@ -100,15 +100,17 @@ int  fortis_plan_permute(fortis_plan* p, int src, int dst, long C, long S, int t
  * All of them work on float32 tensors in the row layout of the other calls and refuse (-1 and a message) tensors
  * that are too small or whose windows overlap.  Side tensors (index, lengths, states) are declared with
  * fortis_plan_tensor like any other; the caller fills them through fortis_plan_tensor_ptr (a host behind the bind(c)
- * entries: fortis_model_tensor) before a pass, and they keep their contents from pass to pass. */
+ * entries: fortis_model_tensor) before a pass, and they keep their contents from pass to pass.  A fortis_begin that grows
+ * the step moves every tensor: addresses are asked for again, an index starts over with -1, lengths with len, states with 0. */
 
 /* Group normalisation with an activation, NB samples of S positions and C channels, channels last ([NB][S][C]) or, with
  * channels_first, [NB][C][S]: for every sample and every group of C / G neighbouring channels
  *     dst = act(gamma[c] * (src - mean) / sqrt(var + eps) + beta[c])
  * over the group's S * C / G values, var their biased variance.  gamma, beta: host pointers of length C, copied, or NULL
- * (1 and 0).  G has to divide C; eps >= 0.  S = 1 normalises rows (one head of C / G features per group).  The mean is
- * kept to twice float32's digits and sums are joined in float64, so a large common offset costs no accuracy.  A NaN or
- * an infinity makes its own group NaN and no other. */
+ * (1 and 0).  G has to divide C, C < 2^20; eps >= 0 (with 0 a group of equal values is NaN).  S = 1 normalises rows (one
+ * head of C / G features per group).  The mean is kept to twice float32's digits and sums are joined in float64 where a group
+ * does not fit in registers, so a large common offset costs no accuracy.  A value further than about 1e19 from its group's
+ * mean (its square leaves float32), a NaN or an infinity spoils its own group (NaN in front of the activation) and no other. */
 int  fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma, const float* beta, float eps,
                             long NB, long S, long C, long G, int channels_first, int act, float alpha);
 /* fortis_plan_linear with a low-rank adapter chosen per row:
@@ -117,7 +119,8 @@ int  fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma
  * copied.  index: a tensor of B int32, read on the device at every pass, rows in any order; an index outside
  * [0, nadapt) means no adapter for that row, and so all rows start (index is filled with -1 at finalize).  1 <= nadapt
  * <= FORTIS_MAX_ADAPTERS, 1 <= rank <= FORTIS_MAX_RANK, B < 2^31, K and N < 2^19.  A row's result depends on that row alone: not on the
- * order of rows, nor on the adapters of the others. */
+ * order of rows, nor on the adapters of the others.  (Values of U that are not finite are kept to their own adapter's rows by a
+ * slower kernel.) */
 #define FORTIS_MAX_ADAPTERS 4096
 #define FORTIS_MAX_RANK 256
 int  fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, const float* W, const float* bias,
@@ -132,8 +135,10 @@ int  fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, co
  * receives the state behind the last one, -1: none.  h_in == h_out carries the state from pass to pass (len = 1 is one
  * step of a host that steps through time); a state that no operation of the plan writes first starts as zeros.
  * lengths: tensor of nseq int32, -1: all `len`; sequence s takes steps 0 .. lengths[s] - 1 only (values are clamped to
- * [0, len]; filled with len at finalize).  Rows of dst at and behind a sequence's length are left as they were, a
- * sequence without steps hands its state on unchanged. */
+ * [0, len]; filled with len at finalize).  Rows of dst at and behind a sequence's length are left as they were (a tensor
+ * between two operations shares its memory with others: what stands there is then whatever they left), a sequence without
+ * steps hands its state on unchanged.  Long sequences are cut into chunks whose maps are composed first: an infinite value
+ * in front of a chunk may come out as NaN behind it. */
 int  fortis_plan_recurrence(fortis_plan* p, int src, int dst, int h_in, int h_out, int lengths, long nseq, long len,
                             long ch, int time_major, int reverse);
 
