@@ -117,7 +117,7 @@ struct NormDesc {
     float eps;
     int act;
     float alpha;
-    const float *gamma, *beta;  // device, length C, or null
+    const float *gamma, *beta;  // device, length C
 };
 long fortis_norm_workspace(const NormDesc& d);          // bytes fortis_launch_group_norm needs at ws
 void fortis_launch_group_norm(const NormDesc& d, const float* x, float* y, void* ws, hipStream_t s);

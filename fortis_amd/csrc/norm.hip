@@ -4,14 +4,14 @@
 //
 // Memory-bound: 8 bytes and about ten operations a value.  Three forms:
 //   lanes    up to 2048 values an instance (512 vectors): 1 to 64 lanes hold it in registers, one read, one write, no barrier.
-//            71040 rows of 64 in heads of 16: 9.7 us, 3.8 TB/s (a copy of as many bytes 5.4 us);
+//            71040 rows of 64 in heads of 16: 9.1 us, 4.0 TB/s (a copy of as many bytes 5.4 us);
 //   block    up to 32768: one workgroup holds an instance (or the neighbouring instances whose channels share 128-byte
 //            lines) in registers, one read, one write.  512 x 8 instances of 16384, channels first: 102 us, 5.2 TB/s;
 //   split    beyond, and where few workgroups would have much each (a compute unit alone moves some 25 GB/s: eight instances of
 //            32768 take 8.3 us in the block form, 7.6 in two launches): one launch sums over chunks of every sample, a second joins
 //            a sample's chunk sums and normalises.  The input is read twice, the second time from the caches as far as they
-//            hold it.  287496 x 64 in 8 groups: 37.5 us, 13 of them the sums (the first read runs at what HBM gives), the rest
-//            the second at 6 TB/s; 65536 x 32: 11.1 us, both launches bound by their start, two barriers and the join.
+//            hold it.  287496 x 64 in 8 groups: 36.2 us, 13 of them the sums (the first read runs at what HBM gives), the rest
+//            the second at 6 TB/s; 65536 x 32: 10.8 us, both launches bound by their start, two barriers and the join.
 // Sums.  Where the values stay in registers the mean comes first, summed about the instance's first value as a pivot, and the
 // squares of what is left after it second, in float32.  The split form has to take both sums in one read: every thread sums at
 // most 64 values about the first one it meets, and from there on everything is joined in float64 about the instance's first
@@ -106,6 +106,19 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
             else { const unsigned c = (e - q * a.row.d) * V; at[k] = base + (long)q * d.C + c; ch[k] = (unsigned)(g * a.cg) + c; }
             if (have[k]) v[k] = ld<V>(a.x + at[k]);
         }
+        Vals<V> ga[E], be[E];
+        auto scales = [&](int k) __attribute__((always_inline)) {
+            if (d.first) {
+                const float gs = d.gamma[ch[k]], bs = d.beta[ch[k]];
+#pragma unroll
+                for (int c = 0; c < V; c++) { ga[k].v[c] = gs; be[k].v[c] = bs; }
+            } else { ga[k] = ld<V>(d.gamma + ch[k]); be[k] = ld<V>(d.beta + ch[k]); }
+        };
+        constexpr bool EARLY = E <= 2;      // few enough to travel beside the values: 9.7 -> 9.1 us for 71040 rows of 64
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int k = 0; k < E; k++) if (have[k]) scales(k);
+        }
         const float pivot = __shfl(v[0].v[0], lane & ~(L - 1), 64);
         const float inv = 1.f / (float)a.count;
         float s = 0.f;
@@ -130,19 +143,10 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(NormArgs a, long total)
 #pragma unroll
         for (int k = 0; k < E; k++) {
             if (!have[k]) continue;
-            Vals<V> ga, be, o;
-            if (d.first) {
-                const float gs = d.gamma ? d.gamma[ch[k]] : 1.f, bs = d.beta ? d.beta[ch[k]] : 0.f;
+            if constexpr (!EARLY) scales(k);
+            Vals<V> o;
 #pragma unroll
-                for (int c = 0; c < V; c++) { ga.v[c] = gs; be.v[c] = bs; }
-            } else {
-#pragma unroll
-                for (int c = 0; c < V; c++) { ga.v[c] = 1.f; be.v[c] = 0.f; }
-                if (d.gamma) ga = ld<V>(d.gamma + ch[k]);
-                if (d.beta) be = ld<V>(d.beta + ch[k]);
-            }
-#pragma unroll
-            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf((v[k].v[c] - off) * rstd, ga.v[c], be.v[c]), decltype(act)::value, d.alpha);
+            for (int c = 0; c < V; c++) o.v[c] = fortis_act_any(fmaf((v[k].v[c] - off) * rstd, ga[k].v[c], be[k].v[c]), decltype(act)::value, d.alpha);
             st<V>(a.y + at[k], o);
         }
         });
@@ -223,7 +227,7 @@ __global__ __launch_bounds__(T) void norm_block_kernel(NormArgs a, long total)
 #pragma unroll
             for (int c = 0; c < V; c++) {
                 const unsigned i = ch + (d.first ? 0 : c);
-                o.v[c] = fortis_act_any(fmaf((v[k].v[c] - off) * rstd, d.gamma ? d.gamma[i] : 1.f, d.beta ? d.beta[i] : 0.f), decltype(act)::value, d.alpha);
+                o.v[c] = fortis_act_any(fmaf((v[k].v[c] - off) * rstd, d.gamma[i], d.beta[i]), decltype(act)::value, d.alpha);
             }
             st<V>(y + at, o);
         }
@@ -249,6 +253,8 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
 #pragma unroll
         for (int k = 0; k < E; k++)
             if (on && row + k * rows < d.S) v[k] = ld<V>(a.x + base + (long)(row + k * rows) * d.C);
+        Vals<V> ga, be;
+        if (on) { ga = ld<V>(d.gamma + c0); be = ld<V>(d.beta + c0); }
         const float pivot = a.x[n * d.S * d.C + (g0 + gl) * a.cg], inv = 1.f / (float)a.count;
         // the group's sum: its threads are (row, columns gl cgv .. + cgv); one wave adds each group's partial sums
         auto group_sum = [&](float s, float s2) __attribute__((always_inline)) {
@@ -287,9 +293,6 @@ __global__ __launch_bounds__(T) void norm_block_groups_kernel(NormArgs a, int gs
         const float2 both = group_sum(s, s2);
         const float off = both.x * inv, rstd = 1.f / sqrtf(fmaf(-off, off, both.y * inv) + d.eps);
         if (!on) continue;
-        Vals<V> ga, be;
-#pragma unroll
-        for (int c = 0; c < V; c++) { ga.v[c] = d.gamma ? d.gamma[c0 + c] : 1.f; be.v[c] = d.beta ? d.beta[c0 + c] : 0.f; }
         fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < E; k++) {
@@ -541,6 +544,8 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, Spli
         for (int k = 0; k < GS_AHEAD; k++)
             if (at + w.row + k * w.rows < total) v[k] = ld<V>((const float*)(x + k * pass + off));
     }
+    Vals<V> ga, bt;
+    if (on) { ga = ld<V>(d.gamma + c0); bt = ld<V>(d.beta + c0); }
     for (int q = threadIdx.x >> 6; q < w.ng; q += GS_THREADS / 64) {
         const Stat s = join(in + (w.n * d.G + w.g0 + q) * h.parts, h.parts, (double)a.x[w.n * d.S * d.C + (w.g0 + q) * a.cg], (double)a.count, d.eps);
         if ((threadIdx.x & 63) == 0) stat[q] = s;
@@ -552,8 +557,8 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_kernel(NormArgs a, Spli
     for (int c = 0; c < V; c++) {
         const Stat s = stat[h.blocks > 1 ? 0 : (int)fortis_div((unsigned)(c0 + c), h.by_cg) - w.g0];
         hi[c] = s.hi; lo[c] = s.lo;
-        sc[c] = s.rstd * (d.gamma ? d.gamma[c0 + c] : 1.f);
-        be[c] = d.beta ? d.beta[c0 + c] : 0.f;
+        sc[c] = s.rstd * ga.v[c];
+        be[c] = bt.v[c];
     }
     const float alpha = d.alpha;
     fortis_with_act(d.act, [&](auto act) __attribute__((always_inline)) {
@@ -608,7 +613,7 @@ __global__ __launch_bounds__(GS_THREADS) void norm_apply_first_kernel(NormArgs a
         auto put = [&](int k) __attribute__((always_inline)) {
             const long e = e0 + at + k * GS_THREADS + tid;
             const long c = c0 + (small ? (long)fortis_div((unsigned)e, a.row) : e / (d.S / V));
-            const float sc = s.rstd * (d.gamma ? d.gamma[c] : 1.f), be = d.beta ? d.beta[c] : 0.f;
+            const float sc = s.rstd * d.gamma[c], be = d.beta[c];
             Vals<V> o;
 #pragma unroll
             for (int q = 0; q < V; q++) o.v[q] = fortis_act_any(fmaf((v[k].v[q] - s.hi) - s.lo, sc, be), decltype(act)::value, alpha);
@@ -639,7 +644,9 @@ static SplitShape split_shape(const NormDesc& d)
 {
     SplitShape h = {};
     const long cg = d.C / d.G;
-    const long want = 256;              // workgroups of 1024 threads: one for every compute unit
+    // Workgroups of 1024 threads: one for every compute unit.  64, 128, 256 and 512 of them take 15.1, 12.6, 11.1 and 16.3 us for 65536 x 32
+    // channels last, 61, 40, 36 and 42 for 287496 x 64.
+    const long want = 256;
     if (d.first) {
         h.V = d.S % 4 == 0 ? 4 : d.S % 2 == 0 ? 2 : 1;
         const long nv = cg * d.S / h.V, insts = d.NB * d.G;

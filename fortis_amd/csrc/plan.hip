@@ -319,9 +319,11 @@ int fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma,
     if (!tensor_ok(p, src, need) || !tensor_ok(p, dst, need) || overlap(p, src, dst)) return bad("group_norm: tensors too small or overlapping");
     Op o; o.kind = OP_NORM; o.src = src; o.dst = dst; o.B = NB; o.H = S; o.C = C; o.F = G; o.flag = channels_first ? 1 : 0;
     o.act = act; o.alpha = alpha; o.eps = eps;
-    if (gamma) { o.v0.assign(gamma, gamma + C); o.has_v[0] = true; }
-    if (beta) { o.v1.assign(beta, beta + C); o.has_v[1] = true; }
-    p->ops.push_back(std::move(o));
+    try {
+        if (gamma) o.v0.assign(gamma, gamma + C); else o.v0.assign(C, 1.f);
+        if (beta) o.v1.assign(beta, beta + C); else o.v1.assign(C, 0.f);
+        p->ops.push_back(std::move(o));
+    } catch (const std::bad_alloc&) { return bad("group_norm: out of host memory"); }
     return 0;
 }
 int fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, const float* W, const float* bias, const float* A,
@@ -705,8 +707,8 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
                 ex.kind = EX_NORM;
                 if (o.H == 1) ex.rows = ex.rows_cap = o.B;
                 ex.norm = { o.B, o.H, o.C, o.F, o.flag, o.eps, o.act, o.alpha, nullptr, nullptr };
-                if (o.has_v[0]) ex.norm.gamma = (const float*)upload(p, o.v0.data(), o.v0.size() * 4);
-                if (o.has_v[1]) ex.norm.beta = (const float*)upload(p, o.v1.data(), o.v1.size() * 4);
+                ex.norm.gamma = (const float*)upload(p, o.v0.data(), o.v0.size() * 4);
+                ex.norm.beta = (const float*)upload(p, o.v1.data(), o.v1.size() * 4);
                 break;
             case OP_ADAPT: {
                 ex.kind = EX_ADAPT; ex.side = o.side; ex.rows = ex.rows_cap = o.B;
