@@ -337,7 +337,8 @@ static void narrow_by_columns(const AdaptDesc& d, const float* X, const int* ind
 
 // ---- many rows ---------------------------------------------------------------------------------------------------
 // Rows of a window in order of their adapter, those without one behind: perm[p] = row inside the window, key[p] = its
-// adapter or -1.  A counting sort in LDS, one workgroup a window: 4.7 us whether 3 windows or 12, its barriers and atomics in turn.
+// adapter or -1.  A counting sort in LDS, one workgroup a window: 4.7 us whether 3 windows or 12, its barriers and atomics in
+// turn (rows of one adapter 1.5 us more when they were counted a second time instead of keeping what the first count returned).
 __global__ __launch_bounds__(1024) void adapt_sort_kernel(const int* __restrict__ index, int* __restrict__ perm, int* __restrict__ key, long B, int nadapt)
 {
     extern __shared__ int bin[];        // [nadapt + 1], then 16 wave sums
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(1024) void adapt_sort_kernel(const int* __restrict_
     const long r0 = (long)blockIdx.x * AD_WINDOW;
     for (int b = tid; b < bins; b += 1024) bin[b] = 0;
     __syncthreads();
-    int mine[AD_WINDOW / 1024];
+    int mine[AD_WINDOW / 1024], place[AD_WINDOW / 1024];      // bin, and how many of the bin came before
 #pragma unroll
     for (int k = 0; k < AD_WINDOW / 1024; k++) {
         const long r = r0 + tid + k * 1024;
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(1024) void adapt_sort_kernel(const int* __restrict_
         if (r < B) {
             const int i = index[r];
             mine[k] = i >= 0 && i < nadapt ? i : nadapt;
-            atomicAdd(&bin[mine[k]], 1);
+            place[k] = atomicAdd(&bin[mine[k]], 1);
         }
     }
     __syncthreads();
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(1024) void adapt_sort_kernel(const int* __restrict_
 #pragma unroll
     for (int k = 0; k < AD_WINDOW / 1024; k++) {
         if (mine[k] < 0) continue;
-        const int p = atomicAdd(&bin[mine[k]], 1);
+        const int p = bin[mine[k]] + place[k];
         perm[r0 + p] = tid + k * 1024;
         key[r0 + p] = mine[k] < nadapt ? mine[k] : -1;
     }
