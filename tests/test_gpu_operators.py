@@ -51,6 +51,16 @@ def test_group_norm(L, gpu, NB, S, Cc, G, first):
     within(run_norm(x, G, gamma, beta, 1e-5, act, alpha, first), *R.group_norm(x, G, gamma, beta, 1e-5, act, alpha, first))
 
 
+@pytest.mark.parametrize("NB,S,Cc,G", [(1, 300, 2048, 2048), (1, 600, 4096, 2048), (4, 600, 4092, 1364), (1, 400, 1028, 1028), (1, 300, 4096, 4096),
+                                       (2, 257, 1025, 1025), (1, 300, 2050, 1025), (1, 300, 6144, 2048), (1, 300, 1024, 1024)])
+def test_group_norm_of_more_groups_than_a_workgroup_has_threads(L, gpu, NB, S, Cc, G):
+    """Groups of one to three channels, channels last, positions beyond what a workgroup holds: the statistics of a slice of groups at a time."""
+    rng = np.random.default_rng(Cc + G)
+    x = (rng.standard_normal((NB, S, Cc)) + 2 * rng.standard_normal(Cc)).astype(np.float32)
+    gamma, beta = (1 + 0.2 * rng.standard_normal(Cc)).astype(np.float32), (0.1 * rng.standard_normal(Cc)).astype(np.float32)
+    within(run_norm(x, G, gamma, beta, 1e-5, "silu"), *R.group_norm(x, G, gamma, beta, 1e-5, "silu", 0, False))
+
+
 @pytest.mark.parametrize("first", [False, True])
 @pytest.mark.parametrize("act,alpha", [(None, 0.0), ("relu", 0.0), ("leaky", 0.2), ("leaky", -0.5), ("leaky", 1.5), ("silu", 0.0)])
 def test_group_norm_activations_without_vectors(L, gpu, act, alpha, first):
