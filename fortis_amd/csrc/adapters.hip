@@ -586,10 +586,20 @@ static void launch_adapt_gemm(const AdaptDesc& d, const float* X, float* Y, long
     hipLaunchKernelGGL((adapt_gemm_kernel<SC>), dim3((unsigned)grid), dim3(GM_THREADS), shmem, s, X, d.W, Y, B, d.N, d.K, sc, epi, ext);
 }
 
+// A launch has to stay under 2^32 work-items, and both forms have many to a row: rows beyond AD_PIECE, or beyond few_piece(), go through
+// them in pieces, one behind the other through the same scratch.
+#define AD_PIECE (1L << 26)     // sorted rows: up to 32 work-items each; a multiple of AD_WINDOW
+// few rows: 16 work-items a row and rank, 512 a tile of 16 rows and 16 columns; a multiple of 16 and at least 2048 (N < 2^19)
+static long few_piece(const AdaptDesc& d)
+{
+    const long by_rank = (1L << 27) / d.p.Rp / 16 * 16, by_columns = (1L << 22) / cdiv(d.N, 16) * 16;
+    return by_rank < by_columns ? by_rank : by_columns;
+}
 // Both forms' scratch: a step that has been re-sized to fewer rows may take the other one.
 long fortis_adapters_workspace(const AdaptDesc& d, long B)
 {
-    return up(B, AD_WINDOW) * 8 + B * d.p.Rp * 4;
+    const long n = B < AD_PIECE ? B : AD_PIECE;
+    return up(n, AD_WINDOW) * 8 + n * d.p.Rp * 4;
 }
 template <int ROW>
 static void launch_few(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
@@ -604,16 +614,8 @@ static void launch_few(const AdaptDesc& d, const float* X, const int* index, flo
     hipLaunchKernelGGL((adapt_few_kernel<ROW, false>), grid, block, 0, s, d, X, index, (const float*)H, Y, B);
 }
 template <bool SC>
-static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
+static void launch_sorted(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {
-    if (B > AD_FEW_ROWS && d.p.narrow) {
-        if (d.K <= 16) narrow_by_columns<1, SC>(d, X, index, Y, B, s);
-        else if (d.K <= 32) narrow_by_columns<2, SC>(d, X, index, Y, B, s);
-        else narrow_by_columns<4, SC>(d, X, index, Y, B, s);
-        return;
-    }
-    if (d.K < 4) { launch_few<ROWTINY>(d, X, index, Y, B, ws, s); return; }
-    if (B <= AD_FEW_ROWS || !d.p.finite) { launch_few<SC ? ROWANY : ROW4>(d, X, index, Y, B, ws, s); return; }
     const long Bw = up(B, AD_WINDOW);
     int *perm = (int*)ws, *key = perm + Bw;
     float* H = (float*)(key + Bw);
@@ -625,6 +627,26 @@ static void launch_adapters(const AdaptDesc& d, const float* X, const int* index
     else hipLaunchKernelGGL((adapt_low_sorted_kernel<8, SC>), blocks, dim3(512), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
     const AdaptRows<SC> ext = { perm, key, H, d.U, d.p.ldw, B, d.N, d.p.Rp };
     launch_adapt_gemm<SC>(d, X, Y, B, ext, s);
+}
+template <bool SC>
+static void launch_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
+{
+    if (B > AD_FEW_ROWS && d.p.narrow) {
+        if (d.K <= 16) narrow_by_columns<1, SC>(d, X, index, Y, B, s);
+        else if (d.K <= 32) narrow_by_columns<2, SC>(d, X, index, Y, B, s);
+        else narrow_by_columns<4, SC>(d, X, index, Y, B, s);
+        return;
+    }
+    const bool few = d.K < 4 || B <= AD_FEW_ROWS || !d.p.finite;         // by all rows: the pieces of a call take one form
+    const long piece = few ? few_piece(d) : AD_PIECE;
+    for (long r = 0; r < B; r += piece) {
+        const long n = B - r < piece ? B - r : piece;
+        const float* x = X + r * d.K;
+        float* y = Y + r * d.N;
+        if (!few) launch_sorted<SC>(d, x, index + r, y, n, ws, s);
+        else if (d.K < 4) launch_few<ROWTINY>(d, x, index + r, y, n, ws, s);
+        else launch_few<SC ? ROWANY : ROW4>(d, x, index + r, y, n, ws, s);
+    }
 }
 void fortis_launch_linear_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
 {

@@ -603,6 +603,29 @@ def test_adapters_beyond_four_gigabytes(L, gpu, K, N, block, copies):
     L.fortis_pool_trim()
 
 
+@pytest.mark.parametrize("K,N,nadapt,rank,block,copies", [(3, 8, 3, 256, 5000, 211), (2, 700, 4, 1, 8192, 380), (4, 1, 5, 17, 70000, 960)])
+def test_adapters_of_more_rows_than_a_launch_has_work_items(L, gpu, K, N, nadapt, rank, block, copies):
+    """2^28 rows x ranks and 2^31 outputs of a network too narrow for the other forms, and 2^26 sorted rows: rows go through in pieces."""
+    a = Adapted(block, K, N, nadapt, rank)
+    B = block * copies
+    p = P.Plan()
+    t, i, o = p.tensor(B * K), p.tensor(B), p.tensor(B * N)
+    p.linear_adapters(t, o, i, a.W, a.bias, a.A, a.U, B, a.scale, "leaky", a.alpha)
+    p.finalize(t, o)
+    p.write(t, a.X)
+    p.write(i, a.index)
+    _repeat(L, p.ptr(t), block * K * 4, copies)
+    _repeat(L, p.ptr(i), block * 4, copies)
+    p.run()
+    a.act = "leaky"
+    first = _block(L, p.ptr(o), (block, N))
+    within(first, *a.ref())
+    for c in sorted(set(range(0, copies, copies // 24)) | {copies - 1}):
+        assert bits_equal(_block(L, p.ptr(o) + c * block * N * 4, (block, N)), first), c
+    p.close()
+    L.fortis_pool_trim()
+
+
 @pytest.mark.parametrize("NB,S,Cc,G,first", [(1 << 14, 1, 80, 4, False), (6, 20000, 64, 8, False), (6, 20000, 64, 8, True), (512, 64, 32, 2, False)])
 def test_group_norm_beyond_four_gigabytes(L, gpu, NB, S, Cc, G, first):
     rng = np.random.default_rng(3)
