@@ -30,6 +30,7 @@ struct RecurArgs {
     const int* lengths;
     float2* maps;               // [nseq * ch][chunks]: (F, B) of a chunk, then (h in front of it, unused)
     long chunks, per;           // chunks of a sequence, steps a chunk
+    long first;                 // lane that the launch starts with
 };
 
 template <int V> __device__ __forceinline__ void load(float (&o)[V], const float* p)
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(RC_THREADS) void recurrence_walk_kernel(RecurArgs a
 {
     const RecurDesc& d = a.d;
     const long lanes = d.nseq * d.ch / V;
-    const long id = (long)blockIdx.x * RC_THREADS + threadIdx.x;
+    const long id = a.first + (long)blockIdx.x * RC_THREADS + threadIdx.x;
     if (id >= lanes * a.chunks) return;
     const long k = id / lanes, e = (id - k * lanes) * V;      // chunk, first of the lane's values in [nseq][ch]
     const long s = e / d.ch, c = e - s * d.ch;
@@ -189,21 +190,30 @@ long fortis_recurrence_workspace(const RecurDesc& d)
     return r.chunks > 1 ? d.nseq * d.ch * r.chunks * (long)sizeof(float2) : 0;
 }
 
+// A launch has to stay under 2^32 work-items.
+#define RC_PIECE (1L << 31)
+template <class K> static void launch_walk(K kernel, RecurArgs a, long lanes, hipStream_t s)
+{
+    for (a.first = 0; a.first < lanes; a.first += RC_PIECE) {
+        const long n = lanes - a.first < RC_PIECE ? lanes - a.first : RC_PIECE;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(n, RC_THREADS)), dim3(RC_THREADS), 0, s, a);
+    }
+}
 template <int V> static void launch_walks(const RecurArgs& a, hipStream_t s)
 {
-    const dim3 grid((unsigned)cdiv(a.d.nseq * a.d.ch / V * a.chunks, RC_THREADS)), block(RC_THREADS);
+    const long lanes = a.d.nseq * a.d.ch / V * a.chunks;
     if (a.chunks > 1) {
-        hipLaunchKernelGGL((recurrence_walk_kernel<V, false, false>), grid, block, 0, s, a);
-        hipLaunchKernelGGL(recurrence_scan_kernel, dim3((unsigned)cdiv(a.d.nseq * a.d.ch, RC_THREADS / 64)), block, 0, s, a);
+        launch_walk(recurrence_walk_kernel<V, false, false>, a, lanes, s);
+        hipLaunchKernelGGL(recurrence_scan_kernel, dim3((unsigned)cdiv(a.d.nseq * a.d.ch, RC_THREADS / 64)), dim3(RC_THREADS), 0, s, a);
     }
     // an output that the eight L2s (32 MB) cannot hold is written past them: 106 -> 96 us for 2 x 32768 x 384
-    if (a.d.nseq * a.d.len * a.d.ch * 4 > (32L << 20)) hipLaunchKernelGGL((recurrence_walk_kernel<V, true, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((recurrence_walk_kernel<V, true, false>), grid, block, 0, s, a);
+    if (a.d.nseq * a.d.len * a.d.ch * 4 > (32L << 20)) launch_walk(recurrence_walk_kernel<V, true, true>, a, lanes, s);
+    else launch_walk(recurrence_walk_kernel<V, true, false>, a, lanes, s);
 }
 void fortis_launch_recurrence(const RecurDesc& d, const float* src, float* dst, const float* h_in, float* h_out, const int* lengths, void* ws, hipStream_t s)
 {
     const RecurShape r = recur_shape(d);
-    const RecurArgs a = { d, src, dst, h_in, h_out, lengths, (float2*)ws, r.chunks, r.per };
+    const RecurArgs a = { d, src, dst, h_in, h_out, lengths, (float2*)ws, r.chunks, r.per, 0 };
     if (r.V == 2) launch_walks<2>(a, s);
     else launch_walks<1>(a, s);
     HIP_OK(hipGetLastError());

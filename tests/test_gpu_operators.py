@@ -665,3 +665,25 @@ def test_recurrence_beyond_four_gigabytes(L, gpu, q, n, c):
     assert bits_equal(_block(L, p.ptr(h) + (copies - 1) * q * c * 4, (q, c)), _block(L, p.ptr(h), (q, c)))
     p.close()
     L.fortis_pool_trim()
+
+
+def test_recurrence_of_more_lanes_than_a_launch_has_work_items(L, gpu):
+    """2^32 values of one step, one a lane: the walk takes them in pieces."""
+    rng = np.random.default_rng(14)
+    q, c, copies = 64, 65537, 1025
+    assert q * c * copies > 1 << 32
+    src = rng.standard_normal((q, 2 * c)).astype(np.float32)
+    p = P.Plan()
+    t, o = p.tensor(src.size * copies), p.tensor(q * c * copies)
+    p.recurrence(t, o, q * copies, 1, c)
+    p.finalize(t, o)
+    p.write(t, src)
+    _repeat(L, p.ptr(t), src.nbytes, copies)
+    p.run()
+    first = _block(L, p.ptr(o), (q, c))
+    ry, _, ey, _ = R.recurrence(src, None, None, q, 1, c, True, False, np.zeros((q, c)))
+    within(first, ry, ey)
+    for k in list(range(0, copies, 128)) + [copies - 2, copies - 1]:
+        assert bits_equal(_block(L, p.ptr(o) + k * q * c * 4, (q, c)), first), k
+    p.close()
+    L.fortis_pool_trim()
