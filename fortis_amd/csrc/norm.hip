@@ -757,7 +757,7 @@ template <int V> static void launch_block(const NormArgs& a, NormKind kind, int 
     else if (d.S <= 1024 / wv * 4) hipLaunchKernelGGL((norm_block_groups_kernel<V, 1024, 4>), grid, dim3(1024), 0, s, a, gs, slices, total);
     else hipLaunchKernelGGL((norm_block_groups_kernel<V, 1024, 8>), grid, dim3(1024), 0, s, a, gs, slices, total);
 }
-template <int V> static void launch_split(const NormArgs& a, const SplitShape& h, void* ws, hipStream_t s)
+template <int V> static void launch_split(NormArgs a, const SplitShape& h, void* ws, hipStream_t s)
 {
     const NormDesc& d = a.d;
     double2* part = (double2*)ws;
@@ -765,18 +765,21 @@ template <int V> static void launch_split(const NormArgs& a, const SplitShape& h
     // launch is about to read (287496 x 64, 74 MB: 49.7 us through the caches, 40.5 us past them; 65536 x 32, 8 MB: no difference,
     // and the next kernel finds it there).
     const bool stream = d.NB * d.S * d.C * 4 > (32L << 20);
-    if (d.first) {
-        const dim3 grid((unsigned)(d.NB * d.G * h.chunks));
-        hipLaunchKernelGGL((norm_sums_first_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, part);
-        if (stream) hipLaunchKernelGGL((norm_apply_first_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
-        else hipLaunchKernelGGL((norm_apply_first_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
-        return;
+    // A launch has to stay under 2^32 work-items: as many samples at a time as 2^21 workgroups take.
+    const long wgs = d.first ? d.G * h.chunks : (long)h.slices * h.blocks * h.chunks, piece = (1L << 21) / wgs;
+    for (long n = 0; n < d.NB; n += piece, a.x += piece * d.S * d.C, a.y += piece * d.S * d.C, part += piece * d.G * h.parts) {
+        const dim3 grid((unsigned)((d.NB - n < piece ? d.NB - n : piece) * wgs));
+        if (d.first) {
+            hipLaunchKernelGGL((norm_sums_first_kernel<V>), grid, dim3(GS_THREADS), 0, s, a, h, part);
+            if (stream) hipLaunchKernelGGL((norm_apply_first_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+            else hipLaunchKernelGGL((norm_apply_first_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+            continue;
+        }
+        if (a.cg % V == 0) hipLaunchKernelGGL((norm_sums_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, part);
+        else if constexpr (V > 1) hipLaunchKernelGGL((norm_sums_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, part);
+        if (stream) hipLaunchKernelGGL((norm_apply_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
+        else hipLaunchKernelGGL((norm_apply_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
     }
-    const dim3 grid((unsigned)(d.NB * h.slices * h.blocks * h.chunks));
-    if (a.cg % V == 0) hipLaunchKernelGGL((norm_sums_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, part);
-    else if constexpr (V > 1) hipLaunchKernelGGL((norm_sums_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, part);
-    if (stream) hipLaunchKernelGGL((norm_apply_kernel<V, true>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
-    else hipLaunchKernelGGL((norm_apply_kernel<V, false>), grid, dim3(GS_THREADS), 0, s, a, h, (const double2*)part);
 }
 
 void fortis_launch_group_norm(const NormDesc& in, const float* x, float* y, void* ws, hipStream_t s)

@@ -645,6 +645,27 @@ def test_group_norm_beyond_four_gigabytes(L, gpu, NB, S, Cc, G, first):
     L.fortis_pool_trim()
 
 
+def test_group_norm_of_more_values_than_a_launch_has_work_items(L, gpu):
+    """Rows of 32769, 33 workgroups of 1024 threads each: 2^32 work-items at 130150 rows."""
+    rng = np.random.default_rng(15)
+    block, Cc, copies = 64, 32769, 2050
+    assert block * copies * 33 * 1024 > 1 << 32
+    x = rng.standard_normal((block, 1, Cc)).astype(np.float32)
+    p = P.Plan()
+    t, o = p.tensor(x.size * copies), p.tensor(x.size * copies)
+    p.group_norm(t, o, block * copies, 1, Cc, 1, act="relu")
+    p.finalize(t, o)
+    p.write(t, x)
+    _repeat(L, p.ptr(t), x.nbytes, copies)
+    p.run()
+    first = _block(L, p.ptr(o), x.shape)
+    within(first, *R.group_norm(x, 1, None, None, 1e-5, "relu", 0, False))
+    for k in list(range(0, copies, 128)) + [copies - 2, copies - 1]:
+        assert bits_equal(_block(L, p.ptr(o) + k * x.nbytes, x.shape), first), k
+    p.close()
+    L.fortis_pool_trim()
+
+
 @pytest.mark.parametrize("q,n,c", [(64, 100, 40), (2, 3000, 8)])
 def test_recurrence_beyond_four_gigabytes(L, gpu, q, n, c):
     """Sequence-major: a block of sequences again and again."""
