@@ -40,9 +40,12 @@ __global__ void zero_kernel(float* __restrict__ dst, long n)
 }
 void fortis_launch_zero(float* dst, long n, hipStream_t s)
 {
-    if (n <= 0) return;
-    hipLaunchKernelGGL(zero_kernel, dim3((unsigned)cdiv(n, EW_THREADS)), dim3(EW_THREADS), 0, s, dst, n);
-    HIP_OK(hipGetLastError());
+    // (a launch has to stay under 2^32 work-items)
+    for (const long piece = 1L << 31; n > 0; n -= piece, dst += piece) {
+        const long m = n < piece ? n : piece;
+        hipLaunchKernelGGL(zero_kernel, dim3((unsigned)cdiv(m, EW_THREADS)), dim3(EW_THREADS), 0, s, dst, m);
+        HIP_OK(hipGetLastError());
+    }
 }
 __global__ void fill_int_kernel(int* __restrict__ dst, int v, long n)
 {

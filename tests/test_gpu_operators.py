@@ -708,3 +708,27 @@ def test_recurrence_of_more_lanes_than_a_launch_has_work_items(L, gpu):
         assert bits_equal(_block(L, p.ptr(o) + k * q * c * 4, (q, c)), first), k
     p.close()
     L.fortis_pool_trim()
+
+
+def test_states_of_2_to_the_32_values_start_as_zeros(L, gpu):
+    q, c = 65600, 65537
+    n = 1 << 20
+    held = P.Plan()                                  # its buffer, filled, is what the state's is taken from
+    t, o, s = held.tensor(2), held.tensor(1), held.tensor(q * c)
+    held.recurrence(t, o, 1, 1, 1, h_in=s)
+    held.finalize(t, o)
+    held.write(s, np.full(n, 7, np.float32))
+    _repeat(L, held.ptr(s), n * 4, q * c // n)
+    L.fortis_d2d(held.ptr(s) + (q * c - n) * 4, held.ptr(s), n * 4)
+    at = held.ptr(s)
+    held.close()
+    p = P.Plan()
+    s, t, o = p.tensor(q * c), p.tensor(q * c * 2), p.tensor(q * c)
+    p.recurrence(t, o, q, 1, c, h_in=s)
+    p.finalize(t, o)
+    assert p.ptr(s) == at
+    for k in (0, (1 << 31) // n, q * c // n - 1):
+        assert not _block(L, p.ptr(s) + k * n * 4, (n,)).any(), k
+    assert not _block(L, p.ptr(s) + (q * c - n) * 4, (n,)).any()
+    p.close()
+    L.fortis_pool_trim()
