@@ -468,23 +468,10 @@ static int assign_buffers(fortis_plan* p)
         if (e.head_dst < 0) writes(e.dst, i);
         writes(e.pool_dst, i); writes(e.head_dst, i); writes(e.h_out, i);
     }
-    // A side tensor (adapter indices, lengths, a state that comes in) that no earlier kernel of the pass writes is the
-    // caller's or the last pass's: its buffer is never shared, whatever is written to other windows of it.  Nor is that
-    // of a state that goes out, which the caller reads behind the pass.
-    auto written_before = [&](int t, int i) {
-        for (int j = 0; j < i; j++) {
-            const Exec& e = p->exec[j];
-            for (int w : { e.head_dst < 0 ? e.dst : -1, e.pool_dst, e.head_dst, e.h_out }) if (w >= 0 && overlap(p, w, t)) return true;
-        }
-        return false;
-    };
-    std::vector<char> fill_side(ne, 0), fill_in(ne, 0), fill_out(ne, 0);
-    for (int i = 0; i < ne; i++) {
-        const Exec& e = p->exec[i];
-        if (e.side >= 0 && !written_before(e.side, i)) { fill_side[i] = 1; first[base(e.side)] = -1; last[base(e.side)] = ne; }
-        if (e.h_in >= 0 && !written_before(e.h_in, i)) { fill_in[i] = 1; first[base(e.h_in)] = -1; last[base(e.h_in)] = ne; }
-        if (e.h_out >= 0) { fill_out[i] = !written_before(e.h_out, i); first[base(e.h_out)] = -1; last[base(e.h_out)] = ne; }
-    }
+    // A side tensor (adapter indices, lengths, a state that comes in) is the caller's or the last pass's, and a state that goes out is
+    // read behind the pass: their buffers are never shared.  That holds too where an earlier kernel writes into them: it may write a part only.
+    for (const Exec& e : p->exec)
+        for (int t : { e.side, e.h_in, e.h_out }) if (t >= 0) { first[base(t)] = -1; last[base(t)] = ne; }
     for (int t = 0; t < nt; t++) if (first[t] == -1) last[t] = ne;          // filled by the caller: never handed back
     first[base(p->in_t)] = -1; last[base(p->in_t)] = ne;
     if (first[base(p->out_t)] == never) first[base(p->out_t)] = -1;
@@ -526,14 +513,13 @@ static int assign_buffers(fortis_plan* p)
     if (rc != 0) { p->tptr.assign(nt, nullptr); return -1; }
     for (int t = 0; t < nt; t++)
         if (p->view_of[t] >= 0 && p->tptr[p->view_of[t]]) p->tptr[t] = (char*)p->tptr[p->view_of[t]] + p->view_off[t];
-    // what a side tensor that no kernel writes holds until the caller writes it (not for a test's host allocator: no device)
+    // what a side tensor holds until it is written (not for a test's host allocator: no device)
     if (!fortis_pool_on_device()) return 0;
-    for (int i = 0; i < ne; i++) {
-        const Exec& e = p->exec[i];
-        if (fill_side[i])
-            fortis_launch_fill_int((int*)p->tptr[e.side], e.kind == EX_ADAPT ? -1 : (int)e.op->H, e.kind == EX_ADAPT ? e.rows_cap : e.op->B, fortis_stream_get());
-        if (fill_in[i]) fortis_launch_zero((float*)p->tptr[e.h_in], e.op->B * e.op->C, fortis_stream_get());
-        if (fill_out[i]) fortis_launch_zero((float*)p->tptr[e.h_out], e.op->B * e.op->C, fortis_stream_get());
+    hipStream_t s = fortis_stream_get();
+    for (const Exec& e : p->exec) {
+        if (e.side >= 0)
+            fortis_launch_fill_int((int*)p->tptr[e.side], e.kind == EX_ADAPT ? -1 : (int)e.op->H, e.kind == EX_ADAPT ? e.rows_cap : e.op->B, s);
+        for (int t : { e.h_in, e.h_out }) if (t >= 0) fortis_launch_zero((float*)p->tptr[t], e.op->B * e.op->C, s);
     }
     return 0;
 }

@@ -147,6 +147,29 @@ def test_states_and_lengths_keep_buffers_of_their_own(pool):  # noqa: F811
     assert stats(L)[1] == 0
 
 
+def test_side_tensors_that_a_kernel_writes_in_part_keep_buffers_of_their_own(pool):  # noqa: F811
+    """The lengths and the state lie in tensors whose front an earlier operation writes: the rest is still the caller's."""
+    L, dev = pool
+    dev.capacity = 4000
+    p = L.fortis_plan_create()
+    T = lambda n: L.fortis_plan_tensor(p, 4 * n)  # noqa: E731
+    x, c, d, e, y = T(16), T(16), T(8), T(36), T(46)
+    le, st = T(40), T(48)
+    lengths, state = L.fortis_plan_view(p, le, 64, 96), L.fortis_plan_view(p, st, 64, 128)
+    ok = lambda r: r == 0 or pytest.fail("refused")  # noqa: E731
+    ok(L.fortis_plan_mask_relu(p, x, c, 1, 16, 16))
+    ok(L.fortis_plan_mask_relu(p, c, le, 1, 16, 16))
+    ok(L.fortis_plan_mask_relu(p, c, st, 1, 16, 16))
+    ok(L.fortis_plan_recurrence(p, c, d, state, -1, lengths, 1, 1, 8, 1, 0))
+    ok(L.fortis_plan_mask_relu(p, d, e, 1, 8, 8))
+    ok(L.fortis_plan_mask_relu(p, e, y, 1, 8, 8))
+    assert L.fortis_plan_finalize(p, x, y) == 0
+    ptr = {t: L.fortis_plan_tensor_ptr(p, t) for t in (x, c, d, e, y, le, st)}
+    for t in (le, st):
+        assert all(ptr[t] != q for k, q in ptr.items() if k != t), t
+    L.fortis_plan_destroy(p)
+
+
 def test_model_tensor_without_a_step(L):
     L.fortis_step_reset()
     assert L.fortis_model_tensor(0) is None
