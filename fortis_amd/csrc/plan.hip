@@ -446,6 +446,8 @@ static size_t try_chain(fortis_plan* p, size_t i, Exec* ex)
     return j - i;
 }
 
+static bool leaves_rows(const Exec& e) { return e.kind == EX_RECUR && e.side >= 0; }
+
 // Gives every tensor its device buffer by walking the kernels in launch order the way the reference's generated
 // host code does at run time (compiler/FortisFuse.cpp:512-516: a temporary is taken from the pool in front of
 // the group that first writes it and handed back behind the group that last reads it), so that temporaries
@@ -470,8 +472,9 @@ static int assign_buffers(fortis_plan* p)
     }
     // A side tensor (adapter indices, lengths, a state that comes in) is the caller's or the last pass's, and a state that goes out is
     // read behind the pass: their buffers are never shared.  That holds too where an earlier kernel writes into them: it may write a part only.
+    // Nor is the output of a recurrence with lengths shared, which leaves rows as they were.
     for (const Exec& e : p->exec)
-        for (int t : { e.side, e.h_in, e.h_out }) if (t >= 0) { first[base(t)] = -1; last[base(t)] = ne; }
+        for (int t : { e.side, e.h_in, e.h_out, leaves_rows(e) ? e.dst : -1 }) if (t >= 0) { first[base(t)] = -1; last[base(t)] = ne; }
     for (int t = 0; t < nt; t++) if (first[t] == -1) last[t] = ne;          // filled by the caller: never handed back
     first[base(p->in_t)] = -1; last[base(p->in_t)] = ne;
     if (first[base(p->out_t)] == never) first[base(p->out_t)] = -1;
@@ -513,9 +516,10 @@ static int assign_buffers(fortis_plan* p)
     if (rc != 0) { p->tptr.assign(nt, nullptr); return -1; }
     for (int t = 0; t < nt; t++)
         if (p->view_of[t] >= 0 && p->tptr[p->view_of[t]]) p->tptr[t] = (char*)p->tptr[p->view_of[t]] + p->view_off[t];
-    // what a side tensor holds until it is written (not for a test's host allocator: no device)
+    // what a side tensor, or a row behind the lengths, holds until it is written (not for a test's host allocator: no device)
     if (!fortis_pool_on_device()) return 0;
     hipStream_t s = fortis_stream_get();
+    for (const Exec& e : p->exec) if (leaves_rows(e)) fortis_launch_zero((float*)p->tptr[e.dst], e.op->B * e.op->H * e.op->C, s);
     for (const Exec& e : p->exec) {
         if (e.side >= 0)
             fortis_launch_fill_int((int*)p->tptr[e.side], e.kind == EX_ADAPT ? -1 : (int)e.op->H, e.kind == EX_ADAPT ? e.rows_cap : e.op->B, s);
@@ -1373,9 +1377,11 @@ void mlp_forward(void* in, void* out)
     bool direct = nin <= 32 * 1024 && nout <= 32 * 1024 && !getenv("FORTIS_NO_ZEROCOPY") && p->in_t != p->out_t;
     for (size_t t = 0; direct && t < p->view_of.size(); t++)
         if (p->view_of[t] == p->in_t || p->view_of[t] == p->out_t) direct = false;
-    // a side tensor or a carried state keeps its place on the device
-    for (const Exec& e : p->exec)
+    // a side tensor, a carried state or an output of which rows are left as they were keeps its place on the device
+    for (const Exec& e : p->exec) {
+        if (leaves_rows(e) && overlap(p, e.dst, p->out_t)) direct = false;
         for (int t : { e.side, e.h_in, e.h_out }) if (t >= 0 && (t == p->in_t || t == p->out_t)) direct = false;
+    }
     if (direct) {
         if (!g_step.X) setup_xy();
         memcpy(g_step.X, in, nin);

@@ -135,9 +135,9 @@ int  fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, co
  * receives the state behind the last one, -1: none.  h_in == h_out carries the state from pass to pass (len = 1 is one
  * step of a host that steps through time); a state that no operation of the plan writes first starts as zeros.
  * lengths: tensor of nseq int32, -1: all `len`; sequence s takes steps 0 .. lengths[s] - 1 only (values are clamped to
- * [0, len]; filled with len at finalize).  Rows of dst at and behind a sequence's length are left as they were (a tensor
- * between two operations shares its memory with others: what stands there is then whatever they left), a sequence without
- * steps hands its state on unchanged.  Long sequences are cut into chunks whose maps are composed first: an infinite value
+ * [0, len]; filled with len at finalize).  Rows of dst at and behind a sequence's length are left as they were, zeros until
+ * something else writes them (with lengths, dst never shares its memory with other tensors; an entry that copies the output
+ * to the host copies those rows too), a sequence without steps hands its state on unchanged.  Long sequences are cut into chunks whose maps are composed first: an infinite value
  * in front of a chunk may come out as NaN behind it. */
 int  fortis_plan_recurrence(fortis_plan* p, int src, int dst, int h_in, int h_out, int lengths, long nseq, long len,
                             long ch, int time_major, int reverse);

@@ -501,6 +501,35 @@ def test_recurrent_block_through_the_entries_and_a_graph(L, gpu, q, monkeypatch)
     eager.close()
 
 
+@pytest.mark.parametrize("q", [6, 3000])
+def test_rows_behind_the_lengths_through_the_entries(L, gpu, q):
+    """Two norms in front, whose buffers the output must not take over; the host's array receives what the device tensor holds in the rows
+    that are left as they were: zeros at first, then what the host wrote there.  6 sequences take the path without copies, 3000 the other."""
+    n, c = 5, 8
+    rows = q * n
+    rng = np.random.default_rng(q)
+    lengths = rng.integers(0, n + 1, q).astype(np.int32)
+    lengths[:2] = 0, n
+    p = P.Plan()
+    x, a, b, y, le = p.tensor(rows * 2 * c), p.tensor(rows * 2 * c), p.tensor(rows * 2 * c), p.tensor(rows * c), p.tensor(q)
+    p.group_norm(x, a, rows, 1, 2 * c, 2)
+    p.group_norm(a, b, rows, 1, 2 * c, 2)
+    p.recurrence(b, y, q, n, c, lengths=le)
+    p.finalize(x, y)
+    p.write(le, lengths)
+    behind = np.arange(n)[:, None] >= lengths[None]
+    step.reset()
+    step.bind(p, rows * 2 * c, rows * c)
+    for k in range(3):
+        out = np.full((n, q, c), -5, np.float32)
+        step.mlp_forward(rng.standard_normal((rows, 2 * c)).astype(np.float32), out)
+        assert (out[behind] == (0 if k == 0 else -77)).all() and (out[~behind] != -77).all()
+        held = np.full((n, q, c), -77, np.float32)
+        L.fortis_h2d(step.fortis_model_tensor(y), _vp(held), held.nbytes)
+    step.reset()
+    p.close()
+
+
 def test_run_time_extents_of_an_adapted_row_network(L, gpu):
     """fortis_begin re-sizes a batched step of adapted projections and one-position norms, down and up."""
     K, c, N, rows = 27, 32, 3, 500

@@ -170,6 +170,28 @@ def test_side_tensors_that_a_kernel_writes_in_part_keep_buffers_of_their_own(poo
     L.fortis_plan_destroy(p)
 
 
+def test_rows_left_as_they_were_share_no_buffer(pool):  # noqa: F811
+    """The output of a recurrence with lengths, at the end of a plan and between two operations."""
+    L, dev = pool
+    dev.capacity = 4000
+    p = L.fortis_plan_create()
+    T = lambda n: L.fortis_plan_tensor(p, 4 * n)  # noqa: E731
+    x, a, b, c, d, e, y, le = T(16), T(16), T(16), T(8), T(16), T(16), T(8), T(1)
+    ok = lambda r: r == 0 or pytest.fail("refused")  # noqa: E731
+    ok(L.fortis_plan_mask_relu(p, x, a, 1, 16, 16))
+    ok(L.fortis_plan_mask_relu(p, a, b, 1, 16, 16))
+    ok(L.fortis_plan_recurrence(p, b, c, -1, -1, le, 1, 1, 8, 1, 0))
+    ok(L.fortis_plan_concat_copy(p, c, d, 1, 8, 0, 2))
+    ok(L.fortis_plan_concat_copy(p, c, d, 1, 8, 1, 2))
+    ok(L.fortis_plan_mask_relu(p, d, e, 1, 16, 16))
+    ok(L.fortis_plan_recurrence(p, e, y, -1, -1, le, 1, 1, 8, 1, 0))
+    assert L.fortis_plan_finalize(p, x, y) == 0
+    ptr = {t: L.fortis_plan_tensor_ptr(p, t) for t in (x, a, b, c, d, e, y, le)}
+    for t in (c, y):
+        assert all(ptr[t] != q for k, q in ptr.items() if k != t), t
+    L.fortis_plan_destroy(p)
+
+
 def test_model_tensor_without_a_step(L):
     L.fortis_step_reset()
     assert L.fortis_model_tensor(0) is None
