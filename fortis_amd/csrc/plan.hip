@@ -1357,6 +1357,13 @@ void mlp_forward(void* in, void* out)
 {
     if (!bound("mlp_forward")) return;
     const fortis_host_t& h = g_step.h;
+    if (h.verdict == FORTIS_VERDICT_BATCHED)
+        for (const Exec& e : g_step.plan->exec)
+            if (e.h_out >= 0) {
+                // the other rows would be run again on the inputs of an earlier pass
+                fprintf(stderr, "mlp_forward: one row of a batched step whose plan writes states would move the states of all rows; nothing computed\n");
+                return;
+            }
     hipStream_t s = fortis_stream_get();
     if (h.verdict == FORTIS_VERDICT_BATCHED) {
         // a call outside the distributed loop: one row through the batched model (driver/fortis_shim.py:122)

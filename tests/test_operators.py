@@ -7,7 +7,7 @@ import subprocess
 import numpy as np
 import pytest
 
-from fortis_amd import plan as P, shim_hip as SH
+from fortis_amd import plan as P, shim_hip as SH, step
 from test_host_logic import pool, stats  # noqa: F401  (fixture)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -190,6 +190,23 @@ def test_rows_left_as_they_were_share_no_buffer(pool):  # noqa: F811
     for t in (c, y):
         assert all(ptr[t] != q for k, q in ptr.items() if k != t), t
     L.fortis_plan_destroy(p)
+
+
+def test_one_row_of_a_batched_step_moves_no_states(pool, capfd):  # noqa: F811
+    L, dev = pool
+    for h_in, h_out in ((True, True), (False, True)):
+        p = P.Plan()
+        x, y, st = p.tensor(4 * 6), p.tensor(4 * 3), p.tensor(4 * 3)
+        p.recurrence(x, y, 4, 1, 3, h_in=st if h_in else -1, h_out=st if h_out else -1)
+        p.finalize(x, y)
+        step.reset()
+        step.bind(p, 24, 12, verdict="batched", count=4)
+        out, errors = np.full(3, -5, np.float32), L.fortis_error_count()
+        step.mlp_forward(np.ones(6, np.float32), out)
+        assert (out == -5).all() and L.fortis_error_count() == errors            # nothing was asked of a device
+        assert "one row" in capfd.readouterr().err
+        step.reset()
+        p.close()
 
 
 def test_model_tensor_without_a_step(L):
