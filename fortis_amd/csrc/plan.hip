@@ -446,6 +446,8 @@ static size_t try_chain(fortis_plan* p, size_t i, Exec* ex)
     return j - i;
 }
 
+// The recurrence of `e` over its first `rows` rows where it takes one step (and can be re-sized), over all its sequences otherwise.
+static RecurDesc recur_desc(const Exec& e, long rows) { return { e.op->H == 1 ? rows : e.op->B, e.op->H, e.op->C, e.op->flag & 1, e.op->flag >> 1 }; }
 static bool leaves_rows(const Exec& e) { return e.kind == EX_RECUR && e.side >= 0; }
 
 // Gives every tensor its device buffer by walking the kernels in launch order the way the reference's generated
@@ -519,11 +521,14 @@ static int assign_buffers(fortis_plan* p)
     // what a side tensor, or a row behind the lengths, holds until it is written (not for a test's host allocator: no device)
     if (!fortis_pool_on_device()) return 0;
     hipStream_t s = fortis_stream_get();
-    for (const Exec& e : p->exec) if (leaves_rows(e)) fortis_launch_zero((float*)p->tptr[e.dst], e.op->B * e.op->H * e.op->C, s);
+    for (const Exec& e : p->exec)
+        if (leaves_rows(e)) { const RecurDesc d = recur_desc(e, e.rows_cap); fortis_launch_zero((float*)p->tptr[e.dst], d.nseq * d.len * d.ch, s); }
     for (const Exec& e : p->exec) {
-        if (e.side >= 0)
-            fortis_launch_fill_int((int*)p->tptr[e.side], e.kind == EX_ADAPT ? -1 : (int)e.op->H, e.kind == EX_ADAPT ? e.rows_cap : e.op->B, s);
-        for (int t : { e.h_in, e.h_out }) if (t >= 0) fortis_launch_zero((float*)p->tptr[t], e.op->B * e.op->C, s);
+        if (e.kind == EX_ADAPT) fortis_launch_fill_int((int*)p->tptr[e.side], -1, e.rows_cap, s);
+        if (e.kind != EX_RECUR) continue;
+        const RecurDesc d = recur_desc(e, e.rows_cap);
+        if (e.side >= 0) fortis_launch_fill_int((int*)p->tptr[e.side], (int)d.len, d.nseq, s);
+        for (int t : { e.h_in, e.h_out }) if (t >= 0) fortis_launch_zero((float*)p->tptr[t], d.nseq * d.ch, s);
     }
     return 0;
 }
@@ -540,7 +545,7 @@ static int assign_workspaces(fortis_plan* p)
             n = fortis_norm_workspace(d);
         }
         else if (e.kind == EX_ADAPT) n = fortis_adapters_workspace(e.adapt, e.rows_cap);
-        else if (e.kind == EX_RECUR) n = fortis_recurrence_workspace({ e.op->B, e.op->H, e.op->C, e.op->flag & 1, e.op->flag >> 1 });
+        else if (e.kind == EX_RECUR) n = fortis_recurrence_workspace(recur_desc(e, e.rows_cap));
         e.ws = nullptr;
         if (n <= 0) continue;
         if (fortis_dev_malloc(&e.ws, (size_t)n, "kernel scratch") != 0) return -1;
@@ -720,6 +725,7 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
             }
             case OP_RECUR:
                 ex.kind = EX_RECUR; ex.side = o.side; ex.h_in = o.h_in; ex.h_out = o.h_out;
+                if (o.H == 1) ex.rows = ex.rows_cap = o.B;
                 break;
         }
         p->exec.push_back(ex);
@@ -728,8 +734,8 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
     bool rowwise = true;
     long rows = -1;
     for (const Exec& e : p->exec) {
-        // (one-position group norms and adapted projections work row by row too)
-        if (e.kind > EX_MASK && e.kind != EX_ADAPT && !(e.kind == EX_NORM && e.norm.S == 1)) { rowwise = false; break; }
+        // (one-position group norms, adapted projections and recurrences of one step work row by row too)
+        if (e.kind > EX_MASK && e.kind != EX_ADAPT && !(e.kind == EX_NORM && e.norm.S == 1) && !(e.kind == EX_RECUR && e.op->H == 1)) { rowwise = false; break; }
         if (rows < 0) rows = e.rows; else if (rows != e.rows) rowwise = false;
     }
     p->rows0 = rowwise ? rows : 0;
@@ -819,7 +825,7 @@ void fortis_plan_run(fortis_plan* p)
             }
             case EX_ADAPT: fortis_launch_linear_adapters(e.adapt, src, (const int*)p->tptr[e.side], dst, e.rows, e.ws, s); break;
             case EX_RECUR:
-                fortis_launch_recurrence({ o->B, o->H, o->C, o->flag & 1, o->flag >> 1 }, src, dst, e.h_in >= 0 ? (const float*)p->tptr[e.h_in] : nullptr,
+                fortis_launch_recurrence(recur_desc(e, e.rows), src, dst, e.h_in >= 0 ? (const float*)p->tptr[e.h_in] : nullptr,
                                          e.h_out >= 0 ? (float*)p->tptr[e.h_out] : nullptr, e.side >= 0 ? (const int*)p->tptr[e.side] : nullptr, e.ws, s);
                 break;
         }

@@ -100,8 +100,10 @@ int  fortis_plan_permute(fortis_plan* p, int src, int dst, long C, long S, int t
  * All of them work on float32 tensors in the row layout of the other calls and refuse (-1 and a message) tensors
  * that are too small or whose windows overlap.  Side tensors (index, lengths, states) are declared with
  * fortis_plan_tensor like any other; the caller fills them through fortis_plan_tensor_ptr (a host behind the bind(c)
- * entries: fortis_model_tensor) before a pass, and they keep their contents from pass to pass.  A fortis_begin that grows
- * the step moves every tensor: addresses are asked for again, an index starts over with -1, lengths with len, states with 0. */
+ * entries: fortis_model_tensor) before a pass, and they keep their contents from pass to pass.  fortis_begin re-sizes plans that work
+ * row by row: projections with adapters, group norms with S = 1 and recurrences with len = 1 among them.  With fewer rows the first
+ * ones are taken and the states of the others stay; a fortis_begin that grows the step moves every tensor: addresses are asked for
+ * again, an index starts over with -1, lengths with len, states with 0. */
 
 /* Group normalisation with an activation, NB samples of S positions and C channels, channels last ([NB][S][C]) or, with
  * channels_first, [NB][C][S]: for every sample and every group of C / G neighbouring channels

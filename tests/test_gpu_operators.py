@@ -557,6 +557,43 @@ def test_run_time_extents_of_an_adapted_row_network(L, gpu):
     p.close()
 
 
+def test_run_time_extents_of_a_step_through_time(L, gpu):
+    """A batched step with a recurrence of one step: fewer rows advance the states of the first rows only, more rows move the tensors and start
+    over with states of zero and lengths of one."""
+    K, c, rows = 9, 16, 300
+    rng = np.random.default_rng(17)
+    f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+    W, A, U = f(2 * c, K) / np.float32(3), f(3, 2, K), f(3, 2 * c, 2)
+    p = P.Plan()
+    x, i, g, h, st, le, y = p.tensor(rows * K), p.tensor(rows), p.tensor(rows * 2 * c), p.tensor(rows * c), p.tensor(rows * c), p.tensor(rows), p.tensor(rows * c)
+    p.linear_adapters(x, g, i, W, None, A, U, rows)
+    p.recurrence(g, h, rows, 1, c, st, st, le)
+    p.group_norm(h, y, rows, 1, c, 2, act="silu")
+    p.finalize(x, y)
+    step.reset()
+    step.bind(p, rows * K, rows * c, verdict="batched", count=rows)
+    state, old, at = np.zeros((rows, c)), np.zeros((rows, c)), p.ptr(st)
+    for n in (300, 40, 40, 300, 2500, 2500, 7):
+        step.fortis_begin(n)
+        if n > len(state):
+            assert p.ptr(st) != at
+            state, old = np.zeros((n, c)), np.zeros((n, c))
+        X, Y, index = f(n, K), np.zeros((n, c), np.float32), rng.integers(-1, 3, n).astype(np.int32)
+        L.fortis_h2d(step.fortis_model_tensor(i), _vp(index), index.nbytes)
+        lengths = np.ones(n, np.int32)
+        if n != 2500:                                # there the lengths that a growth starts with
+            lengths[::5] = 0
+            L.fortis_h2d(step.fortis_model_tensor(le), _vp(lengths), lengths.nbytes)
+        step.mlp_forward_batched(X, Y)
+        g64, _ = R.linear_adapters(X, index, W, None, A, U, None, None, 0)
+        old[:n], state[:n], _, _ = R.recurrence(g64, state[:n], lengths, n, 1, c, True, False, old[:n])
+        z, _ = R.group_norm(old[:n, None], 2, None, None, 1e-5, "silu", 0, False)
+        assert np.abs(p.read(st, state.shape) - state).max() < BLOCK_TOL * np.abs(state).max()
+        assert np.abs(Y - z[:, 0]).max() < BLOCK_TOL * np.abs(z).max()
+    step.reset()
+    p.close()
+
+
 def test_image_block_channels_first_behind_a_convolution(L, gpu):
     """conv 3 x 3 -> group norm + SiLU on the convolution's own order -> channels last -> adapted 1 x 1 projection."""
     from oracle import oracle as O
