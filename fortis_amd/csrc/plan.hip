@@ -224,6 +224,7 @@ int fortis_plan_conv2d(fortis_plan* p, int src, int dst, const float* W, const f
 {
     if (!p || p->finalized) return bad("plan is null or already finalized");
     if (C <= 0 || H <= 0 || Wd <= 0 || F <= 0 || KH <= 0 || KW <= 0 || stride <= 0 || pad < 0 || !W) return bad("conv2d: bad shape");
+    if (act < 0 || act > FORTIS_ACT_LEAKY) return bad("conv2d: unknown activation");
     const long Ho = (H + 2 * pad - KH) / stride + 1, Wo = (Wd + 2 * pad - KW) / stride + 1;
     if (ctot <= 0) { ctot = F; coff = 0; }
     if (Ho <= 0 || Wo <= 0 || coff < 0 || coff + F > ctot) return bad("conv2d: bad output shape or channel offset");
@@ -244,6 +245,7 @@ int fortis_plan_convt2d(fortis_plan* p, int src, int dst, const float* W, const 
 {
     if (!p || p->finalized) return bad("plan is null or already finalized");
     if (C <= 0 || H <= 0 || Wd <= 0 || F <= 0 || KH <= 0 || KW <= 0 || stride <= 0 || pad < 0 || !W) return bad("convt2d: bad shape");
+    if (act < 0 || act > FORTIS_ACT_LEAKY) return bad("convt2d: unknown activation");
     const long Ho = (H - 1) * stride - 2 * pad + KH + output_padding, Wo = (Wd - 1) * stride - 2 * pad + KW + output_padding;
     if (ctot <= 0) { ctot = F; coff = 0; }
     if (Ho <= 0 || Wo <= 0 || coff < 0 || coff + F > ctot) return bad("convt2d: bad output shape or channel offset");
@@ -288,6 +290,7 @@ int fortis_plan_conv3d(fortis_plan* p, int src, int dst, int res, const float* W
 {
     if (!p || p->finalized) return bad("plan is null or already finalized");
     if (C <= 0 || D <= 0 || H <= 0 || Wd <= 0 || F <= 0 || K <= 0 || pad < 0 || !W) return bad("conv3d: bad shape");
+    if (act < 0 || act > FORTIS_ACT_LEAKY) return bad("conv3d: unknown activation");
     const long Do = D + 2 * pad - K + 1, Ho = H + 2 * pad - K + 1, Wo = Wd + 2 * pad - K + 1;
     if (Do <= 0 || Ho <= 0 || Wo <= 0) return bad("conv3d: empty output");
     if (!tensor_ok(p, src, C * D * H * Wd * 4) || !tensor_ok(p, dst, F * Do * Ho * Wo * 4) || src == dst) return bad("conv3d: tensors too small or aliased");

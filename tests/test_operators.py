@@ -85,6 +85,15 @@ def test_silu_stays_with_the_operators_that_compute_it(plan):
     assert plan._L.fortis_plan_linear(plan.handle, x, y, P._p(_f(6, 6)), None, 6, 6, 6, 3, 0.0) == -1
 
 
+def test_convolutions_refuse_activations_that_they_do_not_compute(plan):
+    x, y, w = plan.tensor(4 * 8 * 8 * 8), plan.tensor(4 * 16 * 16 * 16), _f(4, 4, 3, 3, 3)
+    L, h = plan._L, plan.handle
+    for act, rc in ((0, 0), (1, 0), (2, 0), (3, -1), (4, -1), (-1, -1)):
+        assert L.fortis_plan_conv2d(h, x, y, P._p(w), None, None, None, None, None, 1e-5, 4, 8, 8, 4, 3, 3, 1, 1, act, 0.1, 0, 0) == rc
+        assert L.fortis_plan_convt2d(h, x, y, P._p(w), None, 4, 8, 8, 4, 2, 2, 2, 0, 0, act, 0.1, 0, 0) == rc
+        assert L.fortis_plan_conv3d(h, x, y, -1, P._p(w), None, 4, 8, 8, 8, 4, 3, 1, act, 0.1) == rc
+
+
 def test_recurrence_refusals(plan, capfd):
     q, n, c = 4, 3, 5
     x, y, h0, h1, le = plan.tensor(q * n * 2 * c), plan.tensor(q * n * c), plan.tensor(q * c), plan.tensor(q * c), plan.tensor(q)
