@@ -90,7 +90,7 @@ __global__ __launch_bounds__(RC_THREADS) void recurrence_walk_kernel(RecurArgs a
             for (int v = 0; v < V; v++) {
                 float hi, lo;
                 const float gv = g[set][u][v];
-                fortis_sigmoids(gv, hi, lo);
+                fortis_sigmoids<false>(gv, hi, lo);
                 const float f = gv >= 0.f ? hi : lo, b = (gv >= 0.f ? lo : hi) * x[set][u][v];
                 h[v] = fmaf(f, h[v], b);
                 if (!APPLY) F[v] *= f;

@@ -381,6 +381,47 @@ def test_gates_at_their_limits(L, gpu):
     r.p.close()
 
 
+FAR = np.concatenate([np.arange(80, 112, 0.37), [87.0, 87.3, 87.34, 87.5, 104.0, 150.0, 150.5, 1e30]]).astype(np.float32)
+
+
+@pytest.mark.parametrize("n", [1, 13, 400])
+def test_gates_far_out_run_out_through_the_subnormals(L, gpu, n):
+    """f and 1 - f where exp(-|g|) leaves the normal range: off by their bound and half a subnormal step, 2^-150, which the state or the candidate
+    multiplies (one more for the product).  Large states and candidates of zero, and the other way round."""
+    c = FAR.size
+    r = Recur(1, n, c, True, False)
+    for sign, x, h in ((-1, 0.0, 1e30), (1, 1e30, 0.0), (1, 1e30, 0.5)):
+        src = np.full((n, 2 * c), x, np.float32)
+        src[:, :c] = sign * FAR
+        if n > 1:
+            src[1:, :c] = 200.0                      # steps behind the first keep what it left
+        r.h0 = np.full((1, c), h, np.float32)
+        r.p.write(r.hi, r.h0)
+        y, state = r.run(src)
+        ry, rh, ey, _ = r.ref(src=src)
+        assert (np.abs(y - ry) <= ey + 2.0 ** -149 * (abs(x) + abs(h))).all()
+        assert bits_equal(state[0], y[-1])
+    r.p.close()
+
+
+def test_silu_far_out_runs_out_through_the_subnormals(L, gpu):
+    """v / (1 + exp(-v)): the sigmoid is off by 6 u and half a subnormal step, which v multiplies; the products add 2 u and half a step each."""
+    v = np.concatenate([-FAR[:-1], FAR]).astype(np.float32)
+    n = v.size
+    with np.errstate(over="ignore"):
+        ref = v.astype(np.float64) / (1 + np.exp(-v.astype(np.float64)))
+    bound = 10 * R.U32 * np.abs(ref) + 2.0 ** -149 * (np.abs(v.astype(np.float64)) + 2)
+    norm = run_norm(np.random.default_rng(0).standard_normal((3, 1, n)).astype(np.float32), 1, np.zeros(n), v, act="silu")
+    p = P.Plan()
+    x, i, y = p.tensor(5 * 8), p.tensor(5), p.tensor(5 * n)
+    p.linear_adapters(x, y, i, np.zeros((n, 8), np.float32), v, np.zeros((1, 2, 8), np.float32), np.zeros((1, n, 2), np.float32), 5, act="silu")
+    p.finalize(x, y)
+    adapted = p.forward(np.ones((5, 8), np.float32), (5, n))
+    p.close()
+    for got in (norm[:, 0], adapted):
+        assert (np.abs(got - ref) <= bound).all()
+
+
 def test_a_nan_spoils_its_own_channel_from_its_step_on(L, gpu):
     q, n, c = 3, 2500, 20
     r = Recur(q, n, c, True, False)
