@@ -2,6 +2,7 @@
 their formulas in float64 (tests/refops.py, where the error bounds are derived)."""
 import ctypes as C
 import os
+import re
 
 import numpy as np
 import pytest
@@ -236,6 +237,68 @@ def test_nan_and_infinity_stay_with_their_rows_and_adapters(L, gpu, B, K, N, nad
     assert np.isnan(z[1, N // 2]) and not np.isfinite(z[3]).any()
     one, other = a.index == 1, np.arange(N) != N // 2
     within(z[one][:, other], ref[one][:, other], bound[one][:, other])
+
+
+# The forms for many rows, in which rows are placed by atomics and multiplied with other rows' adapters: sizes follow the source's own limit.
+with open(os.path.join(os.path.dirname(P.__file__), "csrc", "adapters.hip")) as _f:
+    _DEFINES = dict(re.findall(r"#define (AD_FEW_ROWS|NARROW_K|NARROW_N|NARROW_RANK) (\d+)", _f.read()))
+FEW, NK, NN, NR = [int(_DEFINES[k]) for k in ("AD_FEW_ROWS", "NARROW_K", "NARROW_N", "NARROW_RANK")]
+SORTED = [(3 * FEW - 7, 64, 2 * NN + 2, 30, 16), (2 * FEW + 452, 2 * NK + 5, 200, 6, 9), (FEW + 1, 556, 40, 3, 40), (FEW + 300, 16, 33, 2, NR + 1)]
+NARROW = [(3 * FEW - 1, 27, NN, 15, 4), (3 * FEW, NK, NN, 8, NR), (FEW + 1, NK - 3, 37, 5, 9), (2 * FEW + 9, 5, 1, 3, 1)]
+
+
+@pytest.mark.parametrize("B,K,N,nadapt,rank", SORTED + NARROW)
+def test_many_rows_in_any_order_with_wild_indices(L, gpu, B, K, N, nadapt, rank):
+    a = Adapted(B, K, N, nadapt, rank, "silu")
+    p = a.plan()
+    y = a.run(p=p)
+    within(y, *a.ref())
+    for seed in (3, 4):
+        order = np.random.default_rng(seed).permutation(B)
+        assert bits_equal(a.run(a.X[order], a.index[order], p=p), y[order])
+    order = np.argsort(a.index, kind="stable")
+    assert bits_equal(a.run(a.X[order], a.index[order], p=p), y[order])
+    wild = a.index.copy()
+    wild[wild < 0] = np.resize([-1, -2 ** 31, nadapt, 2 ** 31 - 1, nadapt + 5], (wild < 0).sum())
+    assert bits_equal(a.run(index=wild, p=p), y)
+    some = np.random.default_rng(5).integers(-1, nadapt, B).astype(np.int32)     # the others' adapters do not matter
+    some[::7] = a.index[::7]
+    assert bits_equal(a.run(index=some, p=p)[::7], y[::7])
+    p.close()
+
+
+@pytest.mark.parametrize("B,K,N,nadapt,rank", SORTED + NARROW)
+def test_many_rows_keep_nan_and_infinity_to_themselves(L, gpu, B, K, N, nadapt, rank):
+    """Rows of X, then an adapter's A and its scale, that are not finite (a U that is not takes the kernels for few rows)."""
+    a = Adapted(B, K, N, nadapt, rank)
+    a.index[:4] = [0, 1, -1, nadapt - 1]
+    y = a.run()
+    X = a.X.copy()
+    X[0, K - 1], X[2, 0], X[3, 0] = np.nan, np.inf, -np.inf
+    X[B - 1, K // 2] = np.nan
+    z = a.run(X)
+    keep = np.ones(B, bool)
+    keep[[0, 2, 3, B - 1]] = False
+    assert np.isnan(z[[0, B - 1]]).all() and not np.isfinite(z[[2, 3]]).any() and bits_equal(z[keep], y[keep])
+    a.A[nadapt - 1, rank - 1, K // 2] = np.inf
+    a.scale[0] = np.nan
+    z = a.run()
+    keep = (a.index != nadapt - 1) & (a.index != 0)
+    assert bits_equal(z[keep], y[keep])
+    assert np.isnan(z[a.index == 0]).all() and not np.isfinite(z[a.index == nadapt - 1]).any()
+
+
+@pytest.mark.parametrize("B,K,N,nadapt,rank", [(FEW + 1, NK, NN, 4, 8), (FEW + 1, 33, 1, 4, NR), (24 * FEW, NK, NN, 8, 8), (5000, 48, 17, 9, 3), (4001, 63, 48, 2, 16),
+                                               (3333, 34, 33, 40, 5), (2050, 62, 64, 3, 13), (70001, 36, 32, 7, 1), (1500, 40, 3, 2, 2), (1500, 41, 16, 2, 11)])
+def test_narrow_layers_of_up_to_64_features(L, gpu, B, K, N, nadapt, rank):
+    assert B > FEW and 32 < K <= NK and N <= NN and rank <= NR
+    kind = ["relu", "leaky", None, "silu"][(B + K + N) % 4]
+    a = Adapted(B, K, N, nadapt, rank, kind, bias=B % 3 != 0, scale=B % 2 != 0, seed=B + K)
+    p = a.plan()
+    within(a.run(p=p), *a.ref())
+    for index in (np.sort(a.index), np.full(B, nadapt - 1, np.int32), np.full(B, -1, np.int32)):
+        within(a.run(index=index, p=p), *a.ref(index=index))
+    p.close()
 
 
 # ---- recurrence ----------------------------------------------------------------------------------------------
