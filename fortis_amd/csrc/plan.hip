@@ -1391,8 +1391,9 @@ void mlp_forward(void* in, void* out)
     const size_t nin = (size_t)h.n_in * h.in_esz, nout = (size_t)h.n_out * h.out_esz;
     fortis_plan* p = g_step.plan;
     bool direct = nin <= 32 * 1024 && nout <= 32 * 1024 && !getenv("FORTIS_NO_ZEROCOPY") && p->in_t != p->out_t;
-    for (size_t t = 0; direct && t < p->view_of.size(); t++)
-        if (p->view_of[t] == p->in_t || p->view_of[t] == p->out_t) direct = false;
+    // (the host memory stands in for one tensor: not where a window of it, or what it is a window of, is another)
+    for (int t = 0; direct && t < (int)p->tbytes.size(); t++)
+        if ((t != p->in_t && overlap(p, t, p->in_t)) || (t != p->out_t && overlap(p, t, p->out_t))) direct = false;
     // a side tensor, a carried state or an output of which rows are left as they were keeps its place on the device
     for (const Exec& e : p->exec) {
         if (leaves_rows(e) && overlap(p, e.dst, p->out_t)) direct = false;

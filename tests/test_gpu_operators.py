@@ -634,6 +634,29 @@ def test_rows_behind_the_lengths_through_the_entries(L, gpu, q):
     p.close()
 
 
+def test_small_steps_whose_input_or_output_is_a_window(L, gpu):
+    """The model's input is the front of a tensor that the plan reads whole, its output the back of one that the plan writes whole: the path
+    without copies cannot stand in for either."""
+    rng = np.random.default_rng(18)
+    X, rest, W = [rng.standard_normal(s).astype(np.float32) for s in ((4, 8), (4, 8), (6, 8))]
+    p = P.Plan()
+    whole, out = p.tensor(64), p.tensor(48)
+    x, y = p.view(whole, 0, 32), p.view(out, 24, 24)
+    p.linear(whole, out, W, None, 8)
+    p.finalize(x, y)
+    L.fortis_h2d(p.ptr(whole) + 128, _vp(rest), rest.nbytes)
+    step.reset()
+    step.bind(p, 32, 24)
+    for k in range(2):
+        got = np.zeros((4, 6), np.float32)
+        step.mlp_forward(X * (k + 1), got)
+        assert np.abs(got - rest @ W.T).max() < 1e-5
+        first = p.read(out, (8, 6))[:4]
+        assert np.abs(first - (k + 1) * (X @ W.T)).max() < 1e-5
+    step.reset()
+    p.close()
+
+
 def test_run_time_extents_of_an_adapted_row_network(L, gpu):
     """fortis_begin re-sizes a batched step of adapted projections and one-position norms, down and up."""
     K, c, N, rows = 27, 32, 3, 500
