@@ -689,7 +689,7 @@ int fortis_plan_finalize(fortis_plan* p, int in_t, int out_t)
                 static int direct_only = -1;
                 if (direct_only < 0) direct_only = getenv("FORTIS_CONV_DIRECT") != 0;
                 if (!direct_only && o.nd == 3 && o.sfac == 2 && i + 1 < ops.size() && ops[i + 1].kind == OP_CONV3D &&
-                    ops[i + 1].src == o.dst && ops[i + 1].KD == 3 && ops[i + 1].pad == 1 && ops[i + 1].F >= 16 && out_t != o.dst) {
+                    ops[i + 1].src == o.dst && ops[i + 1].KD == 3 && ops[i + 1].pad == 1 && ops[i + 1].F >= 16 && !overlap(p, out_t, o.dst)) {
                     bool other = false;
                     for (size_t j = 0; j < ops.size(); j++)
                         if (j != i + 1)

@@ -787,6 +787,22 @@ def test_a_window_of_a_tensor_that_would_be_folded_away(L, gpu):
     p.close()
 
 
+def test_an_output_window_of_an_upsampled_volume_is_written(L, gpu):
+    """upsample -> conv3d folds into one kernel that does not store the volume between them, unless the plan's output is a window of it."""
+    rng = np.random.default_rng(19)
+    Cc, D, F = 4, 6, 16
+    x, w = rng.standard_normal((Cc, D, D, D)).astype(np.float32), rng.standard_normal((F, Cc, 3, 3, 3)).astype(np.float32)
+    p = P.Plan()
+    n = (2 * D) ** 3
+    t, up, y = p.tensor(x.size), p.tensor(Cc * n), p.tensor(F * n)
+    last = p.view(up, (Cc - 1) * n, n)
+    p.upsample(t, up, Cc, D, D, D, 2, 3)
+    p.conv3d(up, y, w, None, Cc, 2 * D, 2 * D, 2 * D, 1)
+    p.finalize(t, last)
+    assert bits_equal(p.forward(x, (2 * D,) * 3), x[-1].repeat(2, 0).repeat(2, 1).repeat(2, 2))
+    p.close()
+
+
 # ---- offsets beyond 32 bits: the same block again and again, results have to repeat to the bit -----------------
 def _repeat(L, ptr, block_bytes, copies):
     done = 1
