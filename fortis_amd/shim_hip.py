@@ -163,6 +163,11 @@ class OpList:
         self.weights.append(np.ascontiguousarray(a, dtype=np.float32))
         return "w%d" % (len(self.weights) - 1)
 
+    @staticmethod
+    def _shape(what, a, *shape):
+        if a is not None and not isinstance(a, str) and np.shape(a) != shape:
+            raise ValueError("%s has shape %r, not %r" % (what, np.shape(a), shape))
+
     # -- the Plan interface
     def tensor(self, nelem, esz=4):
         self.tensors.append(dict(elems=int(nelem), esz=esz))
@@ -223,12 +228,16 @@ class OpList:
         self.ops.append(dict(op="permute", src=src, dst=dst, C=int(C_), S=int(S), to_channels_first=bool(to_channels_first)))
 
     def group_norm(self, src, dst, NB, S, C_, G, gamma=None, beta=None, eps=1e-5, act=None, alpha=0.0, channels_first=False):
+        self._shape("gamma", gamma, C_)
+        self._shape("beta", beta, C_)
         self.ops.append(dict(op="group_norm", src=src, dst=dst, gamma=self._w(gamma), beta=self._w(beta), eps=float(eps), NB=int(NB), S=int(S),
                              C=int(C_), G=int(G), channels_first=bool(channels_first), act=act or "none", alpha=float(alpha)))
 
     def linear_adapters(self, src, dst, index, W, bias, A, U, B, scale=None, act=None, alpha=0.0):
         N, K = np.asarray(W).shape
         nadapt, rank, _ = np.asarray(A).shape
+        for what, a, shape in (("A", A, (nadapt, rank, K)), ("U", U, (nadapt, N, rank)), ("bias", bias, (N,)), ("scale", scale, (nadapt,))):
+            self._shape(what, a, *shape)
         self.ops.append(dict(op="linear_adapters", src=src, dst=dst, index=int(index), w=self._w(W), b=self._w(bias), A=self._w(A), U=self._w(U),
                              scale=self._w(scale), B=int(B), K=int(K), N=int(N), nadapt=int(nadapt), rank=int(rank), act=act or "none",
                              alpha=float(alpha)))

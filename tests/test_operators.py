@@ -248,3 +248,19 @@ def test_generator_writes_the_operators(tmp_path):
         broken["ops"][op][key] = value
         with pytest.raises(ValueError):
             SH.emit_step({}, outline, broken)
+
+
+def test_op_lists_refuse_weights_of_other_shapes():
+    """What a live plan asserts: the generated C hands the sizes of W and A to calls that read the other blobs with them."""
+    o = SH.OpList()
+    x, i, y = o.tensor(54), o.tensor(6), o.tensor(42)
+    ok = dict(src=x, dst=y, index=i, W=_f(7, 9), bias=_f(7), A=_f(3, 2, 9), U=_f(3, 7, 2), B=6, scale=_f(3))
+    for bad in (dict(A=_f(3, 2, 8)), dict(U=_f(3, 2, 7)), dict(U=_f(2, 7, 2)), dict(bias=_f(6)), dict(scale=_f(4))):
+        with pytest.raises(ValueError):
+            o.linear_adapters(**dict(ok, **bad))
+    for bad in (dict(gamma=_f(11)), dict(beta=_f(12, 1))):
+        with pytest.raises(ValueError):
+            o.group_norm(x, y, 2, 2, 12, 3, **bad)
+    assert not o.ops and not o.weights
+    o.linear_adapters(**ok)
+    o.group_norm(x, y, 2, 2, 12, 3, "g0", _f(12))
