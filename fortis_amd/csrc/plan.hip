@@ -368,7 +368,8 @@ int fortis_plan_recurrence(fortis_plan* p, int src, int dst, int h_in, int h_out
             if (t[a] >= 0 && t[b] >= 0 && overlap(p, t[a], t[b]) && !(a == 2 && b == 3 && h_in == h_out)) return bad("recurrence: tensors overlap");
     Op o; o.kind = OP_RECUR; o.src = src; o.dst = dst; o.side = lengths < 0 ? -1 : lengths; o.h_in = h_in < 0 ? -1 : h_in; o.h_out = h_out < 0 ? -1 : h_out;
     o.B = nseq; o.H = len; o.C = ch; o.flag = (time_major ? 1 : 0) | (reverse ? 2 : 0);
-    p->ops.push_back(std::move(o));
+    try { p->ops.push_back(std::move(o)); }
+    catch (const std::bad_alloc&) { return bad("recurrence: out of host memory"); }
     return 0;
 }
 

@@ -3,6 +3,7 @@ buffers a plan gives their side tensors, and what the step generator writes for 
 import ctypes as C
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -264,3 +265,22 @@ def test_op_lists_refuse_weights_of_other_shapes():
     assert not o.ops and not o.weights
     o.linear_adapters(**ok)
     o.group_norm(x, y, 2, 2, 12, 3, "g0", _f(12))
+
+
+def test_recurrence_without_host_memory_is_refused():
+    """In a process of its own whose memory is bounded: the call says so instead of ending the program."""
+    code = """
+import resource
+from fortis_amd import plan as P
+p = P.Plan()
+x, y = p.tensor(2), p.tensor(1)
+call, h = p._L.fortis_plan_recurrence, p.handle
+size = 1024 * int(next(l for l in open("/proc/self/status") if l.startswith("VmSize")).split()[1])
+resource.setrlimit(resource.RLIMIT_AS, (size + (64 << 20),) * 2)
+n = 0
+while n < 1000000 and call(h, x, y, -1, -1, -1, 1, 1, 1, 1, 0) == 0:
+    n += 1
+print("refused", n < 1000000)
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "refused True" in r.stdout and "recurrence: out of host memory" in r.stderr, r
