@@ -10,7 +10,7 @@
 // takes 16 rows at a time from X to Y.
 //
 // Many rows: bound by the matrix pipes.  Rows are sorted by adapter inside windows of AD_WINDOW rows (one launch), H is
-// formed for 32 sorted rows at a time, and the GEMM tile of gemm.hip runs over the sorted rows: a row of A is found through
+// formed for 16 sorted rows at a time, and the GEMM tile of gemm.hip runs over the sorted rows: a row of A is found through
 // the permutation, and behind the k loop each wave adds, per 32 rows and adapter among them, H U_i^T with the H of other
 // adapters' rows as zeros.  Sorted rows leave one or two adapters to a block of 32; rows that were not sorted would leave up to
 // 32.  A window keeps a tile's rows and the rows it writes within a few megabytes of each other.  Sorting places equal
@@ -19,8 +19,12 @@
 
 #define AD_THREADS 256
 #define AD_WINDOW 2048          // rows sorted together; a multiple of the tile's 128
-// Few rows against sorted ones, us at K = N = 768, rank 16: 513 rows with 64 adapters 29 against 62, with 4 adapters 28 against 39;
-// 1024 rows with 64 adapters 49 against 52, with 8 adapters 47 against 41; 2048 rows with 24 adapters 90 against 55.
+// Few rows against sorted ones, us at rank 16, 8 / 64 adapters:
+//   K = N = 256     512 rows 12.5 : 23 / 12.4 : 32      1024 rows 20 : 23 / 19 : 27
+//   K = N = 768     512 rows 25 : 33 / 25 : 39          1024 rows 44 : 34 / 45 : 38
+//   K = N = 2048    256 rows 74 : 73 / 75 : 115         512 rows 140 : 74 / 143 : 95      1024 rows 273 : 97 / 277 : 107
+// The limit holds for K = N = 256.  Wider layers would change over sooner, as W is read again for every 16 rows: between 512 and 1024 rows at
+// 768, at 256 rows at 2048.
 #define AD_FEW_ROWS 1024
 
 static inline long up(long n, long m) { return (n + m - 1) / m * m; }
@@ -189,8 +193,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
 // A wave owns 16 rows: their X as KG operands of four k (k = 16 g + 4 q + c, as above).  Per adapter among the rows: all
 // are multiplied with its A, the products change places through the wave's own piece of LDS into
 // operands of the second product, where those of other adapters' rows are zeros.  Loads of X start before W is brought to LDS.
-// 71040 rows of 27 -> 64 with 15 adapters of rank 4 in bands (26 MB): 12.9 us, 2.0 TB/s, bound by a wave's chain of loads, two products
-// and the way through LDS between them; 32 rows a wave gain 0.3 us there and lose where neighbours' adapters differ, adapter operands
+// 71040 rows of 27 -> 64 with 15 adapters of rank 4 in bands (26 MB): 13.0 us, 2.0 TB/s, bound by a wave's chain of loads, two products
+// and the way through LDS between them, and by a second round: 1110 workgroups, of which 1024 are resident (106 registers); 32 rows a wave gain 0.3 us there and lose where neighbours' adapters differ, adapter operands
 // loaded a block of rows ahead cost 1.6.
 #define NARROW_WAVE_FLOATS(KG, SC) (16 * 20 + ((SC) ? 16 * (16 * (KG) + 4) : 0))
 template <int KG, int NT, bool SC>
@@ -445,7 +449,7 @@ __global__ __launch_bounds__(64 * KS) void adapt_low_sorted_kernel(AdaptDesc d, 
 
 // The GEMM tile over sorted rows.  24576 x 768 -> 768 with 24 adapters of rank 16: 240 us, 126 TFLOP/s of the 149 that a large product
 // reaches (the same layer without adapters 227: what is added is 2.1 % of the multiplications, rows found through the list and
-// written row by row the rest); 4099 x 556 -> 368: 29 us, 390 tiles of 64 x 64 on 256 compute units.
+// written row by row the rest); 4099 x 556 -> 368: 29 us, 390 tiles of 64 x 64 on 256 compute units.  (SC spills 12 vector registers.)
 template <bool SC> struct AdaptRows {
     static constexpr bool kPlain = false, kAnyRow = SC;
     const int *perm, *key;
@@ -620,7 +624,9 @@ static void launch_sorted(const AdaptDesc& d, const float* X, const int* index, 
     int *perm = (int*)ws, *key = perm + Bw;
     float* H = (float*)(key + Bw);
     hipLaunchKernelGGL(adapt_sort_kernel, dim3((unsigned)(Bw / AD_WINDOW)), dim3(1024), (size_t)(d.nadapt + 1 + 16) * 4, s, index, perm, key, B, (int)d.nadapt);
-    // as many waves as leave each the six groups that it loads at once
+    // Waves by K; each loads six groups of 16 at once, and up to 12 groups are left to one wave, 24 to two.  One / two / four / eight waves take, in
+    // all with N = 256, 24 adapters of rank 16, us: K = 96 39 / 42 / 49 / 56, K = 192 53 / 50 / 57 / 67, K = 384 79 / 76 / 74 / 84, K = 768 130 / 126 / 124 / 119
+    // for 24576 rows; K = 96 17.9 / 18.3 / 18.4 / 19.9, K = 192 22.1 / 20.2 / 20.4 / 22.2, K = 384 32 / 28 / 25 / 27, K = 768 52 / 43 / 39 / 36 for 4096.
     const dim3 blocks((unsigned)cdiv(B, LOW_ROWS));
     if (d.p.Ka <= 12 * 16) hipLaunchKernelGGL((adapt_low_sorted_kernel<1, SC>), blocks, dim3(64), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
     else if (d.p.Ka <= 24 * 16) hipLaunchKernelGGL((adapt_low_sorted_kernel<2, SC>), blocks, dim3(128), 0, s, d, X, (const int*)perm, (const int*)key, H, B);

@@ -4,14 +4,16 @@
 //
 // Memory-bound: 8 bytes and about ten operations a value.  Three forms:
 //   lanes    up to 2048 values an instance (512 vectors): 1 to 64 lanes hold it in registers, one read, one write, no barrier.
-//            71040 rows of 64 in heads of 16: 9.1 us, 4.0 TB/s (a copy of as many bytes 5.4 us);
+//            71040 rows of 64 in heads of 16, SiLU: 9.2 us, 3.9 TB/s (a copy of as many bytes 5.4 us), bound by issuing vector instructions:
+//            some 265 for a wave's 256 values, 7.7 us at four cycles each;
 //   block    up to 32768: one workgroup holds an instance (or the neighbouring instances whose channels share 128-byte
 //            lines) in registers, one read, one write.  512 x 8 instances of 16384, channels first: 102 us, 5.2 TB/s;
 //   split    beyond, and where few workgroups would have much each (a compute unit alone moves some 25 GB/s: eight instances of
-//            32768 take 8.3 us in the block form, 7.6 in two launches): one launch sums over chunks of every sample, a second joins
+//            32768 take 8.3 us in the block form, 7.6-7.7 in two launches): one launch sums over chunks of every sample, a second joins
 //            a sample's chunk sums and normalises.  The input is read twice, the second time from the caches as far as they
 //            hold it.  287496 x 64 in 8 groups: 36.2 us, 13 of them the sums (the first read runs at what HBM gives), the rest
-//            the second at 6 TB/s; 65536 x 32: 10.8 us, both launches bound by their start, two barriers and the join.
+//            the second at 6 TB/s; 65536 x 32: 10.8 us, both launches bound by their start and two barriers, the second by the join as well: each of
+//            its 256 workgroups adds up 256 partial sums of eight groups.
 // Sums.  Where the values stay in registers the mean comes first, summed about the instance's first value as a pivot, and the
 // squares of what is left after it second, in float32.  The split form has to take both sums in one read: every thread sums at
 // most 64 values about the first one it meets, and from there on everything is joined in float64 about the instance's first
@@ -746,6 +748,7 @@ template <int V> static void launch_block(const NormArgs& a, NormKind kind, int 
         else if (nv <= 1024 * 4) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 4>), grid, dim3(1024), 0, s, a, total);
         else if (nv <= 1024 * 8) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 8>), grid, dim3(1024), 0, s, a, total);
         if constexpr (V <= 2) if (nv > 1024 * 8 && nv <= 1024 * 16) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 16>), grid, dim3(1024), 0, s, a, total);
+        // (32 single values a thread do not fit in 128 registers: 26 are spilled)
         if constexpr (V == 1) if (nv > 1024 * 16) hipLaunchKernelGGL((norm_block_kernel<V, 1024, 32>), grid, dim3(1024), 0, s, a, total);
         return;
     }

@@ -109,8 +109,8 @@ int  fortis_plan_permute(fortis_plan* p, int src, int dst, long C, long S, int t
  * channels_first, [NB][C][S]: for every sample and every group of C / G neighbouring channels
  *     dst = act(gamma[c] * (src - mean) / sqrt(var + eps) + beta[c])
  * over the group's S * C / G values, var their biased variance.  gamma, beta: host pointers of length C, copied, or NULL
- * (1 and 0).  G has to divide C, C < 2^20; eps >= 0 (with 0 a group of equal values is NaN).  S = 1 normalises rows (one
- * head of C / G features per group).  The mean is kept to twice float32's digits and sums are joined in float64 where a group
+ * (1 and 0).  G has to divide C, C < 2^20; eps >= 0 (with 0 a group of equal values, or of values closer than about 1e-19, is
+ * NaN or infinite).  S = 1 normalises rows (one head of C / G features per group).  The mean is kept to twice float32's digits and sums are joined in float64 where a group
  * does not fit in registers, so a large common offset costs no accuracy.  A value further than about 1e19 from its group's
  * mean (its square leaves float32), a NaN or an infinity spoils its own group (NaN in front of the activation) and no other. */
 int  fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma, const float* beta, float eps,
@@ -120,9 +120,9 @@ int  fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma
  * A [nadapt][rank][K], U [nadapt][N][rank], scale [nadapt] (NULL: 1), W, bias as in fortis_plan_linear: host pointers,
  * copied.  index: a tensor of B int32, read on the device at every pass, rows in any order; an index outside
  * [0, nadapt) means no adapter for that row, and so all rows start (index is filled with -1 at finalize).  1 <= nadapt
- * <= FORTIS_MAX_ADAPTERS, 1 <= rank <= FORTIS_MAX_RANK, B < 2^31, K and N < 2^19.  A row's result depends on that row alone: not on the
- * order of rows, nor on the adapters of the others.  (Values of U that are not finite are kept to their own adapter's rows by a
- * slower kernel.) */
+ * <= FORTIS_MAX_ADAPTERS, 1 <= rank <= FORTIS_MAX_RANK, B < 2^31, K and N < 2^19.  A row's result depends on that row (and on
+ * how many there are, which chooses the kernel), not on the order of rows, nor on the adapters of the others.  (Values of U that
+ * are not finite are kept to their own adapter's rows by a slower kernel.) */
 #define FORTIS_MAX_ADAPTERS 4096
 #define FORTIS_MAX_RANK 256
 int  fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, const float* W, const float* bias,
