@@ -1367,7 +1367,7 @@ void mlp_forward(void* in, void* out)
 {
     if (!bound("mlp_forward")) return;
     const fortis_host_t& h = g_step.h;
-    if (h.verdict == FORTIS_VERDICT_BATCHED)
+    if (h.verdict == FORTIS_VERDICT_BATCHED && h.count > 1)
         for (const Exec& e : g_step.plan->exec)
             if (e.h_out >= 0) {
                 // the other rows would be run again on the inputs of an earlier pass

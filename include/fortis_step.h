@@ -184,7 +184,8 @@ void  mlp_forward_dev(void);                      /* :82-90  capture on call #2,
 void  mlp_download(void* out);                    /* :92 */
 void  mlp_forward(void* in, void* out);           /* :122 (single row, batched build) / :132-133 (whole array) */
 /* (The single row runs as row 0 of the batch, the others on what they held: with the adapter that index[0] names, and refused, a
- * message and `out` as it was, where the plan writes the state of a recurrence, which would move for every row.) */
+ * message and `out` as it was, where the plan writes the state of a recurrence, which would move for every row.  A batch of one
+ * row, after fortis_begin(1) say, is no such case.) */
 /* One symbol, two reference forms: the expanded form takes no arguments (:113-115) and ignores
  * what it is passed; the slice form takes the host's whole in/out arrays (:117-121). */
 void  mlp_forward_batched(void* in, void* out);

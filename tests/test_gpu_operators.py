@@ -700,7 +700,7 @@ def test_run_time_extents_of_a_step_through_time(L, gpu):
     step.reset()
     step.bind(p, rows * K, rows * c, verdict="batched", count=rows)
     state, old, at = np.zeros((rows, c)), np.zeros((rows, c)), p.ptr(st)
-    for n in (300, 40, 40, 300, 2500, 2500, 7):
+    for n in (300, 40, 40, 300, 2500, 2500, 7, 1):
         step.fortis_begin(n)
         if n > len(state):
             assert p.ptr(st) != at
@@ -711,7 +711,7 @@ def test_run_time_extents_of_a_step_through_time(L, gpu):
         if n != 2500:                                # there the lengths that a growth starts with
             lengths[::5] = 0
             L.fortis_h2d(step.fortis_model_tensor(le), _vp(lengths), lengths.nbytes)
-        step.mlp_forward_batched(X, Y)
+        (step.mlp_forward if n == 1 else step.mlp_forward_batched)(X, Y)       # one row is the whole batch then
         g64, _ = R.linear_adapters(X, index, W, None, A, U, None, None, 0)
         old[:n], state[:n], _, _ = R.recurrence(g64, state[:n], lengths, n, 1, c, True, False, old[:n])
         z, _ = R.group_norm(old[:n, None], 2, None, None, 1e-5, "silu", 0, False)
