@@ -606,11 +606,11 @@ long fortis_adapters_workspace(const AdaptDesc& d, long B)
     return up(n, AD_WINDOW) * 8 + n * d.p.Rp * 4;
 }
 template <int ROW>
-static void launch_few(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)
+static void launch_few(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, bool fused, void* ws, hipStream_t s)
 {
     float* H = (float*)ws;
     const dim3 grid((unsigned)(cdiv(B, 16) * cdiv(d.N, 16))), block(64 * FEW_WAVES);
-    if (B * d.p.Rp <= FEW_FUSED) {
+    if (fused) {
         hipLaunchKernelGGL((adapt_few_kernel<ROW, true>), grid, block, 0, s, d, X, index, (const float*)H, Y, B);
         return;
     }
@@ -643,15 +643,16 @@ static void launch_adapters(const AdaptDesc& d, const float* X, const int* index
         else narrow_by_columns<4, SC>(d, X, index, Y, B, s);
         return;
     }
-    const bool few = d.K < 4 || B <= AD_FEW_ROWS || !d.p.finite;         // by all rows: the pieces of a call take one form
+    // by all rows: the pieces of a call take one form
+    const bool few = d.K < 4 || B <= AD_FEW_ROWS || !d.p.finite, fused = B * d.p.Rp <= FEW_FUSED;
     const long piece = few ? few_piece(d) : AD_PIECE;
     for (long r = 0; r < B; r += piece) {
         const long n = B - r < piece ? B - r : piece;
         const float* x = X + r * d.K;
         float* y = Y + r * d.N;
         if (!few) launch_sorted<SC>(d, x, index + r, y, n, ws, s);
-        else if (d.K < 4) launch_few<ROWTINY>(d, x, index + r, y, n, ws, s);
-        else launch_few<SC ? ROWANY : ROW4>(d, x, index + r, y, n, ws, s);
+        else if (d.K < 4) launch_few<ROWTINY>(d, x, index + r, y, n, fused, ws, s);
+        else launch_few<SC ? ROWANY : ROW4>(d, x, index + r, y, n, fused, ws, s);
     }
 }
 void fortis_launch_linear_adapters(const AdaptDesc& d, const float* X, const int* index, float* Y, long B, void* ws, hipStream_t s)

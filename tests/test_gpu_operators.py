@@ -863,6 +863,30 @@ def test_adapters_of_more_rows_than_a_launch_has_work_items(L, gpu, K, N, nadapt
     L.fortis_pool_trim()
 
 
+def test_the_last_piece_of_many_rows_sums_like_the_others(L, gpu):
+    """Two rows beyond a piece: alone they would take the kernel that forms the low-rank rows itself, and round elsewhere."""
+    K, N, rank = 300, 700, 8
+    B = (1 << 22) // 44 * 16 + 2                     # 44 tiles of 16 columns
+    a = Adapted(2, K, N, 3, rank)
+    a.index[:] = 1, 2
+    a.U[0, 0, 0] = np.nan                            # this form at every size
+    p = P.Plan()
+    t, i, o = p.tensor(B * K), p.tensor(B), p.tensor(B * N)
+    p.linear_adapters(t, o, i, a.W, a.bias, a.A, a.U, B, a.scale)
+    p.finalize(t, o)
+    p.write(t, a.X)
+    p.write(i, a.index)
+    _repeat(L, p.ptr(t), 2 * K * 4, B // 2)
+    _repeat(L, p.ptr(i), 2 * 4, B // 2)
+    p.run()
+    first = _block(L, p.ptr(o), (2, N))
+    within(first, *a.ref())
+    for r in (B // 4 * 2, B - 4, B - 2):
+        assert bits_equal(_block(L, p.ptr(o) + r * N * 4, (2, N)), first), r
+    p.close()
+    L.fortis_pool_trim()
+
+
 @pytest.mark.parametrize("NB,S,Cc,G,first", [(1 << 14, 1, 80, 4, False), (6, 20000, 64, 8, False), (6, 20000, 64, 8, True), (512, 64, 32, 2, False)])
 def test_group_norm_beyond_four_gigabytes(L, gpu, NB, S, Cc, G, first):
     rng = np.random.default_rng(3)
