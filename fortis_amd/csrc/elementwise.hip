@@ -54,9 +54,11 @@ __global__ void fill_int_kernel(int* __restrict__ dst, int v, long n)
 }
 void fortis_launch_fill_int(int* dst, int v, long n, hipStream_t s)
 {
-    if (n <= 0) return;
-    hipLaunchKernelGGL(fill_int_kernel, dim3((unsigned)cdiv(n, EW_THREADS)), dim3(EW_THREADS), 0, s, dst, v, n);
-    HIP_OK(hipGetLastError());
+    for (const long piece = 1L << 31; n > 0; n -= piece, dst += piece) {
+        const long m = n < piece ? n : piece;
+        hipLaunchKernelGGL(fill_int_kernel, dim3((unsigned)cdiv(m, EW_THREADS)), dim3(EW_THREADS), 0, s, dst, v, m);
+        HIP_OK(hipGetLastError());
+    }
 }
 void fortis_launch_mask_relu(const float* src, float* dst, long rows, long n, long tail, hipStream_t s)
 {

@@ -993,3 +993,22 @@ def test_states_of_2_to_the_32_values_start_as_zeros(L, gpu):
     assert not _block(L, p.ptr(s) + (q * c - n) * 4, (n,)).any()
     p.close()
     L.fortis_pool_trim()
+
+
+def test_lengths_of_2_to_the_32_sequences_start_as_all_steps(L, gpu):
+    q, n = (1 << 32) + 4096, 1 << 20
+    p = P.Plan()
+    t, o, le = p.tensor(2 * q), p.tensor(q), p.tensor(q)
+    p.recurrence(t, o, q, 1, 1, lengths=le)
+    p.finalize(t, o)
+    for at in (0, (1 << 31) - n // 2, q - n):
+        assert (_block(L, p.ptr(le) + at * 4, (n,)).view(np.int32) == 1).all(), at
+    p.write(t, np.zeros(2 * n, np.float32))
+    _repeat(L, p.ptr(t), 2 * n * 4, q // n)
+    L.fortis_d2d(p.ptr(t) + 8 * (q - n), p.ptr(t), 8 * n)
+    x = np.array([0.0, 3.0], np.float32)             # the last sequence: half of its candidate
+    L.fortis_h2d(p.ptr(t) + 8 * (q - 1), _vp(x), 8)
+    p.run()
+    assert _block(L, p.ptr(o) + 4 * (q - 2), (2,)).tolist() == [0.0, 1.5]
+    p.close()
+    L.fortis_pool_trim()
