@@ -23,8 +23,8 @@
 //   K = N = 256     512 rows 12.5 : 23 / 12.4 : 32      1024 rows 20 : 23 / 19 : 27
 //   K = N = 768     512 rows 25 : 33 / 25 : 39          1024 rows 44 : 34 / 45 : 38
 //   K = N = 2048    256 rows 74 : 73 / 75 : 115         512 rows 140 : 74 / 143 : 95      1024 rows 273 : 97 / 277 : 107
-// The limit holds for K = N = 256.  Wider layers would change over sooner, as W is read again for every 16 rows: between 512 and 1024 rows at
-// 768, at 256 rows at 2048.
+// The limit holds for K = N = 256.  Wider layers would change over sooner, as W is read again for every 16 rows: between 512 and
+// 1024 rows at 768, at 256 rows at 2048.
 #define AD_FEW_ROWS 1024
 
 static inline long up(long n, long m) { return (n + m - 1) / m * m; }
@@ -194,8 +194,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void adapt_few_kernel(AdaptDesc d, 
 // are multiplied with its A, the products change places through the wave's own piece of LDS into
 // operands of the second product, where those of other adapters' rows are zeros.  Loads of X start before W is brought to LDS.
 // 71040 rows of 27 -> 64 with 15 adapters of rank 4 in bands (26 MB): 13.0 us, 2.0 TB/s, bound by a wave's chain of loads, two products
-// and the way through LDS between them, and by a second round: 1110 workgroups, of which 1024 are resident (106 registers); 32 rows a wave gain 0.3 us there and lose where neighbours' adapters differ, adapter operands
-// loaded a block of rows ahead cost 1.6.
+// and the way through LDS between them, and by a second round: 1110 workgroups, of which 1024 are resident (106 registers); 32 rows
+// a wave gain 0.3 us there and lose where neighbours' adapters differ, adapter operands loaded a block of rows ahead cost 1.6.
 #define NARROW_WAVE_FLOATS(KG, SC) (16 * 20 + ((SC) ? 16 * (16 * (KG) + 4) : 0))
 template <int KG, int NT, bool SC>
 __global__ __launch_bounds__(AD_THREADS, 3) void adapt_narrow_kernel(AdaptDesc d, const float* __restrict__ X, const int* __restrict__ index,
@@ -590,8 +590,8 @@ static void launch_adapt_gemm(const AdaptDesc& d, const float* X, float* Y, long
     hipLaunchKernelGGL((adapt_gemm_kernel<SC>), dim3((unsigned)grid), dim3(GM_THREADS), shmem, s, X, d.W, Y, B, d.N, d.K, sc, epi, ext);
 }
 
-// A launch has to stay under 2^32 work-items, and both forms have many to a row: rows beyond AD_PIECE, or beyond few_piece(), go through
-// them in pieces, one behind the other through the same scratch.
+// A launch has to stay under 2^32 work-items, and both forms have many to a row: more than AD_PIECE rows, or few_piece(), go through
+// in pieces, one behind the other through the same scratch.
 #define AD_PIECE (1L << 26)     // sorted rows: up to 32 work-items each; a multiple of AD_WINDOW
 // few rows: 16 work-items a row and rank, 512 a tile of 16 rows and 16 columns; a multiple of 16 and at least 2048 (N < 2^19)
 static long few_piece(const AdaptDesc& d)
@@ -624,9 +624,10 @@ static void launch_sorted(const AdaptDesc& d, const float* X, const int* index, 
     int *perm = (int*)ws, *key = perm + Bw;
     float* H = (float*)(key + Bw);
     hipLaunchKernelGGL(adapt_sort_kernel, dim3((unsigned)(Bw / AD_WINDOW)), dim3(1024), (size_t)(d.nadapt + 1 + 16) * 4, s, index, perm, key, B, (int)d.nadapt);
-    // Waves by K; each loads six groups of 16 at once, and up to 12 groups are left to one wave, 24 to two.  One / two / four / eight waves take, in
-    // all with N = 256, 24 adapters of rank 16, us: K = 96 39 / 42 / 49 / 56, K = 192 53 / 50 / 57 / 67, K = 384 79 / 76 / 74 / 84, K = 768 130 / 126 / 124 / 119
-    // for 24576 rows; K = 96 17.9 / 18.3 / 18.4 / 19.9, K = 192 22.1 / 20.2 / 20.4 / 22.2, K = 384 32 / 28 / 25 / 27, K = 768 52 / 43 / 39 / 36 for 4096.
+    // Waves by K: each loads six groups of 16 at once; up to 12 groups are left to one wave, 24 to two.  One / two / four / eight
+    // waves take, in all, with N = 256 and 24 adapters of rank 16, us:
+    //   24576 rows   K = 96  39 / 42 / 49 / 56          K = 192  53 / 50 / 57 / 67          K = 384  79 / 76 / 74 / 84   K = 768  130 / 126 / 124 / 119
+    //   4096 rows    K = 96  17.9 / 18.3 / 18.4 / 19.9  K = 192  22.1 / 20.2 / 20.4 / 22.2  K = 384  32 / 28 / 25 / 27   K = 768  52 / 43 / 39 / 36
     const dim3 blocks((unsigned)cdiv(B, LOW_ROWS));
     if (d.p.Ka <= 12 * 16) hipLaunchKernelGGL((adapt_low_sorted_kernel<1, SC>), blocks, dim3(64), 0, s, d, X, (const int*)perm, (const int*)key, H, B);
     else if (d.p.Ka <= 24 * 16) hipLaunchKernelGGL((adapt_low_sorted_kernel<2, SC>), blocks, dim3(128), 0, s, d, X, (const int*)perm, (const int*)key, H, B);

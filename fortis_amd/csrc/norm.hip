@@ -664,8 +664,8 @@ static SplitShape split_shape(const NormDesc& d)
     h.V = d.C % 4 == 0 && d.C <= 4 * GS_THREADS ? 4 : cg % 4 == 0 ? 4 : cg % 2 == 0 ? 2 : 1;
     const long fit = GS_THREADS * h.V;                  // channels a workgroup spans
     h.gs = (int)(d.C <= fit ? d.G : cg <= fit ? fit / cg : 1);
-    // The second launch keeps a group's statistics per entry of an array of GS_THREADS: narrower groups than V channels would be up to four
-    // times as many.  (V divides C and GS_THREADS cg: every slice is whole vectors.)
+    // The second launch keeps its groups' statistics in an array of GS_THREADS; with groups narrower than V channels there would be up
+    // to four times as many.  (V divides C and GS_THREADS cg: every slice is whole vectors.)
     if (h.gs > GS_THREADS) h.gs = GS_THREADS;
     h.slices = (int)cdiv(d.G, h.gs);
     h.blocks = (int)cdiv(cg, fit);

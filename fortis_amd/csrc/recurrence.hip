@@ -4,7 +4,7 @@
 //
 // Memory-bound: 12 bytes and about 25 instructions a value.  A lane owns one or two neighbouring channels of a sequence and
 // walks its steps with two batches of loads in flight.  4736 columns of up to 15 levels of 64 channels: 7.9 us, 3.8 TB/s (with 8 to 15 steps the
-// one round's last loads are its own first batch again and the rest's travel behind it); one step: 3.3 us, the launch; 4736 x 60 x 64: 43.5 us, 5.0 TB/s.
+// one round's last loads are its own first batch again and the rest's travel behind it); one step: 3.3 us, the launch; 4736 x 60 x 64: 43.7 us, 5.0 TB/s.
 // Where sequences and channels alone do not fill the chip, every sequence is cut into K chunks: a step is the map
 // h -> f h + b, maps compose to (F, B), so one launch composes every chunk's steps, one wave per sequence and channel scans the
 // K compositions and leaves the state in front of every chunk, and a third launch walks the chunks from there: 8 bytes a value
@@ -175,9 +175,10 @@ static RecurShape recur_shape(const RecurDesc& d)
     r.chunks = 1;
     // One chunk costs 70 ns a step, two more launches 5 us: 64, 128 and 512 steps of 1 x 64 channels take 6.0, 10.1 and 36.7 us in one chunk,
     // 7.9, 8.1 and 8.9 in chunks of 8, 8.8, 8.9 and 9.7 of 16, 10.8, 11.0 and 11.6 of 32.  Where the scan has many to go through longer chunks
-    // win: 4 x 4096 steps of 64 take 15.1, 12.2 and 12.8 us.  One walk against chunks at 100 / 200 / 1000 steps, us: 4096 values 9.8 : 9.5 / 17 : 10.8 /
-    // 87 : 20, 16384 10.5 : 14.6 / 19 : 17.7 / 88 : 51, 32768 11.4 : 19.7 / 21 : 31 / 92 : 93, 65472 13.8 : 36.5 / 23 : 53 / 174 : 242: from about 16384
-    // values on the limit on their number asks for chunks too soon where the sequences are short, and from 32768 on always.
+    // win: 4 x 4096 steps of 64 take 15.1, 12.2 and 12.8 us.  One walk against chunks, us at 100, 200 and 1000 steps:
+    //   4096 values   9.8 : 9.5   17 : 10.8   87 : 20          32768 values  11.4 : 19.7   21 : 31   92 : 93
+    //   16384 values  10.5 : 14.6   19 : 17.7   88 : 51        65472 values  13.8 : 36.5   23 : 53   174 : 242
+    // From about 16384 values on the limit on their number asks for chunks too soon where the sequences are short, from 32768 on always.
     const long least = d.len > 512 ? 16 : 8;
     if (d.len > 96 && values / r.V < full / 2) r.chunks = cdiv(full, values / r.V);
     if (r.chunks > cdiv(d.len, least)) r.chunks = cdiv(d.len, least);

@@ -110,9 +110,10 @@ int  fortis_plan_permute(fortis_plan* p, int src, int dst, long C, long S, int t
  *     dst = act(gamma[c] * (src - mean) / sqrt(var + eps) + beta[c])
  * over the group's S * C / G values, var their biased variance.  gamma, beta: host pointers of length C, copied, or NULL
  * (1 and 0).  G has to divide C, C < 2^20; eps >= 0 (with 0 a group of equal values, or of values closer than about 1e-19, is
- * NaN or infinite).  S = 1 normalises rows (one head of C / G features per group).  The mean is kept to twice float32's digits and sums are joined in float64 where a group
- * does not fit in registers, so a large common offset costs no accuracy.  A value further than about 1e19 from its group's
- * mean (its square leaves float32), a NaN or an infinity spoils its own group (NaN in front of the activation) and no other. */
+ * NaN or infinite).  S = 1 normalises rows (one head of C / G features per group).  The mean is kept to twice float32's digits
+ * and sums are joined in float64 where a group does not fit in registers, so a large common offset costs no accuracy.  A value
+ * further than about 1e19 from its group's mean (its square leaves float32), a NaN or an infinity spoils its own group (NaN in
+ * front of the activation) and no other. */
 int  fortis_plan_group_norm(fortis_plan* p, int src, int dst, const float* gamma, const float* beta, float eps,
                             long NB, long S, long C, long G, int channels_first, int act, float alpha);
 /* fortis_plan_linear with a low-rank adapter chosen per row:
@@ -139,8 +140,8 @@ int  fortis_plan_linear_adapters(fortis_plan* p, int src, int dst, int index, co
  * lengths: tensor of nseq int32, -1: all `len`; sequence s takes steps 0 .. lengths[s] - 1 only (values are clamped to
  * [0, len]; filled with len at finalize).  Rows of dst at and behind a sequence's length are left as they were, zeros until
  * something else writes them (with lengths, dst never shares its memory with other tensors; an entry that copies the output
- * to the host copies those rows too), a sequence without steps hands its state on unchanged.  Long sequences are cut into chunks whose maps are composed first: an infinite value
- * in front of a chunk may come out as NaN behind it. */
+ * to the host copies those rows too), a sequence without steps hands its state on unchanged.  Long sequences are cut into
+ * chunks whose maps are composed first: an infinite value in front of a chunk may come out as NaN behind it. */
 int  fortis_plan_recurrence(fortis_plan* p, int src, int dst, int h_in, int h_out, int lengths, long nseq, long len,
                             long ch, int time_major, int reverse);
 
